@@ -137,6 +137,101 @@ AWQ_API int awq_gemm_f16_silu_mul(const void* x, int64_t ldx, const int32_t* qwe
                                   void* stream);
 
 /*
+ * ---- Between the products: rotary positions, a paged 4-bit key/value cache, attention ----
+ * No counterpart in the reference as such: it keeps an fp16 cache (inference/kv_cache.py),
+ * rotates with one position per token (kernels/rope.py) and attends over fp16 keys and
+ * values (kernels/flash_attention.py).  All entry points enqueue kernels on `stream`,
+ * allocate nothing and do not synchronize; fp16 data, int32 lengths and pages.
+ *
+ * awq_rope_axes: positions int64 or int32 [axes][tokens] (row stride axis_stride), inv_freq
+ * fp32 [half], half = sum of sections[axes] (host array; 1 to 4 axes).  Frequency i turns
+ * the channels (i, i + half) of every head of token t by positions[axis(i)][t] *
+ * inv_freq[i].  axis(i): the section that holds i; with `interleaved`, a = i % axes while
+ * i / axes < sections[a], else axis 0.  Channels from 2 half up are copied.  q or k may have
+ * no heads.  out may be q or k itself with the same strides (in place); it must not overlap
+ * the inputs in any other way.
+ */
+AWQ_API int awq_rope_axes(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                          int64_t q_heads, const void* k, int64_t k_token_stride,
+                          int64_t k_head_stride, int64_t k_heads, int64_t tokens,
+                          int64_t head_dim, const void* positions, int positions_are_64bit,
+                          int64_t axis_stride, const float* inv_freq, const int32_t* sections,
+                          int axes, int interleaved, void* out_q, int64_t out_q_token_stride,
+                          int64_t out_q_head_stride, void* out_k, int64_t out_k_token_stride,
+                          int64_t out_k_head_stride, void* stream);
+
+/*
+ * The cache: num_pages pages of page_size tokens (a power of two, 16 to 1024), each
+ * awq_kv4_page_bytes bytes, contiguous, 16-byte aligned; head_dim 64 or 128.  Keys and
+ * values are held per token and kv head in groups of group_size channels (32, 64 or 128):
+ * codes c in 0..15, fp16 scale s and minimum m, value c s + m, with m = min x, s =
+ * fp16((max x - m) / 15), c = clamp(round((x - m) / s), 0, 15) (ties to even, c = 0 where s
+ * = 0); a group with a NaN or an infinity reads back as NaN.  The byte layout is in
+ * csrc/awq_kv4.cuh.  A slot is page * page_size + offset.
+ *
+ * awq_kv4_append quantizes k and v ([tokens][kv_heads][head_dim], last dimension dense) into
+ * their slots.  A negative slot is skipped; one past the cache is skipped and sets status
+ * bit 2 (awq_device_status).  The slots of one call must differ.  awq_kv4_gather reads slots
+ * back as dense fp16 [tokens][kv_heads][head_dim] (a negative or bad slot as zeros).
+ */
+AWQ_API size_t awq_kv4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t group_size,
+                                  int64_t page_size);
+AWQ_API int awq_kv4_append(const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                           const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                           const int64_t* slots, int64_t tokens, void* cache, int64_t num_pages,
+                           int64_t kv_heads, int64_t head_dim, int64_t group_size,
+                           int64_t page_size, void* stream);
+AWQ_API int awq_kv4_gather(const void* cache, int64_t num_pages, int64_t kv_heads,
+                           int64_t head_dim, int64_t group_size, int64_t page_size,
+                           const int64_t* slots, int64_t tokens, void* out_k, void* out_v,
+                           void* stream);
+
+/*
+ * One step's page bookkeeping on the device, for up to 8192 requests.  State, updated in
+ * place: block_table [requests][max_blocks] (row stride table_stride; unused entries -1),
+ * held [requests] (pages each request holds), the stack free_pages[0 .. *free_count).
+ * Input: kv_lens [requests] tokens cached before the step, new_tokens [requests], and reset
+ * [requests] (or null): a request whose row is reset first gives all its pages back.  Then
+ * each request takes the pages that kv_lens + new_tokens needs beyond those it holds, from
+ * the top of the stack, requests in order; released pages go onto the stack so that the
+ * first one is taken first, and entries at or above *free_count are -1.  Output: slots
+ * [max_tokens] and positions [max_tokens] of the new tokens, request after request (-1 and 0
+ * behind the last), cu_q [requests + 1] (first token of each request), new_lens [requests].
+ * *step_status: 0; n > 0 when the stack is n pages short; -1 when a length, held or count is
+ * out of range (negative, more than max_blocks pages, more than max_tokens tokens).  A
+ * refused step changes no state and gives slots -1, cu_q 0 and new_lens = kv_lens.
+ */
+AWQ_API int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64_t max_blocks,
+                               int32_t* held, int32_t* free_pages, int64_t free_capacity,
+                               int32_t* free_count, const int32_t* kv_lens,
+                               const int32_t* new_tokens, const uint8_t* reset,
+                               int64_t requests, int64_t page_size, int64_t* slots,
+                               int32_t* positions, int64_t max_tokens, int32_t* cu_q,
+                               int32_t* new_lens, int32_t* step_status, void* stream);
+
+/*
+ * Causal attention over the cache.  q [tokens][q_heads][head_dim] (query head h reads kv
+ * head h / (q_heads / kv_heads)); request r has kv_lens[r] cached tokens, found through
+ * block_table, and the query rows cu_q[r] .. cu_q[r + 1] (cu_q null: row r alone), which are
+ * its last tokens: row i of n sees tokens 0 .. kv_lens[r] - n + i.  A row that sees no token
+ * gives zeros.  Rows of out behind cu_q[requests] are left as they are.  max_q: most query
+ * rows of a request (a hint for the choice of kernel).  Tokens in a page outside
+ * 0 .. num_pages - 1 are not seen, kv_lens is clipped to the table, a request whose cu_q is
+ * not ascending within 0 .. tokens is left out; each sets status bit 2.  The workspace
+ * (awq_kv4_attention_workspace_bytes, 16-byte aligned) needs no initialisation; calls that
+ * may overlap on the GPU need different ones.
+ */
+AWQ_API size_t awq_kv4_attention_workspace_bytes(int64_t head_dim);
+AWQ_API int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                              int64_t tokens, int64_t q_heads, const void* cache,
+                              int64_t num_pages, int64_t kv_heads, int64_t head_dim,
+                              int64_t group_size, int64_t page_size, const int32_t* block_table,
+                              int64_t table_stride, int64_t max_blocks, const int32_t* kv_lens,
+                              const int32_t* cu_q, int64_t requests, int64_t max_q, float scale,
+                              void* out, int64_t out_token_stride, int64_t out_head_stride,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * awq_gemm_f16 for callers that cannot allocate device memory: same inputs and
  * output, no workspace argument.  This entry point has no counterpart in the
  * reference.  It serves hosts that forbid allocation on the path where the product

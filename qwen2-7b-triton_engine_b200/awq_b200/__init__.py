@@ -8,6 +8,10 @@ Public functions
   dequant(qweight, qzeros, scales, group_size)      -> fp16 [K, N]   (bit-exact W)
   gemm(x2d, qweight, qzeros, scales, group_size, path) -> fp16 [M, N]
   device_status(stream)                              -> status bits of the kernels
+  rope_axes, KV4Cache, kv4_pages_step, kv4_append, kv4_gather, kv4_attention
+                                                     the operators between the products
+                                                     (layer.py): rotary positions, a paged
+                                                     4-bit key/value cache, attention
 The reference-facing drop-in, ``kernels.awq_gemm.awq_gemm_forward``, is built on
 ``gemm``.
 
@@ -30,8 +34,11 @@ import torch
 from . import _lib
 from ._lib import (AWQ_PATH_AUTO, AWQ_PATH_DECODE, AWQ_PATH_TC, AWQ_PATH_TS, AwqError,  # noqa: F401
                    LIB_PATH)
+from .layer import (KV4Cache, kv4_append, kv4_attention, kv4_gather, kv4_pages_step,  # noqa: F401
+                    rope_axes)
 
 __all__ = ["dequant", "gemm", "gemm_silu_mul", "gemm_allreduce", "TPComm", "device_status", "workspace_for", "AwqError",
+           "KV4Cache", "rope_axes", "kv4_pages_step", "kv4_append", "kv4_gather", "kv4_attention",
            "AWQ_PATH_AUTO", "AWQ_PATH_DECODE", "AWQ_PATH_TC", "AWQ_PATH_TS", "LIB_PATH"]
 
 _ws_lock = threading.Lock()

@@ -57,6 +57,18 @@ SIGNATURES = {
     "awq_gemm_silu_mul_workspace_bytes": ([_I64, _I64, _I64, _I64], _SZ),
     "awq_gemm_f16_silu_mul": ([_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _SZ,
                                _P], _INT),
+    "awq_rope_axes": ([_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _INT, _I64, _P,
+                       _P, _INT, _INT, _P, _I64, _I64, _P, _I64, _I64, _P], _INT),
+    "awq_kv4_page_bytes": ([_I64, _I64, _I64, _I64], _SZ),
+    "awq_kv4_append": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64,
+                        _I64, _P], _INT),
+    "awq_kv4_gather": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P], _INT),
+    "awq_kv4_pages_step": ([_P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _P,
+                            _I64, _P, _P, _P, _P], _INT),
+    "awq_kv4_attention_workspace_bytes": ([_I64], _SZ),
+    "awq_kv4_attention": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P,
+                           _I64, _I64, _P, _P, _I64, _I64, ctypes.c_float, _P, _I64, _I64, _P,
+                           _SZ, _P], _INT),
 }
 
 AWQ_IPC_HANDLE_BYTES = 64

@@ -95,6 +95,15 @@ int check_weights(const int32_t* qweight, const int32_t* qzeros, const void* sca
 
 }  // namespace
 
+int awq::device_context(int* num_sms, int** status) {
+  DeviceInfo* d = nullptr;
+  const int rc = device_info(&d);
+  if (rc) return rc;
+  *num_sms = d->num_sms;
+  *status = d->status;
+  return AWQ_OK;
+}
+
 int awq::set_last_error(int code, const char* msg) {
   g_last_error = msg;
   return code;

@@ -166,6 +166,72 @@ int ts_tokens(int64_t M);
 int ts_splits(int64_t M, int64_t N, int64_t K, int num_sms);
 size_t ts_workspace_bytes(int64_t M, int64_t N, int64_t K, int num_sms);
 
+// ---- paged 4-bit key/value cache (awq_kv4_cache.cu, awq_kv4_attn.cu) -------------------
+struct Kv4Shape {
+  int64_t num_pages;
+  int heads, dim, group, page;   // kv heads, head dim, channels per scale, tokens per page
+};
+constexpr int kKv4MaxRows = 8192;     // requests of one call
+cudaError_t launch_kv4_append(const Kv4Shape& c, const void* k, int64_t k_ts, int64_t k_hs,
+                              const void* v, int64_t v_ts, int64_t v_hs, const int64_t* slots,
+                              int64_t T, void* cache, int num_sms, int* dev_status,
+                              cudaStream_t stream);
+cudaError_t launch_kv4_gather(const Kv4Shape& c, const void* cache, const int64_t* slots, int64_t T,
+                              void* out_k, void* out_v, int num_sms, int* dev_status,
+                              cudaStream_t stream);
+struct Kv4PagesCall {
+  int32_t* table;
+  int64_t table_rs;
+  int32_t *held, *free_pages, *free_count;
+  const int32_t *lens, *new_tokens;
+  const uint8_t* reset;
+  int64_t* slots;
+  int32_t *positions, *cu_q, *new_lens, *status;
+  int64_t max_tokens;
+  int rows, width, capacity, page;
+};
+cudaError_t launch_kv4_pages(const Kv4PagesCall& c, cudaStream_t stream);
+
+struct Kv4AttnCall {
+  Kv4Shape cache;
+  const void* data;
+  const void* q;
+  int64_t q_ts, q_hs;
+  void* out;
+  int64_t o_ts, o_hs;
+  const int32_t* table;
+  int64_t table_rs;
+  const int32_t* lens;
+  const int32_t* cu_q;           // null: one query token per request
+  int64_t tokens;                // rows of q
+  int rows, width, q_heads, max_q;
+  float scale;
+  void* workspace;
+};
+size_t kv4_attention_workspace(int head_dim, int num_sms);
+cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
+                                 cudaStream_t stream);
+
+// ---- rotary positions with several axes (awq_rope.cu) -----------------------------------
+constexpr int kRopeMaxAxes = 4;
+struct RopeCall {
+  const void *q, *k;
+  int64_t q_ts, q_hs, k_ts, k_hs;
+  void *out_q, *out_k;
+  int64_t oq_ts, oq_hs, ok_ts, ok_hs;
+  const void* positions;         // int64 or int32 [axes][T]
+  int pos_is_64;
+  int64_t pos_as;                // axis stride, elements
+  const float* inv_freq;         // [half]
+  int64_t T;
+  int q_heads, k_heads, dim, half, axes, interleaved;
+  int sections[kRopeMaxAxes];
+};
+cudaError_t launch_rope(const RopeCall& c, int num_sms, cudaStream_t stream);
+
+// SM count and status word of the current device (awq_capi.cu); an AWQ_* code.
+int device_context(int* num_sms, int** status);
+
 // Receive-buffer layout of a tensor-parallel communicator (see ArArgs).
 inline size_t tp_data_offset() { return 256; }
 inline size_t tp_buffer_bytes(int world, int max_tiles) {

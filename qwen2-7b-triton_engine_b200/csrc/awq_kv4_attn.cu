@@ -1,0 +1,739 @@
+// awq_kv4_attn.cu -- attention over the paged 4-bit key/value cache.
+//
+// Query row (i, h) of a request with L cached tokens and n query tokens sees the tokens
+// t <= L - n + i:  o = sum_t softmax_t(scale q . k_t) v_t,  k_t = c s + m per channel group.
+// Nothing is dequantized: with integer codes c,
+//   scale q . k_t = scale sum_G ( s_tG (q_G . c_tG) + m_tG sum(q_G) )
+//   o_G = ( sum_t (p_t s_tG) c_tG + sum_t p_t m_tG ) / sum_t p_t
+// so the tensor cores multiply fp16 queries, and fp16 weights p s, with the raw codes (fp16
+// subnormals, one AND per two codes), and scales and minima are applied per token in fp32.
+// The softmax reference M runs over log2(p s) rather than log2(p), so that the fp16 weights
+// stay below 2^8 and near the top of the range whatever the size of the value scales; sums,
+// statistics and accumulators are fp32.
+//
+// Operand order: scores are computed transposed (tokens are the MMA's 16 rows, the query
+// rows of a kv head its 8 columns), as are the outputs (channels x query rows), so seven
+// query heads of a group waste one column in eight instead of nine rows in sixteen.
+//
+// Work split (kv4_attn_kernel): the (request, kv head, 8 NT query rows) items are cut into
+// tiles of 32 tokens, and the linear list of all tiles is dealt evenly to all warps of one
+// CTA per SM; ragged batches balance to within a tile.  A warp streams its tiles through
+// its own ring of bulk copies (no CTA barrier in the loop).  Items that cross warps are
+// joined in the CTA at its end; items that cross CTAs by kv4_merge_kernel, in CTA order, so
+// results do not depend on timing.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "awq_common.cuh"
+#include "awq_internal.h"
+#include "awq_kv4.cuh"
+#include "awq_sm100.cuh"
+
+namespace awq {
+
+namespace {
+
+constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kv4::kBlockTokens;
+constexpr int kPrefixEntries = 1024;     // prefix sums held in shared memory
+constexpr int kDescInts = 8;
+
+struct AttnArgs {
+  const uint8_t* cache;
+  const __half* q;
+  __half* out;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu_q;
+  int64_t q_ts, q_hs, o_ts, o_hs, table_rs;
+  int64_t num_pages;
+  int64_t tokens;
+  float* part;        // [ctas][2] slots of items that cross CTAs
+  float* warp_part;   // [ctas][warps] slots of items that cross warps, not a warp's last
+  int* desc;          // [ctas][kDescInts]
+  int* status;
+  float scale_log2;
+  int R, width, page_shift, kv_heads, G;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+// 2^x of the softmax: 2 ulp, results below 2^-126 are 0 (they are below 2^-100 of the sum).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+template <int D_, int GROUP_, int NT_, int WARPS_>
+struct Geo {
+  static constexpr int D = D_, GROUP = GROUP_, NT = NT_, WARPS = WARPS_;
+  static constexpr int NG = D / GROUP, W = D / 32, ROWS = 8 * NT;
+  static constexpr int BLK = kv4::block_bytes(D, GROUP), TILE = kTileBlocks * BLK;
+  static constexpr int BUDGET = 227 * 1024 - (kPrefixEntries + 1) * 4 - 4096;
+  static constexpr int FIT = BUDGET / (WARPS * TILE);
+  static constexpr int STAGES = FIT < 6 ? FIT : 6;
+  static constexpr int SLOT = ROWS * (D + 2);          // floats: O [ROWS][D], M, l
+  static constexpr int OFF_PRE = WARPS * STAGES * TILE;
+  static constexpr int OFF_BAR = OFF_PRE + (kPrefixEntries + 8) * 4 / 16 * 16;
+  static constexpr int OFF_META = OFF_BAR + WARPS * STAGES * 8;
+  static constexpr int OFF_ENT = (OFF_META + WARPS * STAGES * 4 + 15) / 16 * 16;
+  static constexpr int SMEM = OFF_ENT + WARPS * 2 * 40;
+  static_assert(STAGES >= 2 && SLOT * 4 <= STAGES * TILE && SMEM <= 227 * 1024, "shared memory");
+};
+
+// One request as the work split sees it.
+struct Req {
+  int L, n, q0, tiles, nrt;
+};
+template <int ROWS>
+__device__ __forceinline__ Req request(const AttnArgs& a, int r) {
+  Req x;
+  const int cap = (int)min((long long)a.width << a.page_shift, 0x7fffff00LL);
+  const int len = a.lens[r];
+  x.L = min(max(len, 0), cap);
+  if (len != x.L) atomicOr(a.status, kDevErrShape);
+  if (a.cu_q) {
+    const int b = a.cu_q[r], e = a.cu_q[r + 1];
+    const bool ok = b >= 0 && e >= b && e <= a.tokens;
+    if (!ok) atomicOr(a.status, kDevErrShape);
+    x.q0 = ok ? b : 0;
+    x.n = ok ? e - b : 0;
+  } else {
+    x.q0 = r;
+    x.n = 1;
+  }
+  x.tiles = max(1, (x.L + kTileTokens - 1) / kTileTokens);
+  x.nrt = (x.n * a.G + ROWS - 1) / ROWS;
+  return x;
+}
+
+// A position in the list of tiles: request, kv head, tile of query rows, tile of tokens.
+struct Cursor {
+  Req x;
+  int r, h, rt, tile;
+  int vis;      // tokens the last query row of the row tile sees
+
+  template <int ROWS>
+  __device__ void set_vis(const AttnArgs& a) {
+    const int last = min(x.n - 1, ((rt + 1) * ROWS - 1) / a.G);
+    vis = max(0, x.L - x.n + last + 1);
+  }
+  template <int ROWS>
+  __device__ void locate(const AttnArgs& a, const int* pre, int entries, int shift, int u) {
+    int lo = 0, hi = entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= u) lo = mid; else hi = mid;
+    }
+    int rem = u - pre[lo];
+    r = lo << shift;
+    for (;;) {
+      x = request<ROWS>(a, r);
+      const int units = a.kv_heads * x.nrt * x.tiles;
+      if (rem < units || r + 1 >= a.R) break;
+      rem -= units;
+      ++r;
+    }
+    const int item = rem / x.tiles;
+    tile = rem - item * x.tiles;
+    h = item / x.nrt;
+    rt = item - h * x.nrt;
+    set_vis<ROWS>(a);
+  }
+  template <int ROWS>
+  __device__ void next_item(const AttnArgs& a) {
+    tile = 0;
+    if (++rt == x.nrt) {
+      rt = 0;
+      if (++h == a.kv_heads) {
+        h = 0;
+        do {
+          if (++r >= a.R) return;
+          x = request<ROWS>(a, r);
+        } while (x.nrt == 0);
+      }
+    }
+    set_vis<ROWS>(a);
+  }
+};
+
+struct Entry {          // a part of an item, for the join at the CTA's end
+  int ib, ie;           // the item's tiles in the list
+  int q0, row0, rows, h;
+  const float* ptr;     // slot, or null
+  long long pad;
+};
+static_assert(sizeof(Entry) == 40, "entry size");
+
+template <class G_>
+__global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnArgs a) {
+  constexpr int D = G_::D, NG = G_::NG, W = G_::W, NT = G_::NT, ROWS = G_::ROWS;
+  constexpr int WARPS = G_::WARPS, STAGES = G_::STAGES, BLK = G_::BLK, TILE = G_::TILE;
+  constexpr int GW = W / NG;                           // words (32 channels) per group
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t sbase = sm100::smem_u32(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32, g = lane / 4, t = lane & 3;
+  int* pre = reinterpret_cast<int*>(smem + G_::OFF_PRE);
+  int* meta = reinterpret_cast<int*>(smem + G_::OFF_META) + warp * STAGES;
+  Entry* ent = reinterpret_cast<Entry*>(smem + G_::OFF_ENT);
+  const uint32_t ring = sbase + warp * STAGES * TILE;
+  const uint32_t bar0 = sbase + G_::OFF_BAR + warp * STAGES * 8;
+  __shared__ int wsum[WARPS];
+  __shared__ int s_total;
+
+  if (lane == 0) {
+    for (int s = 0; s < STAGES; ++s) sm100::mbar_init(bar0 + 8 * s, 1);
+    sm100::fence_mbar_init();
+    ent[2 * warp].ptr = ent[2 * warp + 1].ptr = nullptr;
+  }
+
+  // ---- prefix sums of the requests' tiles (1 << shift requests per entry) ---------------
+  int shift = 0;
+  while ((a.R >> shift) + 1 > kPrefixEntries) ++shift;
+  const int entries = (a.R + (1 << shift) - 1) >> shift;
+  if (tid == 0) s_total = 0;
+  __syncthreads();
+  for (int e0 = 0; e0 < entries; e0 += WARPS * 32) {
+    const int e = e0 + tid;
+    int v = 0;
+    if (e < entries)
+      for (int r = e << shift; r < min(a.R, (e + 1) << shift); ++r) {
+        const Req x = request<ROWS>(a, r);
+        v += a.kv_heads * x.nrt * x.tiles;
+      }
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int nb = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += nb;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int before = s_total;
+    for (int w = 0; w < warp; ++w) before += wsum[w];
+    if (e < entries) pre[e] = before + inc - v;
+    __syncthreads();
+    if (tid == WARPS * 32 - 1) s_total = before + inc;
+    __syncthreads();
+  }
+  const int U = s_total;
+  const int ctas = min((int)gridDim.x, (U + WARPS - 1) / WARPS);
+  const int cta = blockIdx.x;
+  if (cta >= ctas) {
+    if (tid == 0) a.desc[cta * kDescInts] = 0;
+    return;
+  }
+  const long long Wt = (long long)ctas * WARPS;
+  auto first_unit = [&](long long w) { return (int)((long long)U * w / Wt); };
+  const int u0 = first_unit((long long)cta * WARPS + warp);
+  const int u1 = first_unit((long long)cta * WARPS + warp + 1);
+
+  if (u0 < u1) {
+    // ---- loads: lane 0 issues one bulk copy per block or per run of blocks in a page -----
+    Cursor lc = {};
+    lc.locate<ROWS>(a, pre, entries, shift, u0);
+    Cursor cc = lc;
+    const int bpp_shift = a.page_shift - 4;
+    auto page_of = [&](const Cursor& c, int b) -> int {   // page of block b of the tile
+      const int blk = c.tile * kTileBlocks + b;
+      if (blk * kv4::kBlockTokens >= c.vis) return -1;
+      return a.table[c.r * a.table_rs + (blk >> bpp_shift)];
+    };
+    int pid0 = page_of(lc, 0), pid1 = page_of(lc, 1);
+    int issued = u0;
+    auto issue = [&]() {
+      const int s = (issued - u0) % STAGES;
+      if (lane == 0) {
+        const int blk = lc.tile * kTileBlocks, nb = min(kTileBlocks, (lc.vis - blk * 16 + 15) / 16);
+        const int m = (1 << (a.page_shift - 4)) - 1;
+        const bool ok0 = nb > 0 && (unsigned long long)(long long)pid0 < (unsigned long long)a.num_pages;
+        const bool ok1 = nb > 1 && (unsigned long long)(long long)pid1 < (unsigned long long)a.num_pages;
+        if ((nb > 0 && !ok0) || (nb > 1 && !ok1)) atomicOr(a.status, kDevErrShape);
+        meta[s] = (int)ok0 | (int)ok1 << 1;
+        sm100::mbar_arrive_expect_tx(bar0 + 8 * s, ((int)ok0 + (int)ok1) * BLK);
+        const uint32_t dst = ring + s * TILE;
+        if (ok0)
+          bulk_load(dst, a.cache + ((((int64_t)pid0 * a.kv_heads + lc.h) << bpp_shift) + (blk & m)) * BLK,
+                    BLK, bar0 + 8 * s);
+        if (ok1)
+          bulk_load(dst + BLK,
+                    a.cache + ((((int64_t)pid1 * a.kv_heads + lc.h) << bpp_shift) + ((blk + 1) & m)) * BLK,
+                    BLK, bar0 + 8 * s);
+      }
+      ++issued;
+      if (issued < u1) {
+        if (++lc.tile == lc.x.tiles) lc.next_item<ROWS>(a);
+        pid0 = page_of(lc, 0), pid1 = page_of(lc, 1);
+      }
+    };
+    for (int s = 0; s < STAGES && issued < u1; ++s) issue();
+
+    bool dead = false;                                  // a wait ran out: stop working
+    int u = u0;
+    while (u < u1) {
+      // ---- one item, or this warp's part of it ----------------------------------------
+      const int rows = cc.x.n * a.G, row0 = cc.rt * ROWS;
+      const int ib = u - cc.tile, ie = ib + cc.x.tiles, ue = min(u1, ie);
+      uint32_t qa[NT][W][2], qb[NT][W][2];              // B operands: even / odd nibbles
+      float qs[NT][NG][2];                              // scale * sum of q over the group
+      int lim[NT][2];                                   // last visible token of the columns
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int row = row0 + nt * 8 + g;
+        const bool in = row < rows;
+        const __half* qp = a.q + (in ? (int64_t)(cc.x.q0 + row / a.G) * a.q_ts +
+                                           (int64_t)(cc.h * a.G + row % a.G) * a.q_hs
+                                     : 0);
+        float sum[NG] = {};
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (in) v = *reinterpret_cast<const uint4*>(qp + 8 * (4 * j + t));
+          qa[nt][j][0] = __byte_perm(v.x, v.z, 0x5410);  // channels 0, 4
+          qb[nt][j][0] = __byte_perm(v.x, v.z, 0x7632);  // 1, 5
+          qa[nt][j][1] = __byte_perm(v.y, v.w, 0x5410);  // 2, 6
+          qb[nt][j][1] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
+          const float2 f0 = __half22float2(u32_as_h2(v.x)), f1 = __half22float2(u32_as_h2(v.y));
+          const float2 f2 = __half22float2(u32_as_h2(v.z)), f3 = __half22float2(u32_as_h2(v.w));
+          sum[j / GW] += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+        }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+          sum[k] *= a.scale_log2;
+          qs[nt][k][0] = __shfl_sync(0xffffffffu, sum[k], 8 * t);
+          qs[nt][k][1] = __shfl_sync(0xffffffffu, sum[k], 8 * t + 4);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          lim[nt][c] = cc.x.L - cc.x.n + (row0 + nt * 8 + 2 * t + c) / a.G;
+      }
+      const int lim_all = cc.x.L - cc.x.n + row0 / a.G;  // every row sees tokens up to here
+      const float ksc = a.scale_log2 * 16777216.0f;      // codes enter the MMA times 2^-24
+      float O[NT][2 * W][4] = {}, M[NT][2], l[NT][2] = {}, pm[NT][NG][2] = {};
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) M[nt][0] = M[nt][1] = -CUDART_INF_F;
+
+      for (; u < ue; ++u) {
+        const int s = (u - u0) % STAGES;
+        if (!dead) {                                     // one verdict for the whole warp
+          const bool got = sm100::mbar_wait_bounded(bar0 + 8 * s, ((u - u0) / STAGES) & 1, a.status);
+          dead = __any_sync(0xffffffffu, !got);
+        }
+        const int tok0 = cc.tile * kTileTokens;
+        const int ok = dead ? 0 : *(volatile int*)(meta + s);
+        ++cc.tile;
+        if (ok) {
+          const uint32_t st = ring + s * TILE;
+          float x[NT][2][4];                             // [block][token g / g + 8, column]
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t kp = st + b * BLK + g * (D / 2) + t * (4 * W);
+            uint32_t k0[W], k1[W];
+            if constexpr (W == 4) {
+              const uint4 v0 = sm100::ld_shared_v4(kp), v1 = sm100::ld_shared_v4(kp + 8 * (D / 2));
+              k0[0] = v0.x, k0[1] = v0.y, k0[2] = v0.z, k0[3] = v0.w;
+              k1[0] = v1.x, k1[1] = v1.y, k1[2] = v1.z, k1[3] = v1.w;
+            } else {
+              const uint2 v0 = sm100::ld_shared_v2(kp), v1 = sm100::ld_shared_v2(kp + 8 * (D / 2));
+              k0[0] = v0.x, k0[1] = v0.y, k1[0] = v1.x, k1[1] = v1.y;
+            }
+            const uint32_t pp = st + b * BLK + kv4::off_kp(D) + g * (4 * NG);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const float2 p0 = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 4 * k)));
+              const float2 p1 = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 8 * 4 * NG + 4 * k)));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float ea[4] = {}, od[4] = {};
+#pragma unroll
+                for (int j = k * GW; j < (k + 1) * GW; ++j) {
+                  const uint32_t s0 = k0[j] >> 8, s1 = k1[j] >> 8;
+                  mma16816(ea, k0[j] & kLoMask, k1[j] & kLoMask, s0 & kLoMask, s1 & kLoMask,
+                           qa[nt][j][0], qa[nt][j][1]);
+                  mma16816(od, k0[j] & kHiMask, k1[j] & kHiMask, s0 & kHiMask, s1 & kHiMask,
+                           qb[nt][j][0], qb[nt][j][1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const float2 p = i < 2 ? p0 : p1;
+                  const float dot = fmaf(od[i], 0.0625f, ea[i]) * ksc;
+                  const float v = fmaf(dot, p.x, p.y * qs[nt][k][i & 1]);
+                  x[nt][b][i] = k == 0 ? v : x[nt][b][i] + v;
+                }
+              }
+            }
+          }
+          // tokens past a row's limit, or in a page the table does not name, are not seen
+          if (tok0 + kTileTokens - 1 > lim_all || ok != 3) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (tok0 + b * 16 + g + (i / 2) * 8 > lim[nt][i & 1] || !((ok >> b) & 1))
+                    x[nt][b][i] = -CUDART_INF_F;
+          }
+          // value scales and minima; the softmax reference follows x + log2(largest scale)
+          float2 vp[2][2][NG];
+          float ls[2][2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t pp = st + b * BLK + kv4::off_vp(D, G_::GROUP) + (g + 8 * e) * (4 * NG);
+              float big = 5.9604645e-8f;                 // 2^-24, fp16's least scale
+#pragma unroll
+              for (int k = 0; k < NG; ++k) {
+                vp[b][e][k] = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 4 * k)));
+                big = fmaxf(big, vp[b][e][k].x);
+              }
+              ls[b][e] = __log2f(big);
+            }
+          bool up = false;
+          float nm[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float m = fmaxf(fmaxf(x[nt][0][c] + ls[0][0], x[nt][0][2 + c] + ls[0][1]),
+                              fmaxf(x[nt][1][c] + ls[1][0], x[nt][1][2 + c] + ls[1][1]));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              nm[nt][c] = m;
+              up |= m > M[nt][c] + 8.0f;
+            }
+          // the reference moves only when it is more than 2^8 behind (the fp16 weights then
+          // reach 2^8 at most); -inf + 8 = -inf, so the first visible token sets it
+          if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float f[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                const float m = fmaxf(M[nt][c], nm[nt][c]);
+                f[c] = M[nt][c] == m ? 1.0f : ex2(M[nt][c] - m);
+                M[nt][c] = m;
+                l[nt][c] *= f[c];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) pm[nt][k][c] *= f[c];
+              }
+#pragma unroll
+              for (int i = 0; i < 2 * W; ++i) {
+                O[nt][i][0] *= f[0], O[nt][i][1] *= f[1];
+                O[nt][i][2] *= f[0], O[nt][i][3] *= f[1];
+              }
+            }
+          }
+          uint32_t wb[NT][2][NG][2];                     // B operands: weights p s per group
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float p[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  p[c] = ex2(x[nt][b][2 * e + c] - (M[nt][c] == -CUDART_INF_F ? 0.f : M[nt][c]));
+                  l[nt][c] += p[c];
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                  // an unseen token's scale and minimum may be anything: no 0 * NaN
+                  float w[2];
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    const bool seen = p[c] != 0.f;
+                    w[c] = seen ? p[c] * vp[b][e][k].x : 0.f;
+                    pm[nt][k][c] += seen ? p[c] * vp[b][e][k].y : 0.f;
+                  }
+                  wb[nt][b][k][e] = movmatrix(h2_as_u32(__floats2half2_rn(w[0], w[1])));
+                }
+              }
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t vq = st + b * BLK + kv4::off_v(D) + t * D + g * (4 * W);
+            uint32_t v0[W], v1[W];
+            if constexpr (W == 4) {
+              const uint4 y0 = sm100::ld_shared_v4(vq), y1 = sm100::ld_shared_v4(vq + 4 * D);
+              v0[0] = y0.x, v0[1] = y0.y, v0[2] = y0.z, v0[3] = y0.w;
+              v1[0] = y1.x, v1[1] = y1.y, v1[2] = y1.z, v1[3] = y1.w;
+            } else {
+              const uint2 y0 = sm100::ld_shared_v2(vq), y1 = sm100::ld_shared_v2(vq + 4 * D);
+              v0[0] = y0.x, v0[1] = y0.y, v1[0] = y1.x, v1[1] = y1.y;
+            }
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              const uint32_t s0 = v0[i] >> 8, s1 = v1[i] >> 8;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816(O[nt][2 * i], v0[i] & kLoMask, s0 & kLoMask, v1[i] & kLoMask, s1 & kLoMask,
+                         wb[nt][b][i / GW][0], wb[nt][b][i / GW][1]);
+                mma16816(O[nt][2 * i + 1], v0[i] & kHiMask, s0 & kHiMask, v1[i] & kHiMask,
+                         s1 & kHiMask, wb[nt][b][i / GW][0], wb[nt][b][i / GW][1]);
+              }
+            }
+          }
+        }
+        __syncwarp();                                    // the stage is read: refill it
+        if (issued < u1 && !dead) issue();
+      }
+
+      // ---- the item's (part's) result ---------------------------------------------------
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) {
+            l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) pm[nt][k][c] += __shfl_xor_sync(0xffffffffu, pm[nt][k][c], o);
+          }
+        }
+      const bool whole = ib >= u0 && ie <= u1;
+      float* slot = nullptr;
+      if (!whole) {
+        slot = ue == u1 ? reinterpret_cast<float*>(smem + warp * STAGES * TILE)
+                        : a.warp_part + (size_t)(cta * WARPS + warp) * G_::SLOT;
+        __syncwarp();
+        if (lane == 0) {
+          Entry& e = ent[2 * warp + (ue == u1)];
+          e.ib = ib, e.ie = ie, e.q0 = cc.x.q0, e.row0 = row0, e.rows = rows, e.h = cc.h;
+          e.ptr = slot;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int col = nt * 8 + 2 * t + c, row = row0 + col;
+          const float inv = l[nt][c] == 0.f ? 0.f : 1.0f / l[nt][c];
+          __half* op = nullptr;
+          if (whole && row < rows)
+            op = a.out + (int64_t)(cc.x.q0 + row / a.G) * a.o_ts + (int64_t)(cc.h * a.G + row % a.G) * a.o_hs;
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const float m = pm[nt][i / GW][c];
+            const float4 v = make_float4(fmaf(O[nt][2 * i][c], 16777216.f, m),
+                                         fmaf(O[nt][2 * i + 1][c], 1048576.f, m),
+                                         fmaf(O[nt][2 * i][2 + c], 16777216.f, m),
+                                         fmaf(O[nt][2 * i + 1][2 + c], 1048576.f, m));
+            if (slot) {
+              *reinterpret_cast<float4*>(slot + col * D + 32 * i + 4 * g) = v;
+            } else if (op) {
+              *reinterpret_cast<uint2*>(op + 32 * i + 4 * g) =
+                  make_uint2(h2_as_u32(__floats2half2_rn(v.x * inv, v.y * inv)),
+                             h2_as_u32(__floats2half2_rn(v.z * inv, v.w * inv)));
+            }
+          }
+          if (slot && g == 0) {
+            slot[ROWS * D + col] = M[nt][c];
+            slot[ROWS * D + ROWS + col] = l[nt][c];
+          }
+        }
+      if (u < u1) cc.next_item<ROWS>(a);
+    }
+    if (dead)                                            // copies in flight land before the exit
+      for (int k = u0 > issued - STAGES ? u0 : issued - STAGES; k < issued; ++k)
+        sm100::mbar_wait_bounded(bar0 + 8 * ((k - u0) % STAGES), ((k - u0) / STAGES) & 1, nullptr, 100000000ull);
+  }
+  sm100::grid_launch_dependents();
+  __syncthreads();
+
+  // ---- join the items that cross this CTA's warps, in order ------------------------------
+  const int cs = first_unit((long long)cta * WARPS), ce = first_unit((long long)(cta + 1) * WARPS);
+  int span = 0;
+  Entry head = {};
+  int i = 0;
+  while (i < 2 * WARPS) {
+    if (!ent[i].ptr) { ++i; continue; }
+    int j = i + 1, last = i;
+    for (; j < 2 * WARPS; ++j) {
+      if (!ent[j].ptr) continue;
+      if (ent[j].ib != ent[i].ib) break;
+      last = j;
+    }
+    const Entry e0 = ent[i];
+    const bool done = e0.ib >= cs && e0.ie <= ce;
+    float* slot = a.part + (size_t)(cta * 2 + (e0.ib < cs ? 0 : 1)) * G_::SLOT;
+    if (!done && e0.ib >= cs) {                          // the item starts here and goes on
+      span = (int)(((long long)e0.ie * Wt - 1) / U / WARPS) - cta + 1;
+      head = e0;
+    }
+    for (int idx = tid; idx < ROWS * (D / 4); idx += WARPS * 32) {
+      const int col = idx / (D / 4), ch = (idx - col * (D / 4)) * 4, row = e0.row0 + col;
+      float m = -CUDART_INF_F;
+      for (int k = i; k <= last; ++k)
+        if (ent[k].ptr) m = fmaxf(m, ent[k].ptr[ROWS * D + col]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+      for (int k = i; k <= last; ++k) {
+        const float* p = ent[k].ptr;
+        if (!p) continue;
+        const float mk = p[ROWS * D + col], f = mk == m ? 1.0f : ex2(mk - m);
+        const float4 v = *reinterpret_cast<const float4*>(p + col * D + ch);
+        l = fmaf(f, p[ROWS * D + ROWS + col], l);
+        o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y);
+        o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+      }
+      if (done) {
+        if (row < e0.rows) {
+          const float inv = l == 0.f ? 0.f : 1.0f / l;
+          __half* op = a.out + (int64_t)(e0.q0 + row / a.G) * a.o_ts + (int64_t)(e0.h * a.G + row % a.G) * a.o_hs;
+          *reinterpret_cast<uint2*>(op + ch) = make_uint2(h2_as_u32(__floats2half2_rn(o.x * inv, o.y * inv)),
+                                                          h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
+        }
+      } else {
+        *reinterpret_cast<float4*>(slot + col * D + ch) = o;
+        if (ch == 0) slot[ROWS * D + col] = m, slot[ROWS * D + ROWS + col] = l;
+      }
+    }
+    i = j;
+  }
+  if (tid == 0) {
+    int* d = a.desc + cta * kDescInts;
+    d[0] = span, d[1] = head.q0, d[2] = head.row0, d[3] = head.rows, d[4] = head.h;
+  }
+}
+
+// Joins an item that crosses CTAs: block (c, col) sums column col of the item that starts in
+// CTA c, over the slots of CTAs c .. c + span - 1, in four (eight) interleaved groups.
+template <int D>
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const int rows_per_item) {
+  constexpr int LANES = D / 4, GROUPS = 128 / LANES;
+  __shared__ float s_m[4], s_l[GROUPS];
+  __shared__ float4 s_o[GROUPS][LANES];
+  sm100::grid_dependency_wait();
+  const int cta = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
+  const int* d = a.desc + cta * kDescInts;
+  const int span = d[0];
+  if (span == 0) return;
+  const int row = d[2] + col;
+  if (row >= d[3]) return;
+  const size_t slot = (size_t)rows_per_item * (D + 2);
+  // CTA c's item is in its slot 1, the following CTAs' parts of it in their slots 0
+  auto part = [&](int k) { return a.part + (size_t)((cta + k) * 2 + (k == 0)) * slot; };
+  float m = -CUDART_INF_F;
+  for (int k = tid; k < span; k += 128) m = fmaxf(m, part(k)[rows_per_item * D + col]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) s_m[tid / 32] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const int grp = tid / LANES, ch = tid % LANES;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int k = grp; k < span; k += GROUPS) {
+    const float* p = part(k);
+    const float mk = p[rows_per_item * D + col], f = mk == m ? 1.0f : ex2(mk - m);
+    const float4 v = *reinterpret_cast<const float4*>(p + col * D + 4 * ch);
+    l = fmaf(f, p[rows_per_item * D + rows_per_item + col], l);
+    o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
+  }
+  s_o[grp][ch] = o;
+  if (ch == 0) s_l[grp] = l;
+  __syncthreads();
+  if (grp != 0) return;
+  l = s_l[0];
+#pragma unroll
+  for (int k = 1; k < GROUPS; ++k) {
+    const float4 v = s_o[k][ch];
+    o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
+    l += s_l[k];
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  __half* op = a.out + (int64_t)(d[1] + row / a.G) * a.o_ts + (int64_t)(d[4] * a.G + row % a.G) * a.o_hs;
+  *reinterpret_cast<uint2*>(op + 4 * ch) = make_uint2(h2_as_u32(__floats2half2_rn(o.x * inv, o.y * inv)),
+                                                      h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
+}
+
+constexpr int kWarps1 = 16, kWarps2 = 8;
+
+template <class G_>
+cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
+  static PerDeviceOnce attr_once;
+  const cudaError_t attr = attr_once.run([] {
+    return cudaFuncSetAttribute(kv4_attn_kernel<G_>, cudaFuncAttributeMaxDynamicSharedMemorySize, G_::SMEM);
+  });
+  if (attr != cudaSuccess) return attr;
+  a.warp_part = a.part + (size_t)num_sms * 2 * G_::SLOT;
+  kv4_attn_kernel<G_><<<num_sms, G_::WARPS * 32, G_::SMEM, stream>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms, G_::ROWS, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<G_::D>, a, (int)G_::ROWS);
+}
+
+template <int D, int GROUP>
+cudaError_t launch_rows(const AttnArgs& a, int max_rows, int num_sms, cudaStream_t stream) {
+  if (max_rows <= 8) return launch_geo<Geo<D, GROUP, 1, kWarps1>>(a, num_sms, stream);
+  return launch_geo<Geo<D, GROUP, 2, kWarps2>>(a, num_sms, stream);
+}
+
+}  // namespace
+
+size_t kv4_attention_workspace(int head_dim, int num_sms) {
+  // descriptors, 2 slots per CTA and one per warp: 8 x 16 warps and 16 x 8 warps alike
+  const size_t slots = (size_t)num_sms * (2 * 16 + kWarps1 * 8);
+  return (size_t)num_sms * kDescInts * 4 + slots * (head_dim + 2) * 4;
+}
+
+cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
+                                 cudaStream_t stream) {
+  AttnArgs a = {};
+  a.cache = static_cast<const uint8_t*>(c.data);
+  a.q = static_cast<const __half*>(c.q), a.out = static_cast<__half*>(c.out);
+  a.table = c.table, a.lens = c.lens, a.cu_q = c.cu_q;
+  a.q_ts = c.q_ts, a.q_hs = c.q_hs, a.o_ts = c.o_ts, a.o_hs = c.o_hs, a.table_rs = c.table_rs;
+  a.num_pages = c.cache.num_pages, a.tokens = c.tokens;
+  a.desc = static_cast<int*>(c.workspace);
+  a.part = reinterpret_cast<float*>(a.desc + num_sms * kDescInts);
+  a.status = dev_status;
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.R = c.rows, a.width = c.width, a.kv_heads = c.cache.heads, a.G = c.q_heads / c.cache.heads;
+  a.page_shift = 0;
+  while ((1 << a.page_shift) < c.cache.page) ++a.page_shift;
+  const int max_rows = c.max_q * a.G;
+  const int D = c.cache.dim, g = c.cache.group;
+  if (D == 64 && g == 32) return launch_rows<64, 32>(a, max_rows, num_sms, stream);
+  if (D == 64 && g == 64) return launch_rows<64, 64>(a, max_rows, num_sms, stream);
+  if (D == 128 && g == 32) return launch_rows<128, 32>(a, max_rows, num_sms, stream);
+  if (D == 128 && g == 64) return launch_rows<128, 64>(a, max_rows, num_sms, stream);
+  if (D == 128 && g == 128) return launch_rows<128, 128>(a, max_rows, num_sms, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace awq

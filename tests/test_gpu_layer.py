@@ -1,0 +1,406 @@
+"""GPU: rotary positions, the paged 4-bit cache, page bookkeeping and attention over the
+cache, each against its 64-bit restatement (oracle/layer.py).
+
+Tolerances.  u16 = 2^-11 is half a step of fp16, u32 = 2^-24 of fp32.
+* cache codes, scales, minima, slots, tables: equal.
+* gather: fp16(c s + m) of an fp32 fma: |err| <= (u16 + u32) |x| + 2^-25 (half the least
+  fp16 step).
+* rope: fp32 sine / cosine within 4 u32 + the reduced angle's 2^-24 of a half turn (pi u32),
+  two products and a sum: |err| <= 12 u32 (|a| + |b|), then u16 |y| + 2^-25.
+* attention: let A = |scale| sum |q| (15 s + |m|) bound the terms of a score.  The fp32 score
+  sums D products and folds s and m in, each rounded at the size of A: off by e = (D + 8) u32
+  A, plus the hardware exponential's 2 ulp (2^-22).  A softmax weight p_t is then off by
+  d_t = e_t + sum_t p_t e_t (its own error and the sum's), relative.  The weights p s are
+  rounded to fp16: u16 relative, or, below fp16's normal range, half a subnormal step 2^-25
+  of the softmax reference, which is at most the largest p s.  Hence
+  |err| <= sum_t (p_t ((u16 + d_t) s c + d_t |m|) + 2^-25 max(p s) 15) + u16 |o| + 2^-25.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import awq_b200
+from oracle import layer as L
+
+pytestmark = pytest.mark.gpu
+U16, U32, TINY = 2.0 ** -11, 2.0 ** -24, 2.0 ** -25
+
+
+@pytest.fixture(autouse=True)
+def _status(cuda):
+    awq_b200.device_status()
+    yield
+
+
+def dev(x, dtype=None):
+    t = torch.as_tensor(np.asarray(x), device="cuda")
+    return t if dtype is None else t.to(dtype)
+
+
+# ---- rope ---------------------------------------------------------------------------------
+ROPE = [  # T, q heads, k heads, D, sections, interleaved
+    (1, 28, 4, 128, (64,), False), (5, 28, 4, 128, (16, 24, 24), False),
+    (3, 7, 1, 128, (16, 24, 24), True), (2, 4, 2, 64, (5, 7, 3), True),
+    (7, 3, 1, 80, (8, 16, 8), False), (4, 1, 0, 16, (1,), False), (2, 2, 2, 512, (100, 156), False),
+]
+
+
+@pytest.mark.parametrize("T,H,Hk,D,sections,inter", ROPE)
+@pytest.mark.parametrize("pos_type", [torch.int64, torch.int32])
+def test_rope(cuda, T, H, Hk, D, sections, inter, pos_type):
+    rng = np.random.default_rng(T * 100 + D)
+    half = sum(sections)
+    x = rng.standard_normal((T, H + Hk, D)).astype(np.float16)
+    pos = rng.integers(0, 2_000_000, (len(sections), T))
+    pos[:, 0] = [0, -5, 2 ** 31 - 1, 1][:len(sections)]
+    inv = (1e6 ** (-np.arange(half) / half)).astype(np.float32)
+    fused = dev(x)
+    q, k = fused[:, :H], fused[:, H:]
+    oq, ok = awq_b200.rope_axes(q, k, dev(pos).to(pos_type), dev(inv), sections, inter)
+    ref = L.rope(x, pos, inv, sections, inter)
+    size = np.abs(x.astype(np.float64))
+    size[..., :2 * half] += np.roll(size[..., :2 * half], half, -1)
+    got = torch.cat([oq, ok], 1).double().cpu().numpy()
+    assert (np.abs(got - ref) <= 12 * U32 * size + U16 * np.abs(ref) + TINY).all()
+    assert torch.equal(fused, dev(x))
+    # in place, on the views
+    awq_b200.rope_axes(q, k, dev(pos).to(pos_type), dev(inv), sections, inter, out_q=q, out_k=k)
+    assert torch.equal(q, oq) and torch.equal(k, ok)
+
+
+def test_rope_unaligned_and_transposed(cuda):
+    """An odd start and a head-major layout take the scalar path, with the same values."""
+    rng = np.random.default_rng(3)
+    x = rng.standard_normal((6, 4, 64)).astype(np.float16)
+    pos = dev(rng.integers(0, 5000, (1, 6)))
+    inv = dev((1e4 ** (-np.arange(32) / 32)).astype(np.float32))
+    want = awq_b200.rope_axes(dev(x), dev(x[:, :2]), pos, inv, (32,))
+    buf = torch.zeros(6 * 4 * 64 + 1, dtype=torch.float16, device="cuda")
+    odd = buf[1:].view(6, 4, 64)
+    odd.copy_(dev(x))
+    heads = dev(x).transpose(0, 1).contiguous().transpose(0, 1)
+    for q in (odd, heads):
+        got = awq_b200.rope_axes(q, q[:, :2], pos[0], inv, (32,))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- append and gather --------------------------------------------------------------------
+def sample(rng, T, H, D):
+    """Rows with wide, narrow, constant, subnormal and large groups."""
+    x = rng.standard_normal((T, H, D)) * np.exp(rng.uniform(-3, 3, (T, H, 1)))
+    x[rng.random((T, H)) < 0.1] = 0.25
+    x[rng.random((T, H)) < 0.1] *= 2.0 ** -22
+    x[rng.random((T, H)) < 0.1] *= 1000
+    tie = rng.random((T, H)) < 0.2                    # quotients that fall on ties
+    x[tie] = rng.integers(0, 31, (int(tie.sum()), D)) / 2.0 - 3
+    return x.clip(-65504, 65504).astype(np.float16)
+
+
+CACHES = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)]
+
+
+@pytest.mark.parametrize("D,group", CACHES)
+@pytest.mark.parametrize("page,H,T", [(16, 1, 1), (16, 4, 37), (64, 3, 50), (1024, 2, 9)])
+def test_append_bytes_and_gather(cuda, D, group, page, H, T):
+    rng = np.random.default_rng(D + group + T)
+    k, v = sample(rng, T, H, D), sample(rng, T, H, D)
+    pages = T // page + 3
+    slots = rng.permutation(pages * page)[:T]
+    cache = awq_b200.KV4Cache.allocate(pages, H, D, page, group)
+    cache.data.random_(0, 256)
+    before = cache.data.cpu().numpy()
+    want = before.copy()
+    for t in range(T):
+        L.write_slot(want, int(slots[t]), k[t], v[t], page, group)
+    fused = dev(np.concatenate([k, v], 1))            # strided views
+    awq_b200.kv4_append(fused[:, :H], fused[:, H:], dev(slots), cache)
+    bad = np.argwhere(cache.data.cpu().numpy() != want)     # and nothing else changed
+    assert len(bad) == 0, bad[:8].tolist()
+    ask = np.concatenate([slots, [-1]])
+    gk, gv = (x.double().cpu().numpy() for x in awq_b200.kv4_gather(cache, dev(ask)))
+    rk, rv = L.read_slots(want, slots, D, page, group)
+    for got, ref in ((gk, rk), (gv, rv)):
+        assert (np.abs(got[:T] - ref) <= (U16 + U32) * np.abs(ref) + TINY).all()
+        assert (got[T] == 0).all()
+    assert awq_b200.device_status() == 0
+
+
+def test_append_skips_and_non_finite(cuda):
+    rng = np.random.default_rng(5)
+    k, v = (rng.standard_normal((4, 2, 64)).astype(np.float16) for _ in range(2))
+    k[0, 0, 3], v[0, 1, 40], k[3, 1, 0] = np.nan, np.inf, -np.inf
+    cache = awq_b200.KV4Cache.allocate(2, 2, 64, 16, 32)
+    awq_b200.kv4_append(dev(k), dev(v), dev(np.array([31, -1, -7, 0])), cache)
+    want = np.zeros(tuple(cache.data.shape), np.uint8)
+    for t, s in ((0, 31), (3, 0)):
+        L.write_slot(want, s, k[t], v[t], 16, 32)
+    gk, gv = awq_b200.kv4_gather(cache, dev(np.array([31, 0])))
+    rk, rv = L.read_slots(want, [31, 0], 64, 16, 32)
+    for got, ref in ((gk, rk), (gv, rv)):
+        got = got.double().cpu().numpy()
+        assert np.array_equal(np.isnan(got), np.isnan(ref))
+        ok = ~np.isnan(ref)
+        assert (np.abs(got - ref)[ok] <= (U16 + U32) * np.abs(ref)[ok] + TINY).all()
+    assert np.isnan(gk[0, 0, :32].cpu().numpy()).all() and not np.isnan(gk[0, 0, 32:].cpu().numpy()).any()
+    assert awq_b200.device_status() == 0
+    awq_b200.kv4_append(dev(k), dev(v), dev(np.array([-1, 32, -1, 10 ** 12])), cache)
+    again = awq_b200.kv4_gather(cache, dev(np.array([31, 0])))
+    assert torch.equal(again[0].view(torch.int16), gk.view(torch.int16))
+    assert awq_b200.device_status() == 2             # slots past the cache are reported
+
+
+# ---- pages --------------------------------------------------------------------------------
+def pages_state(rng, R, width, page, spare, max_new, refill=0.3):
+    lens = rng.integers(0, width * page // 2, R)
+    held = -(-lens // page)
+    reset = rng.random(R) < refill
+    new = rng.integers(0, max_new + 1, R)
+    total = int(held.sum()) + spare
+    ids = rng.permutation(total)
+    table = np.full((R, width), -1)
+    at = 0
+    for r in range(R):
+        table[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+    free = np.full(total, -1)
+    free[:spare] = ids[at:]
+    lens = np.where(reset, 0, lens)
+    return table, held, free, spare, lens, new, reset
+
+
+def run_pages(table, held, free, count, lens, new, reset, page, max_tokens):
+    st = [dev(x).int() for x in (table, held, free, [count], lens, new)]
+    out = awq_b200.kv4_pages_step(*st, page_size=page, max_tokens=max_tokens,
+                                  reset=None if reset is None else dev(reset))
+    ref = L.pages_step(table, held, free, count, lens, new, page, max_tokens, reset)
+    got = [st[0], st[1], st[2], st[3], *out]
+    for name, g, w in zip(("table", "held", "free", "count", "slots", "positions", "cu_q",
+                           "lens", "status"), got, ref):
+        assert np.array_equal(g.cpu().numpy().reshape(np.shape(w)), w), name
+    return ref
+
+
+@pytest.mark.parametrize("R,width,page,max_new", [
+    (1, 1, 16, 1), (1, 40, 16, 300), (7, 12, 16, 40), (64, 16, 64, 1), (511, 9, 32, 3),
+    (513, 9, 32, 3), (2048, 6, 16, 20), (8192, 2, 16, 2), (3, 700, 1, 200)])
+def test_pages_step(cuda, R, width, page, max_new):
+    rng = np.random.default_rng(R)
+    table, held, free, count, lens, new, reset = pages_state(
+        rng, R, width, page, R * (max_new // page + 2) + 5, max_new)
+    new = np.minimum(new, width * page - lens)
+    ref = run_pages(table, held, free, count, lens, new, reset, page, int(new.sum()) + 3)
+    assert ref[-1] == 0
+    # the step after it, without replaced rows, exactly as many tokens as fit
+    table, held, free, count, _, _, _, lens, _ = ref
+    new = np.minimum(1, width * page - lens)
+    assert run_pages(table, held, free, count, lens, new, None, page, int(new.sum()))[-1] == 0
+
+
+def test_pages_step_refusals_change_nothing(cuda):
+    rng = np.random.default_rng(2)
+    table, held, free, count, lens, new, reset = pages_state(rng, 20, 8, 16, 3, 30, refill=0.0)
+    lens, new = np.full(20, 17), np.full(20, 16)
+    held[:] = 2
+    short = run_pages(table, held, free, count, lens, new, None, 16, 400)[-1]
+    assert short == 17
+    assert run_pages(table, held, free, count, lens, new, None, 16, 319)[-1] == -1   # tokens
+    new[3] = 8 * 16
+    assert run_pages(table, held, free, count, lens, new, None, 16, 4000)[-1] == -1  # width
+    new[3] = -1
+    assert run_pages(table, held, free, count, lens, new, None, 16, 4000)[-1] == -1
+    new[3], lens[5] = 1, -1
+    assert run_pages(table, held, free, count, lens, new, None, 16, 4000)[-1] == -1
+    lens[5], held[7] = 1, 9
+    assert run_pages(table, held, free, count, lens, new, None, 16, 4000)[-1] == -1
+    held[7] = 2
+    assert run_pages(table, held, free, -1, lens, new, None, 16, 4000)[-1] == -1
+    assert run_pages(table, held, free, len(free) + 1, lens, new, None, 16, 4000)[-1] == -1
+
+
+# ---- attention ----------------------------------------------------------------------------
+def make_cache(rng, lens, Hk, D, group, page, small=False):
+    """A cache filled by the library's append; returns it, its table and the float64 K, V."""
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + 2
+    cache = awq_b200.KV4Cache.allocate(pages, Hk, D, page, group)
+    cache.data.fill_(0xFF)                             # unwritten params are NaN
+    ids = rng.permutation(pages)
+    table = np.full((len(lens), max(need + [1]) + 1), -1)
+    kv, at = [], 0
+    for r, n in enumerate(lens):
+        table[r, :need[r]] = ids[at:at + need[r]]
+        at += need[r]
+        k = rng.standard_normal((n, Hk, D)) + 4 * (rng.random((1, Hk, D)) < 0.05)
+        v = rng.standard_normal((n, Hk, D)) * np.exp(rng.uniform(-6, 1, (n, Hk, 1)))
+        if small:
+            v *= 2.0 ** -12
+        slots = table[r, np.arange(n) // page] * page + np.arange(n) % page
+        awq_b200.kv4_append(dev(k.astype(np.float16)), dev(v.astype(np.float16)), dev(slots), cache)
+        kv.append((k, v, slots))
+    data = cache.data.cpu().numpy()
+    return cache, dev(table).int(), [L.read_slots(data, s, D, page, group) for _, _, s in kv], data, kv
+
+
+def bound(q, K, V, ref, scale, data, slots, D, page, group):
+    """The module docstring's bound for one request, [n, H, D]."""
+    n, H, _ = q.shape
+    Lk, Hk = K.shape[:2]
+    out = np.zeros(ref.shape)
+    G = D // group
+    par = np.zeros((Lk, Hk, 2, G, 2))
+    for t, slot in enumerate(slots):
+        pg, at = divmod(int(slot), page)
+        p = np.ascontiguousarray(data[pg, :, at // 16, 16 * D:]).view(np.float16)
+        par[t] = p.reshape(Hk, 2, 16, G, 2)[:, :, at % 16].astype(np.float64)
+    rep = lambda x: np.repeat(x, group, -1)
+    ks, km, vs, vm = (rep(par[:, :, a, :, b]) for a in (0, 1) for b in (0, 1))
+    for i in range(n):
+        seen = Lk - n + i + 1
+        if seen <= 0:
+            continue
+        for h in range(H):
+            hk = h // (H // Hk)
+            s = scale * (K[:seen, hk] @ q[i, h])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            size = abs(scale) * ((15 * ks[:seen, hk] + np.abs(km[:seen, hk])) @ np.abs(q[i, h]))
+            e = (D + 8) * U32 * size + 2.0 ** -22
+            d = e + (p @ e)                             # of a weight, and of the sum
+            sc = vs[:seen, hk]
+            c15 = np.abs(V[:seen, hk] - vm[:seen, hk])  # s c
+            w = p[:, None] * sc
+            sub = (2.0 ** -25) * w.max() * np.where(sc > 0, 15.0, 0).max(-1, keepdims=True)
+            out[i, h] = (p[:, None] * ((U16 + d[:, None]) * c15 + d[:, None] * np.abs(vm[:seen, hk]))
+                         + sub).sum(0)
+    return out + U16 * np.abs(ref) + TINY
+
+
+def check_attention(rng, lens, qs, H, Hk, D, group, page, scale=None, small=False, pad=0):
+    cache, table, KV, data, kv = make_cache(rng, lens, Hk, D, group, page, small)
+    scale = D ** -0.5 if scale is None else scale
+    cu = np.concatenate([[0], np.cumsum(qs)])
+    q = rng.standard_normal((cu[-1] + pad, H, D)).astype(np.float16)
+    out = torch.full((cu[-1] + pad, H, D), 7.5, dtype=torch.float16, device="cuda")
+    decode = all(n == 1 for n in qs) and not pad
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev(lens).int(),
+                                 None if decode else dev(cu).int(), 1 if decode else max(qs),
+                                 scale, out)
+    assert got is out
+    assert awq_b200.device_status() == 0
+    got = got.double().cpu().numpy()
+    assert (got[cu[-1]:] == 7.5).all()                  # rows behind the last request
+    for r in range(len(lens)):
+        K, V = KV[r]
+        rows = slice(cu[r], cu[r + 1])
+        ref = L.attention(q[rows], K, V, scale)
+        tol = bound(q[rows].astype(np.float64), K, V, ref, scale, data, kv[r][2], D, page, group)
+        err = np.abs(got[rows] - ref)
+        assert (err <= tol).all(), (r, float((err / tol).max()))
+    if not decode:                                      # one at a time gives the same bits
+        again = awq_b200.kv4_attention(dev(q), cache, table, dev(lens).int(), dev(cu).int(),
+                                       max(qs), scale)
+        assert torch.equal(again[:cu[-1]].cpu(), out[:cu[-1]].cpu())
+        assert (again[cu[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("D,group", CACHES)
+@pytest.mark.parametrize("H,Hk", [(1, 1), (7, 1), (28, 4), (6, 2), (16, 1), (20, 2)])
+def test_attention_decode_heads(cuda, D, group, H, Hk):
+    check_attention(np.random.default_rng(H), [1, 33, 100], [1, 1, 1], H, Hk, D, group, 16)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 1024])
+@pytest.mark.parametrize("lens", [[0], [1], [15, 16, 17, 31, 32, 33], [0, 1000, 0, 5], [2500]])
+def test_attention_decode_lengths(cuda, page, lens):
+    check_attention(np.random.default_rng(page), lens, [1] * len(lens), 14, 2, 128, 64, page)
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 128)])
+def test_attention_small_values_and_scale(cuda, D, group):
+    rng = np.random.default_rng(9)
+    check_attention(rng, [300, 40], [1, 1], 4, 2, D, group, 32, small=True)
+    check_attention(rng, [300, 40], [1, 1], 4, 2, D, group, 32, scale=2.0)
+    check_attention(rng, [300, 40], [1, 1], 4, 2, D, group, 32, scale=-0.3)
+
+
+@pytest.mark.parametrize("D,group,H,Hk", [(128, 128, 28, 4), (64, 32, 6, 2), (128, 32, 3, 3)])
+@pytest.mark.parametrize("lens,qs", [([5], [5]), ([70, 33], [3, 17]), ([9, 4, 130], [0, 6, 65]),
+                                     ([40, 40, 40], [1, 2, 40])])
+def test_attention_chunks(cuda, D, group, H, Hk, lens, qs):
+    check_attention(np.random.default_rng(len(lens)), lens, qs, H, Hk, D, group, 16, pad=3)
+
+
+def test_attention_many_requests(cuda):
+    """More requests than prefix entries, most of them short: items end inside warps."""
+    rng = np.random.default_rng(11)
+    R = 1500
+    lens = rng.integers(0, 3, R) * rng.integers(0, 40, R)
+    check_attention(rng, [int(x) for x in lens], [1] * R, 2, 1, 64, 64, 16)
+
+
+def test_attention_skips_bad_pages_and_lengths(cuda):
+    rng = np.random.default_rng(12)
+    cache, table, KV, _, _ = make_cache(rng, [64, 64], 1, 64, 64, 16)
+    q = rng.standard_normal((2, 4, 64)).astype(np.float16)
+    lens = dev(np.array([64, 64])).int()
+    table[0, 1] = -1                                    # tokens 16..31 are not there
+    table[1, 3] = cache.num_pages
+    got = awq_b200.kv4_attention(dev(q), cache, table, lens).double().cpu().numpy()
+    assert awq_b200.device_status() == 2
+    for r, keep in ((0, [*range(16), *range(32, 64)]), (1, list(range(48)))):
+        K, V = (x[keep] for x in KV[r])
+        ref = L.attention(q[r:r + 1], K, V, 0.125)
+        assert np.abs(got[r:r + 1] - ref).max() <= 2e-3 * np.abs(V).max()
+    table[0, 1] = 0
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev(np.array([10 ** 6, -3])).int())
+    assert awq_b200.device_status() == 2
+    assert (got[1] == 0).all()
+
+
+def test_attention_nan_stays_in_seen_rows(cuda):
+    """A NaN key or value makes the rows that see it NaN, and no other."""
+    rng = np.random.default_rng(13)
+    cache, table, _, _, kv = make_cache(rng, [40], 1, 64, 64, 16)
+    k = torch.full((1, 1, 64), float("nan"), dtype=torch.float16, device="cuda")
+    awq_b200.kv4_append(k, k, dev(kv[0][2][37:38]), cache)
+    q = dev(rng.standard_normal((6, 2, 64)).astype(np.float16))
+    got = awq_b200.kv4_attention(q, cache, table, dev(np.array([40])).int(),
+                                 dev(np.array([0, 6])).int(), 6)
+    bad = torch.isnan(got).flatten(1)
+    assert bad[3:].all() and not bad[:3].any()
+
+
+def test_attention_graph_and_streams(cuda):
+    """Captured once, replayed with other lengths, and two graphs replayed at the same time."""
+    rng = np.random.default_rng(14)
+    lens = [200, 333]
+    cache, table, KV, _, _ = make_cache(rng, lens, 2, 128, 128, 32)
+    q = dev(rng.standard_normal((2, 14, 128)).astype(np.float16))
+    kv_lens = dev(np.array(lens)).int()
+    want = awq_b200.kv4_attention(q, cache, table, kv_lens)
+    part = dev(np.array([57, 1])).int()
+    want2 = awq_b200.kv4_attention(q, cache, table, part)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            live = kv_lens.clone()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                out = awq_b200.kv4_attention(q, cache, table, live)
+            graphs.append((g, live, out))
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for lens_now, ref in ((kv_lens, want), (part, want2), (kv_lens, want)):
+        for _, live, _ in graphs:
+            live.copy_(lens_now)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for st, (g, _, _) in zip((a, b), graphs):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, ref) for _, _, out in graphs)
