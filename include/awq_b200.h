@@ -117,6 +117,28 @@ AWQ_API int awq_gemm_f16_bias(const void* x, int64_t ldx, const int32_t* qweight
                               void* stream);
 
 /*
+ * out = act(x @ W + bias) + residual: the product with bias (fp16 [N] or null), activation
+ * (AWQ_ACT_*) and residual (fp16 [M, N], row stride ldr, or null) in its epilogue, fp32 up to
+ * the one fp16 rounding.  For the residual adds behind o and down, which the reference makes
+ * in the next layer norm (model/qwen2.py:207-229, kernels/fused_add_rmsnorm.py:40-50), and
+ * for activated layers.  residual may be out itself (same pointer and stride); it must not
+ * overlap out in any other way.  relu is max(y, 0); silu y / (1 + exp(-y)); gelu
+ * y (1 + erf(y / sqrt 2)) / 2; gelu_tanh its tanh form.  Same kernels, requirements and
+ * workspace as awq_gemm_f16 (AWQ_PATH_AUTO).
+ */
+#define AWQ_ACT_NONE 0
+#define AWQ_ACT_RELU 1
+#define AWQ_ACT_SILU 2
+#define AWQ_ACT_GELU 3
+#define AWQ_ACT_GELU_TANH 4
+AWQ_API int awq_gemm_f16_epilogue(const void* x, int64_t ldx, const int32_t* qweight,
+                                  const int32_t* qzeros, const void* scales, const void* bias,
+                                  int activation, const void* residual, int64_t ldr, void* out,
+                                  int64_t ldo, int64_t M, int64_t N, int64_t K,
+                                  int64_t group_size, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/*
  * out = silu(G) * U for the fused gate+up product P = x @ W (W = [gate | up], N
  * columns): G = P[:, :N/2], U = P[:, N/2:], out fp16 [M, N/2] (ldo >= N/2).  Replaces the
  * reference MLP's awq_gemm_forward + two .contiguous() slices + silu_mul_forward

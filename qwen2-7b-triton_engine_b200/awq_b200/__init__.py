@@ -7,6 +7,7 @@ the CUDA library; nothing here has a CPU fallback.
 Public functions
   dequant(qweight, qzeros, scales, group_size)      -> fp16 [K, N]   (bit-exact W)
   gemm(x2d, qweight, qzeros, scales, group_size, path) -> fp16 [M, N]
+  gemm_epilogue(x2d, ..., bias, activation, residual) -> act(x2d @ W + bias) + residual
   device_status(stream)                              -> status bits of the kernels
   rope_axes, KV4Cache, kv4_pages_step, kv4_append, kv4_gather, kv4_attention
                                                      the operators between the products
@@ -37,7 +38,7 @@ from ._lib import (AWQ_PATH_AUTO, AWQ_PATH_DECODE, AWQ_PATH_TC, AWQ_PATH_TS, Awq
 from .layer import (KV4Cache, kv4_append, kv4_attention, kv4_gather, kv4_pages_step,  # noqa: F401
                     rope_axes)
 
-__all__ = ["dequant", "gemm", "gemm_silu_mul", "gemm_allreduce", "TPComm", "device_status", "workspace_for", "AwqError",
+__all__ = ["dequant", "gemm", "gemm_epilogue", "gemm_silu_mul", "gemm_allreduce", "TPComm", "device_status", "workspace_for", "AwqError",
            "KV4Cache", "rope_axes", "kv4_pages_step", "kv4_append", "kv4_gather", "kv4_attention",
            "AWQ_PATH_AUTO", "AWQ_PATH_DECODE", "AWQ_PATH_TC", "AWQ_PATH_TS", "LIB_PATH"]
 
@@ -114,6 +115,15 @@ def check_weights(qweight, qzeros, scales, group_size):
 
 def _stream_handle(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors overlap."""
+    def span(t):
+        last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) if t.numel() else -1
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
 
 
 class _DeviceGuard:
@@ -271,6 +281,85 @@ def gemm(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor, scales:
                 scales.data_ptr(), bias.data_ptr(), out.data_ptr(), out.stride(0), M, N, K, gs,
                 ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
                 stream.cuda_stream))
+    return out
+
+
+def gemm_epilogue(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor,
+                  scales: torch.Tensor, group_size: int = 128, bias: torch.Tensor | None = None,
+                  activation: str | None = None, residual: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """fp16 [M, N] = act(x2d @ W + bias) + residual in one call (``awq_gemm_f16_epilogue``):
+    bias fp16 [N], activation None / "none", "relu", "silu", "gelu" or "gelu_tanh", residual
+    fp16 [M, N] (rows may be strided); fp32 up to the one rounding.  ``out`` may be
+    ``residual`` (the residual stream updated in place); otherwise it must overlap no input.
+    Outside graph capture the split-K workspace is the one of the current stream; a captured
+    call gets its own, so that graphs may replay at the same time."""
+    K, N, qweight, qzeros, scales = _prepared_weights(qweight, qzeros, scales, group_size)
+    _require_cuda(x2d, "x")
+    if x2d.dtype != torch.float16:
+        raise TypeError(f"x must be float16, got {x2d.dtype}")
+    if x2d.dim() != 2 or x2d.shape[1] != K:
+        raise ValueError(f"x must be [M, K={K}], got {tuple(x2d.shape)}")
+    dev = x2d.device
+    if dev != qweight.device:
+        raise ValueError("x and the weights must be on one device")
+    M = x2d.shape[0]
+    act = _lib.ACTIVATIONS.get("none" if activation is None else activation)
+    if act is None:
+        raise ValueError(f"activation {activation!r} is none of {sorted(_lib.ACTIVATIONS)}")
+    for t, name, shape in ((bias, "bias", (N,)), (residual, "residual", (M, N))):
+        if t is None:
+            continue
+        _require_cuda(t, name)
+        if t.dtype != torch.float16:
+            raise TypeError(f"{name} must be float16, got {t.dtype}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.float16, device=dev)
+    else:
+        _require_cuda(out, "out")
+        if out.dtype != torch.float16:
+            raise TypeError(f"out must be float16, got {out.dtype}")
+        if tuple(out.shape) != (M, N) or out.device != dev or out.stride(1) != 1 \
+                or (M > 1 and out.stride(0) < N) or out.data_ptr() % 16 or out.stride(0) % 8:
+            raise ValueError(f"out must be a [{M}, {N}] tensor on {dev} with dense, 16-byte "
+                             "aligned rows")
+        same = residual is not None and out.data_ptr() == residual.data_ptr() \
+            and out.stride() == residual.stride()
+        if any(t is not None and not (t is residual and same) and _overlap(out, t)
+               for t in (x2d, bias, residual)):
+            raise ValueError("out overlaps an input (it may only be the residual itself)")
+    if M == 0:
+        return out
+    if bias is not None:
+        bias = bias.contiguous()
+    if residual is not None and (residual.stride(1) != 1 or (M > 1 and residual.stride(0) < N)):
+        residual = residual.contiguous()
+    if x2d.stride(1) != 1 or x2d.data_ptr() % 16 or (x2d.stride(0) * 2) % 16 \
+            or (M > 1 and x2d.stride(0) < K):
+        x2d = x2d.contiguous()
+        if x2d.data_ptr() % 16:
+            x2d = x2d.clone()
+    lib = _lib.load()
+    gs = int(group_size)
+    with _DeviceGuard(dev):
+        stream = torch.cuda.current_stream(dev)
+        need = _workspace_need(lib, dev, M, N, K, gs)
+        ws = None
+        if need and torch.cuda.is_current_stream_capturing():
+            ws = torch.zeros(need, dtype=torch.uint8, device=dev)
+        elif need:
+            ws = workspace_for(dev, need, stream)
+        _lib.check(lib.awq_gemm_f16_epilogue(
+            x2d.data_ptr(), max(x2d.stride(0), K), qweight.data_ptr(), qzeros.data_ptr(),
+            scales.data_ptr(), bias.data_ptr() if bias is not None else None, act,
+            residual.data_ptr() if residual is not None else None,
+            max(residual.stride(0), N) if residual is not None else 0, out.data_ptr(),
+            max(out.stride(0), N), M, N, K, gs, ws.data_ptr() if ws is not None else None,
+            ws.numel() if ws is not None else 0, stream.cuda_stream))
     return out
 
 

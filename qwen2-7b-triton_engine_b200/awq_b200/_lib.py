@@ -25,6 +25,9 @@ AWQ_PATH_DECODE = 1
 AWQ_PATH_TC = 2
 AWQ_PATH_TS = 3
 
+# activations of awq_gemm_f16_epilogue
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
 # Every symbol include/awq_b200.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -57,6 +60,8 @@ SIGNATURES = {
     "awq_gemm_silu_mul_workspace_bytes": ([_I64, _I64, _I64, _I64], _SZ),
     "awq_gemm_f16_silu_mul": ([_P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _SZ,
                                _P], _INT),
+    "awq_gemm_f16_epilogue": ([_P, _I64, _P, _P, _P, _P, _INT, _P, _I64, _P, _I64, _I64, _I64,
+                               _I64, _I64, _P, _SZ, _P], _INT),
     "awq_rope_axes": ([_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _INT, _I64, _P,
                        _P, _INT, _INT, _P, _I64, _I64, _P, _I64, _I64, _P], _INT),
     "awq_kv4_page_bytes": ([_I64, _I64, _I64, _I64], _SZ),

@@ -57,15 +57,6 @@ def _last_dense(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors' address ranges overlap (same start and strides included)."""
-    def span(t):
-        last = sum((n - 1) * abs(s) for n, s in zip(t.shape, t.stride())) if t.numel() else -1
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
-
-
 @dataclass(frozen=True)
 class KV4Cache:
     """A paged key/value cache in 4 bits: ``data`` uint8 [num_pages, kv_heads,
@@ -163,7 +154,7 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
                 raise ValueError(f"{name} must be {tuple(x.shape)} with a dense last dimension")
             same = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
             for y in (q, k):
-                if _overlap(o, y) and not (same and y is x) and not _apart(o, y):
+                if _core()._overlap(o, y) and not (same and y is x) and not _apart(o, y):
                     raise ValueError(f"{name} overlaps an input other than as that input itself")
         outs.append(o)
     oq, ok = outs
@@ -326,7 +317,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
                 or out.stride(0) % 4 or out.stride(1) % 4:
             raise ValueError(f"out must be {(T, H, D)} with a dense last dimension, 8-byte "
                              "aligned rows")
-        if _overlap(out, q):
+        if _core()._overlap(out, q):
             raise ValueError("out overlaps q")
     if T == 0 or R == 0:
         return out

@@ -192,11 +192,12 @@ int awq_tc_supported(const void* x, int64_t ldx, const int32_t* qweight, const i
   return awq::tc_supported(x, ldx, qweight, qzeros, scales, M, N, K, group_size) ? 1 : 0;
 }
 
-// The product behind awq_gemm_f16_ex and awq_gemm_f16_bias (bias: fp16 [N] or null).
+// The product behind awq_gemm_f16_ex, awq_gemm_f16_bias and awq_gemm_f16_epilogue (bias: fp16
+// [N] or null; epi: activation and residual, or null).
 static int gemm_impl(const void* x, int64_t ldx, const int32_t* qweight, const int32_t* qzeros,
                      const void* scales, void* out, int64_t ldo, int64_t M, int64_t N, int64_t K,
                      int64_t group_size, void* workspace, size_t workspace_bytes, void* stream,
-                     int path, const void* bias) {
+                     int path, const void* bias, const awq::EpiArgs* epi = nullptr) {
   int rc = check_weights(qweight, qzeros, scales, K, N, group_size);
   if (rc) return rc;
   if (!x || !out) return fail(AWQ_ERR_INVALID_ARG, "null x or out");
@@ -230,7 +231,7 @@ static int gemm_impl(const void* x, int64_t ldx, const int32_t* qweight, const i
     const char* why = nullptr;
     cudaError_t e = awq::launch_gemm_ts(x, ldx, qweight, qzeros, scales, out, ldo, (int)M, (int)N,
                                         (int)K, (int)group_size, d->num_sms, d->status, st, &why,
-                                        bias, workspace, workspace_bytes);
+                                        bias, workspace, workspace_bytes, false, epi);
     if (why) return fail(AWQ_ERR_UNSUPPORTED, "small-M tcgen05 path: %s", why);
     if (e != cudaSuccess) return fail_cuda(e, "small-M tcgen05 GEMM launch");
     return AWQ_OK;
@@ -262,7 +263,7 @@ static int gemm_impl(const void* x, int64_t ldx, const int32_t* qweight, const i
     const char* why = nullptr;
     cudaError_t e = awq::launch_gemm_tc(x, ldx, qweight, qzeros, scales, out, ldo, (int)M, (int)N,
                                         (int)K, (int)group_size, d->num_sms, d->status, st, &why,
-                                        bias, workspace, workspace_bytes);
+                                        bias, workspace, workspace_bytes, false, epi);
     if (why) return fail(AWQ_ERR_UNSUPPORTED, "tcgen05 path: %s", why);
     if (e != cudaSuccess) return fail_cuda(e, "tcgen05 GEMM launch");
     return AWQ_OK;
@@ -285,10 +286,15 @@ static int gemm_impl(const void* x, int64_t ldx, const int32_t* qweight, const i
       char* ob = static_cast<char*>(out);
       for (int64_t m0 = 0; m0 < M; m0 += 16) {
         const int64_t mc = M - m0 < 16 ? M - m0 : 16;
+        awq::EpiArgs part;                                        // this launch's residual rows
+        if (epi) {
+          part = *epi;
+          if (part.residual) part.residual = static_cast<const char*>(part.residual) + 2 * m0 * part.ldr;
+        }
         cudaError_t e = awq::launch_gemv_tma(mc == m_full ? full : rest, xb + 2 * m0 * ldx, ldx,
                                              qweight, qzeros, scales, ob + 2 * m0 * ldo, ldo, (int)mc,
                                              (int)N, (int)K, (int)group_size, workspace, d->status,
-                                             st, nullptr, bias);
+                                             st, nullptr, bias, false, epi ? &part : nullptr);
         if (e != cudaSuccess) return fail_cuda(e, "decode (TMA) kernel launch");
       }
       return AWQ_OK;
@@ -306,7 +312,7 @@ static int gemm_impl(const void* x, int64_t ldx, const int32_t* qweight, const i
   if (need > 0 && !aligned16(workspace))
     return fail(AWQ_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
   cudaError_t e = awq::launch_gemv(plan, x, ldx, qweight, qzeros, scales, out, ldo, (int)M, (int)N,
-                                   (int)K, (int)group_size, workspace, st, bias);
+                                   (int)K, (int)group_size, workspace, st, bias, epi);
   if (e != cudaSuccess) return fail_cuda(e, "decode kernel launch");
   return AWQ_OK;
 }
@@ -327,6 +333,26 @@ int awq_gemm_f16_bias(const void* x, int64_t ldx, const int32_t* qweight, const 
     return fail(AWQ_ERR_INVALID_ARG, "bias must be a non-null, 2-byte aligned fp16 [N] pointer");
   return gemm_impl(x, ldx, qweight, qzeros, scales, out, ldo, M, N, K, group_size, workspace,
                    workspace_bytes, stream, AWQ_PATH_AUTO, bias);
+}
+
+int awq_gemm_f16_epilogue(const void* x, int64_t ldx, const int32_t* qweight, const int32_t* qzeros,
+                          const void* scales, const void* bias, int activation,
+                          const void* residual, int64_t ldr, void* out, int64_t ldo, int64_t M,
+                          int64_t N, int64_t K, int64_t group_size, void* workspace,
+                          size_t workspace_bytes, void* stream) {
+  if (activation < AWQ_ACT_NONE || activation > AWQ_ACT_GELU_TANH)
+    return fail(AWQ_ERR_INVALID_ARG, "unknown activation %d", activation);
+  if (bias && (reinterpret_cast<uintptr_t>(bias) & 1))
+    return fail(AWQ_ERR_INVALID_ARG, "bias must be 2-byte aligned");
+  if (residual && ((reinterpret_cast<uintptr_t>(residual) & 1) || ldr < N))
+    return fail(AWQ_ERR_INVALID_ARG, "residual must be 2-byte aligned with ldr >= N");
+  awq::EpiArgs epi;
+  epi.residual = residual;
+  epi.ldr = ldr;
+  epi.act = activation;
+  const bool plain = activation == AWQ_ACT_NONE && !residual;    // the biased product's kernels
+  return gemm_impl(x, ldx, qweight, qzeros, scales, out, ldo, M, N, K, group_size, workspace,
+                   workspace_bytes, stream, AWQ_PATH_AUTO, bias, plain ? nullptr : &epi);
 }
 
 // ---- gate+up product followed by SiLU-mul --------------------------------------------

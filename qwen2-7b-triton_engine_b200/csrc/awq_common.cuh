@@ -105,6 +105,27 @@ __device__ __forceinline__ void dequant_word(uint32_t w, const uint32_t zc[4], c
 }
 
 // ---------------------------------------------------------------------------------
+// Epilogue activations (fp32; the code numbers are awq_internal.h's Activation).  silu and
+// gelu_tanh are y / (1 + exp(-z)) with z = y and z = 2 sqrt(2/pi) (y + 0.044715 y^3), the
+// tanh form rewritten.  The hardware exponential and an approximate divide (a few fp32 ulp)
+// stand far below the fp16 rounding that follows.
+// ---------------------------------------------------------------------------------
+__device__ __forceinline__ float logistic_mul(float y, float z) {
+  const float e = __expf(-z);
+  // a divisor past 2^126 makes the approximate divide return 0, which the quotient rounds to
+  return __fdividef(y, 1.0f + e);
+}
+__device__ __forceinline__ float activate(float y, int act) {
+  switch (act) {
+    case 1: return y > 0.f || y != y ? y : 0.f;
+    case 2: return logistic_mul(y, y);
+    case 3: return 0.5f * y * erfcf(-0.70710678f * y);
+    case 4: return logistic_mul(y, 1.5957691f * y * fmaf(0.044715f * y, y, 1.0f));
+    default: return y;
+  }
+}
+
+// ---------------------------------------------------------------------------------
 // Global memory helpers
 // ---------------------------------------------------------------------------------
 __device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {

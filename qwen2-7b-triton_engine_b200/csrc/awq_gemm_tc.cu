@@ -94,6 +94,10 @@ struct TcArgs {
   int M, N, K, gs;
   int* status;
   const __half* bias;   // fp16 [N] added to every output row in fp32, or null
+  const __half* residual;   // EpiArgs (kernels built with EPI)
+  int64_t ldr;
+  int act;
+  int res_vec;          // residual rows can be read 16 bytes at a time
   int splits;           // CTAs along K per output tile (blockIdx.z); > 1: fp32 partials
   float* part;          // [splits][M][N] fp32 partials when splits > 1
   // stream-K (streamk != 0, splits == 1; tiles < gridDim.x): CTA c < tiles runs K steps
@@ -122,6 +126,49 @@ struct TcArgs {
   // fp16(silu(g) * u) with g and u the fp16-rounded products (out is [M, N/2]).
   int silu;
 };
+
+// act(v + bias) + residual of 32 consecutive columns of one row, in fp32 (EpiArgs).  The row
+// may lie past M (its values are not stored): it then reads no residual.
+__device__ __forceinline__ void epilogue32(const TcArgs& a, float (&v)[32], int row, int col) {
+  if (a.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] += __half2float(a.bias[col + j]);
+  }
+  // one unrolled loop per activation: a loop over activate(v[j], act) would index v
+  // dynamically and move it to local memory
+  if (a.act == kActRelu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], kActRelu);
+  } else if (a.act == kActSilu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], kActSilu);
+  } else if (a.act == kActGelu) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], kActGelu);
+  } else if (a.act == kActGeluTanh) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = activate(v[j], kActGeluTanh);
+  }
+  if (a.residual && row < a.M) {
+    const __half* r = a.residual + (int64_t)row * a.ldr + col;
+    if (a.res_vec) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint4 u = *reinterpret_cast<const uint4*>(r + 8 * j);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = __half22float2(u32_as_h2(w[e]));
+          v[8 * j + 2 * e] += f.x;
+          v[8 * j + 2 * e + 1] += f.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] += __half2float(r[j]);
+    }
+  }
+}
 
 // silu(g) * u of fp32 products rounded to fp16 first, as the unfused sequence rounds its
 // product.  The sigmoid uses the hardware exponential and an approximate divide (two
@@ -213,7 +260,8 @@ __device__ __forceinline__ int atom_add_acq_rel_gpu(int* p, int v) {
   return old;
 }
 
-template <int NACC>
+// EPI: the activation / residual epilogue; without it the kernel is the plain product.
+template <int NACC, bool EPI>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmZ,
@@ -558,7 +606,16 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
               sm100::tmem_ld_32x32b_x32(taddr + (c + part) * 32, v);
               sm100::tmem_ld_wait();
               const int ccol = col + part * 32;
-              if (args.bias && ccol < args.N) {  // the columns' bias, added in fp32
+              if constexpr (EPI) {
+                if (ccol < args.N) {
+                  float f[32];
+#pragma unroll
+                  for (int jj = 0; jj < 32; ++jj) f[jj] = __uint_as_float(v[jj]);
+                  epilogue32(args, f, row, ccol);
+#pragma unroll
+                  for (int jj = 0; jj < 32; ++jj) v[jj] = __float_as_uint(f[jj]);
+                }
+              } else if (args.bias && ccol < args.N) {  // the columns' bias, added in fp32
 #pragma unroll
                 for (int jj = 0; jj < 32; ++jj)
                   v[jj] = __float_as_uint(__uint_as_float(v[jj]) + __half2float(args.bias[ccol + jj]));
@@ -683,7 +740,9 @@ gemm_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
                     sum[4 * jj + e] = acc;
                   }
                 }
-                if (args.bias) {
+                if constexpr (EPI) {
+                  epilogue32(args, sum, row, col);
+                } else if (args.bias) {
 #pragma unroll
                   for (int jj = 0; jj < 32; ++jj) sum[jj] += __half2float(args.bias[col + jj]);
                 }
@@ -786,7 +845,7 @@ struct TsGeo {
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 
-template <int NT>
+template <int NT, bool EPI>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_ts_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW,
                const __grid_constant__ CUtensorMap tmS, const __grid_constant__ CUtensorMap tmZ,
@@ -1063,8 +1122,14 @@ gemm_ts_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
             if (row < args.M) {
               if (args.splits > 1)
                 args.part[((size_t)blockIdx.z * args.M + row) * args.N + col] = __uint_as_float(v[j]);
-              else
-                args.out[(int64_t)row * args.ldo + col] = __float2half_rn(__uint_as_float(v[j]) + bias);
+              else {
+                float y = __uint_as_float(v[j]) + bias;
+                if constexpr (EPI) {
+                  y = activate(y, args.act);
+                  if (args.residual) y += __half2float(args.residual[(int64_t)row * args.ldr + col]);
+                }
+                args.out[(int64_t)row * args.ldo + col] = __float2half_rn(y);
+              }
             }
           }
         }
@@ -1121,10 +1186,13 @@ bool make_map_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* ptr, uint64
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// out[M, N] = fp16(sum over z of part[z] (+ bias)), four columns per thread, z in order.
+// out[M, N] = fp16(sum over z of part[z] (+ bias)) (EPI: activated, plus the residual, which
+// may be out), four columns per thread, z in order.
+template <bool EPI>
 __global__ void __launch_bounds__(256)
-tc_splitk_reduce(const float* __restrict__ part, int splits, int M, int N,
-                 __half* __restrict__ out, int64_t ldo, const __half* __restrict__ bias) {
+tc_splitk_reduce(const float* __restrict__ part, int splits, int M, int N, __half* out,
+                 int64_t ldo, const __half* __restrict__ bias, const __half* residual,
+                 int64_t ldr, int act, int res_vec) {
   const int n4 = N / 4;
   const int64_t total = (int64_t)M * n4;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
@@ -1140,9 +1208,88 @@ tc_splitk_reduce(const float* __restrict__ part, int splits, int M, int N,
       acc.x += __half2float(bias[c]); acc.y += __half2float(bias[c + 1]);
       acc.z += __half2float(bias[c + 2]); acc.w += __half2float(bias[c + 3]);
     }
+    if constexpr (EPI) {
+      acc.x = activate(acc.x, act), acc.y = activate(acc.y, act);
+      acc.z = activate(acc.z, act), acc.w = activate(acc.w, act);
+      if (residual) {
+        const __half* r = residual + row * ldr + c;
+        if (res_vec) {
+          const uint2 u = *reinterpret_cast<const uint2*>(r);
+          const float2 a = __half22float2(u32_as_h2(u.x)), b = __half22float2(u32_as_h2(u.y));
+          acc.x += a.x, acc.y += a.y, acc.z += b.x, acc.w += b.y;
+        } else {
+          acc.x += __half2float(r[0]), acc.y += __half2float(r[1]);
+          acc.z += __half2float(r[2]), acc.w += __half2float(r[3]);
+        }
+      }
+    }
     const __half2 lo = __floats2half2_rn(acc.x, acc.y), hi = __floats2half2_rn(acc.z, acc.w);
     *reinterpret_cast<uint2*>(out + row * ldo + c) = make_uint2(h2_as_u32(lo), h2_as_u32(hi));
   }
+}
+
+void set_epilogue(TcArgs* a, const EpiArgs* epi) {
+  a->residual = epi ? static_cast<const __half*>(epi->residual) : nullptr;
+  a->ldr = epi ? epi->ldr : 0;
+  a->act = epi ? epi->act : kActNone;
+  a->res_vec = al16(a->residual) && a->ldr % 8 == 0;
+}
+
+// Kernel attributes, the launch, and the split-K reduction behind it.
+template <bool EPI>
+cudaError_t start_tc(int nacc, dim3 grid, const CUtensorMap& tmA, const CUtensorMap& tmW,
+                     const CUtensorMap& tmS, const CUtensorMap& tmZ, const TcArgs& a, int num_sms,
+                     cudaStream_t stream) {
+  static PerDeviceOnce attr_once;
+  const cudaError_t attr_err = attr_once.run([] {
+    cudaError_t e = cudaFuncSetAttribute(gemm_tc_kernel<1, EPI>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)Geo<1>::SMEM_BYTES);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_tc_kernel<2, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)Geo<2>::SMEM_BYTES);
+    return e;
+  });
+  if (attr_err != cudaSuccess) return attr_err;
+  if (nacc == 2)
+    gemm_tc_kernel<2, EPI><<<grid, kThreads, Geo<2>::SMEM_BYTES, stream>>>(tmA, tmW, tmS, tmZ, a);
+  else
+    gemm_tc_kernel<1, EPI><<<grid, kThreads, Geo<1>::SMEM_BYTES, stream>>>(tmA, tmW, tmS, tmZ, a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  tc_splitk_reduce<EPI><<<num_sms * 4, 256, 0, stream>>>(a.part, a.splits, a.M, a.N, a.out, a.ldo,
+                                                         a.bias, a.residual, a.ldr, a.act, a.res_vec);
+  return cudaGetLastError();
+}
+template <bool EPI>
+cudaError_t start_ts(int nt, dim3 grid, const CUtensorMap& tmX, const CUtensorMap& tmW,
+                     const CUtensorMap& tmS, const CUtensorMap& tmZ, const TcArgs& a, int num_sms,
+                     cudaStream_t stream) {
+  static PerDeviceOnce attr_once;
+  const cudaError_t attr_err = attr_once.run([] {
+    cudaError_t e = cudaFuncSetAttribute(gemm_ts_kernel<16, EPI>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)TsGeo<16>::SMEM_BYTES);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_ts_kernel<32, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)TsGeo<32>::SMEM_BYTES);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(gemm_ts_kernel<64, EPI>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)TsGeo<64>::SMEM_BYTES);
+    return e;
+  });
+  if (attr_err != cudaSuccess) return attr_err;
+  if (nt == 16)
+    gemm_ts_kernel<16, EPI><<<grid, kThreads, TsGeo<16>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
+  else if (nt == 32)
+    gemm_ts_kernel<32, EPI><<<grid, kThreads, TsGeo<32>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
+  else
+    gemm_ts_kernel<64, EPI><<<grid, kThreads, TsGeo<64>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  tc_splitk_reduce<EPI><<<num_sms * 4, 256, 0, stream>>>(a.part, a.splits, a.M, a.N, a.out, a.ldo,
+                                                         a.bias, a.residual, a.ldr, a.act, a.res_vec);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -1221,9 +1368,10 @@ cudaError_t launch_gemm_tc(const void* x, int64_t ldx, const int32_t* qweight,
                            const int32_t* qzeros, const void* scales, void* out, int64_t ldo,
                            int M, int N, int K, int group_size, int num_sms, int* dev_status,
                            cudaStream_t stream, const char** why, const void* bias,
-                           void* workspace, size_t workspace_bytes, bool silu) {
+                           void* workspace, size_t workspace_bytes, bool silu,
+                           const EpiArgs* epi) {
   *why = nullptr;
-  if (silu && (N % (2 * BN) || bias)) {
+  if (silu && (N % (2 * BN) || bias || epi)) {
     *why = "SiLU-mul epilogue needs N % 512 == 0 and no bias";
     return cudaSuccess;
   }
@@ -1251,23 +1399,13 @@ cudaError_t launch_gemm_tc(const void* x, int64_t ldx, const int32_t* qweight,
     *why = "cuTensorMapEncodeTiled failed";
     return cudaSuccess;
   }
-  static PerDeviceOnce attr_once;
-  const cudaError_t attr_err = attr_once.run([] {
-    cudaError_t e = cudaFuncSetAttribute(gemm_tc_kernel<1>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)Geo<1>::SMEM_BYTES);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(gemm_tc_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)Geo<2>::SMEM_BYTES);
-    return e;
-  });
-  if (attr_err != cudaSuccess) return attr_err;
   TcArgs a;
   a.out = static_cast<__half*>(out);
   a.ldo = ldo;
   a.M = M; a.N = N; a.K = K; a.gs = group_size;
   a.status = dev_status;
   a.bias = static_cast<const __half*>(bias);
+  set_epilogue(&a, epi);
   // split-K or stream-K when the caller's workspace holds the partials (after the decode
   // kernels' counter region, which must stay zero); otherwise one CTA per tile
   a.splits = silu ? 1 : tc_splits(M, N, K, num_sms);
@@ -1304,14 +1442,8 @@ cudaError_t launch_gemm_tc(const void* x, int64_t ldx, const int32_t* qweight,
     a.persistent = 1;                    // one CTA per SM, tiles taken in grid order
     grid = dim3(num_sms, 1, 1);
   }
-  if (nacc == 2)
-    gemm_tc_kernel<2><<<grid, kThreads, Geo<2>::SMEM_BYTES, stream>>>(tmA, tmW, tmS, tmZ, a);
-  else
-    gemm_tc_kernel<1><<<grid, kThreads, Geo<1>::SMEM_BYTES, stream>>>(tmA, tmW, tmS, tmZ, a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
-  tc_splitk_reduce<<<num_sms * 4, 256, 0, stream>>>(a.part, a.splits, M, N, a.out, ldo, a.bias);
-  return cudaGetLastError();
+  return epi ? start_tc<true>(nacc, grid, tmA, tmW, tmS, tmZ, a, num_sms, stream)
+             : start_tc<false>(nacc, grid, tmA, tmW, tmS, tmZ, a, num_sms, stream);
 }
 
 // ---- small-M kernel ---------------------------------------------------------------------
@@ -1345,13 +1477,14 @@ cudaError_t launch_gemm_ts(const void* x, int64_t ldx, const int32_t* qweight,
                            const int32_t* qzeros, const void* scales, void* out, int64_t ldo,
                            int M, int N, int K, int group_size, int num_sms, int* dev_status,
                            cudaStream_t stream, const char** why, const void* bias,
-                           void* workspace, size_t workspace_bytes, bool silu) {
+                           void* workspace, size_t workspace_bytes, bool silu,
+                           const EpiArgs* epi) {
   *why = nullptr;
   if (!ts_supported(x, ldx, qweight, qzeros, scales, M, N, K, group_size)) {
     *why = "shape or alignment not supported";
     return cudaSuccess;
   }
-  if (silu && (N % (2 * BN) || bias || ts_splits(M, N, K, num_sms) != 1)) {
+  if (silu && (N % (2 * BN) || bias || epi || ts_splits(M, N, K, num_sms) != 1)) {
     *why = "SiLU-mul epilogue needs N a multiple of 512, no bias and no K split";
     return cudaSuccess;
   }
@@ -1375,26 +1508,13 @@ cudaError_t launch_gemm_ts(const void* x, int64_t ldx, const int32_t* qweight,
     *why = "cuTensorMapEncodeTiled failed";
     return cudaSuccess;
   }
-  static PerDeviceOnce attr_once;
-  const cudaError_t attr_err = attr_once.run([] {
-    cudaError_t e = cudaFuncSetAttribute(gemm_ts_kernel<16>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)TsGeo<16>::SMEM_BYTES);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(gemm_ts_kernel<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)TsGeo<32>::SMEM_BYTES);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(gemm_ts_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)TsGeo<64>::SMEM_BYTES);
-    return e;
-  });
-  if (attr_err != cudaSuccess) return attr_err;
   TcArgs a;
   a.out = static_cast<__half*>(out);
   a.ldo = ldo;
   a.M = M; a.N = N; a.K = K; a.gs = group_size;
   a.status = dev_status;
   a.bias = static_cast<const __half*>(bias);
+  set_epilogue(&a, epi);
   a.splits = ts_splits(M, N, K, num_sms);
   a.part = nullptr;
   a.silu = silu ? 1 : 0;
@@ -1405,16 +1525,8 @@ cudaError_t launch_gemm_ts(const void* x, int64_t ldx, const int32_t* qweight,
       a.splits = 1;
   }
   dim3 grid((M + nt - 1) / nt, (N + BN - 1) / BN, a.splits);
-  if (nt == 16)
-    gemm_ts_kernel<16><<<grid, kThreads, TsGeo<16>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
-  else if (nt == 32)
-    gemm_ts_kernel<32><<<grid, kThreads, TsGeo<32>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
-  else
-    gemm_ts_kernel<64><<<grid, kThreads, TsGeo<64>::SMEM_BYTES, stream>>>(tmX, tmW, tmS, tmZ, a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
-  tc_splitk_reduce<<<num_sms * 4, 256, 0, stream>>>(a.part, a.splits, M, N, a.out, ldo, a.bias);
-  return cudaGetLastError();
+  return epi ? start_ts<true>(nt, grid, tmX, tmW, tmS, tmZ, a, num_sms, stream)
+             : start_ts<false>(nt, grid, tmX, tmW, tmS, tmZ, a, num_sms, stream);
 }
 
 }  // namespace awq

@@ -102,6 +102,9 @@ struct TmaGemvArgs {
   int* status;
   ArArgs ar;       // fused all-reduce across tensor-parallel ranks (ar.world == 1: none)
   const __half* bias;   // fp16 [N] added to every output row in fp32, or null
+  const __half* residual;   // EpiArgs (kernels built with EPI)
+  int64_t ldr;
+  int act;
   // SiLU-mul epilogue (pair_strips > 0): columns [0, N/2) are gate, [N/2, N) up, and
   // out[m, n] = silu(gate[m, n]) * up[m, n] for n < N/2.  Strip s < pair_strips pairs
   // with strip s + pair_strips; each tile parks its final fp32 values in pair_vals and
@@ -192,7 +195,8 @@ __device__ __forceinline__ void warp_range(int cb0, int nb, int w, int& b0, int&
   b1 = cb0 + min(nb, (w + 1) * per);
 }
 
-template <int TOKSETS>
+// EPI: the activation / residual epilogue; without it the kernel is the plain product.
+template <int TOKSETS, bool EPI>
 __global__ void __launch_bounds__(kThreads, 1)
 gemv_tma_kernel(const __grid_constant__ CUtensorMap tmW, const TmaGemvArgs a) {
   constexpr int MP = 4 * TOKSETS;
@@ -522,16 +526,20 @@ gemv_tma_kernel(const __grid_constant__ CUtensorMap tmW, const TmaGemvArgs a) {
   const uint32_t flag = epoch + 1u;
   const size_t ar_rank_stride = (size_t)a.ar.max_tiles * kArTileFloats;
   const size_t ar_tile = ((size_t)(epoch & 1u) * a.ar.world * a.ar.max_tiles + tile) * kArTileFloats;
-  // fp32 sum plus the column's bias (when given), rounded once
-  auto out_value = [&](int n, float v) {
+  // fp32 sum plus the column's bias (EPI: activated, plus the residual), rounded once
+  auto out_value = [&](int m, int n, float v) {
     if (a.bias) v += __half2float(a.bias[n]);
+    if constexpr (EPI) {
+      v = activate(v, a.act);
+      if (a.residual) v += __half2float(a.residual[(int64_t)m * a.ldr + n]);
+    }
     return __float2half_rn(v);
   };
   auto emit = [&](int idx, int m, int n, float v) {
     if (a.pair_strips > 0) {                           // parked for the SiLU-mul pair step
       a.pair_vals[(size_t)tile * slot_stride + idx] = a.bias ? v + __half2float(a.bias[n]) : v;
     } else if (!ar) {
-      a.out[(int64_t)(m0 + m) * a.ldo + n] = out_value(n, v);
+      a.out[(int64_t)(m0 + m) * a.ldo + n] = out_value(m0 + m, n, v);
     } else {
       const size_t off = ar_tile + (size_t)a.ar.rank * ar_rank_stride + idx;
 #pragma unroll
@@ -639,7 +647,7 @@ gemv_tma_kernel(const __grid_constant__ CUtensorMap tmW, const TmaGemvArgs a) {
         }
         v += __uint_as_float(e.x);                     // rank order
       }
-      a.out[(int64_t)(m0 + m) * a.ldo + n] = out_value(n, v);
+      a.out[(int64_t)(m0 + m) * a.ldo + n] = out_value(m0 + m, n, v);
     }
   }
   __syncthreads();
@@ -687,12 +695,12 @@ bool pdl_enabled() {
   return v == 1;
 }
 
-template <int TOKSETS>
+template <int TOKSETS, bool EPI>
 cudaError_t launch_t(const CUtensorMap& tm, const TmaGemvArgs& a, int grid, size_t smem,
                      cudaStream_t stream) {
   static PerDeviceOnce attr_once;
   const cudaError_t attr = attr_once.run([] {
-    return cudaFuncSetAttribute(gemv_tma_kernel<TOKSETS>,
+    return cudaFuncSetAttribute(gemv_tma_kernel<TOKSETS, EPI>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGemvTmaMaxSmem);
   });
   if (attr != cudaSuccess) return attr;
@@ -708,7 +716,7 @@ cudaError_t launch_t(const CUtensorMap& tm, const TmaGemvArgs& a, int grid, size
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, gemv_tma_kernel<TOKSETS>, tm, a);
+  return cudaLaunchKernelEx(&cfg, gemv_tma_kernel<TOKSETS, EPI>, tm, a);
 }
 
 }  // namespace
@@ -785,11 +793,13 @@ cudaError_t launch_gemv_tma(const GemvTmaPlan& p, const void* x, int64_t ldx,
                             const int32_t* qweight, const int32_t* qzeros, const void* scales,
                             void* out, int64_t ldo, int M, int N, int K, int group_size,
                             void* workspace, int* dev_status, cudaStream_t stream,
-                            const ArArgs* ar, const void* bias, bool silu_mul) {
+                            const ArArgs* ar, const void* bias, bool silu_mul,
+                            const EpiArgs* epi) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return cudaErrorNotSupported;
   if ((p.ws_bytes > 0 || silu_mul) && !workspace) return cudaErrorInvalidValue;
   if (silu_mul && (!gemv_tma_silu_ok(p, N) || (ar && ar->world > 1))) return cudaErrorInvalidValue;
+  if (epi && (silu_mul || ar)) return cudaErrorInvalidValue;
   CUtensorMap tm;
   cuuint64_t dims[2] = {(cuuint64_t)(N / 8), (cuuint64_t)K};
   cuuint64_t strides[1] = {(cuuint64_t)N / 2};
@@ -823,6 +833,9 @@ cudaError_t launch_gemv_tma(const GemvTmaPlan& p, const void* x, int64_t ldx,
   a.l2pf = pdl_enabled() ? kL2PrefetchStages : 0;
   a.status = dev_status;
   a.bias = static_cast<const __half*>(bias);
+  a.residual = epi ? static_cast<const __half*>(epi->residual) : nullptr;
+  a.ldr = epi ? epi->ldr : 0;
+  a.act = epi ? epi->act : kActNone;
   a.pair_strips = 0;
   a.pair_vals = nullptr;
   a.pair_cnt = nullptr;
@@ -841,8 +854,11 @@ cudaError_t launch_gemv_tma(const GemvTmaPlan& p, const void* x, int64_t ldx,
     a.ar = ArArgs{};
     a.ar.world = 1;
   }
-  return p.toksets == 1 ? launch_t<1>(tm, a, p.grid, p.smem, stream)
-                        : launch_t<2>(tm, a, p.grid, p.smem, stream);
+  if (epi)
+    return p.toksets == 1 ? launch_t<1, true>(tm, a, p.grid, p.smem, stream)
+                          : launch_t<2, true>(tm, a, p.grid, p.smem, stream);
+  return p.toksets == 1 ? launch_t<1, false>(tm, a, p.grid, p.smem, stream)
+                        : launch_t<2, false>(tm, a, p.grid, p.smem, stream);
 }
 
 }  // namespace awq

@@ -47,6 +47,16 @@ cudaError_t launch_dequant(const int32_t* qweight, const int32_t* qzeros, const 
 constexpr int kMaxCounters = 16384;
 constexpr size_t kCounterRegionBytes = kMaxCounters * sizeof(int);
 
+// Epilogue behind the bias: out = fp16(act(sum + bias) + residual), in fp32 up to the one
+// rounding.  residual fp16 [M, N] with row stride ldr (may be out itself: every kernel reads
+// an element's residual in the thread that then writes it), or null.
+enum Activation : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
+struct EpiArgs {
+  const void* residual = nullptr;
+  int64_t ldr = 0;
+  int act = kActNone;
+};
+
 // ---- decode / skinny GEMM on mma.sync (awq_gemv.cu) ----------------------------------
 struct GemvPlan {
   int strips;      // ceil(N / 256): one warp-wide strip of 32 packed words each
@@ -73,7 +83,7 @@ bool plan_gemv_bounded(int64_t M, int64_t N, int64_t K, int64_t group_size, int 
 cudaError_t launch_gemv(const GemvPlan& plan, const void* x, int64_t ldx, const int32_t* qweight,
                         const int32_t* qzeros, const void* scales, void* out, int64_t ldo, int M,
                         int N, int K, int group_size, void* workspace, cudaStream_t stream,
-                        const void* bias = nullptr);
+                        const void* bias = nullptr, const EpiArgs* epi = nullptr);
 
 // ---- decode on mma.sync with TMA streaming, one CTA per SM (awq_gemv_tma.cu) ---------
 // Shapes TMA can describe (N % 32 == 0, 16-byte aligned qweight and x, ldx % 8 == 0).
@@ -121,7 +131,7 @@ cudaError_t launch_gemv_tma(const GemvTmaPlan& plan, const void* x, int64_t ldx,
                             void* out, int64_t ldo, int M, int N, int K, int group_size,
                             void* workspace, int* dev_status, cudaStream_t stream,
                             const ArArgs* ar = nullptr, const void* bias = nullptr,
-                            bool silu_mul = false);
+                            bool silu_mul = false, const EpiArgs* epi = nullptr);
 bool gemv_tma_silu_ok(const GemvTmaPlan& plan, int64_t N);
 size_t gemv_tma_silu_ws_bytes(const GemvTmaPlan& plan);
 
@@ -141,7 +151,7 @@ cudaError_t launch_gemm_tc(const void* x, int64_t ldx, const int32_t* qweight,
                            int M, int N, int K, int group_size, int num_sms, int* dev_status,
                            cudaStream_t stream, const char** why, const void* bias = nullptr,
                            void* workspace = nullptr, size_t workspace_bytes = 0,
-                           bool silu = false);
+                           bool silu = false, const EpiArgs* epi = nullptr);
 // Split-K factor of the tcgen05 kernel and the workspace its fp32 partials need (0: none).
 // With less workspace than this the kernel runs one CTA per output tile.
 int tc_splits(int64_t M, int64_t N, int64_t K, int num_sms);
@@ -161,7 +171,7 @@ cudaError_t launch_gemm_ts(const void* x, int64_t ldx, const int32_t* qweight,
                            int M, int N, int K, int group_size, int num_sms, int* dev_status,
                            cudaStream_t stream, const char** why, const void* bias = nullptr,
                            void* workspace = nullptr, size_t workspace_bytes = 0,
-                           bool silu = false);
+                           bool silu = false, const EpiArgs* epi = nullptr);
 int ts_tokens(int64_t M);
 int ts_splits(int64_t M, int64_t N, int64_t K, int num_sms);
 size_t ts_workspace_bytes(int64_t M, int64_t N, int64_t K, int num_sms);

@@ -21,6 +21,10 @@ directory first on ``sys.path`` (``import kernels.awq_gemm``) or assign
   ``awq_gemm_forward`` + the two ``.contiguous()`` slices + ``silu_mul_forward`` of the
   reference MLP (``model/qwen2.py:181-194``, ``kernels/silu_mul.py:41-64``).  Output
   ``x.shape[:-1] + (N/2,)``.
+* ``awq_gemm_epilogue_forward(x, qweight, qzeros, scales, group_size=128, bias=None,
+  activation=None, residual=None)`` -- not in the reference: activation(product + bias) +
+  residual in one call, e.g. the residual adds behind o and down
+  (``model/qwen2.py:207-229``).
 * ``_dequant_to_fp16(qweight, qzeros, scales, out_buf, group_size=128)`` --
   reference ``kernels/awq_gemm.py:66-87``; writes the bit-identical fp16 weights.
 """
@@ -31,7 +35,7 @@ import torch
 import awq_b200
 
 __all__ = ["awq_gemm_forward", "awq_gemm_bias_forward", "awq_gemm_silu_mul_forward",
-           "_dequant_to_fp16"]
+           "awq_gemm_epilogue_forward", "_dequant_to_fp16"]
 
 
 def _dequant_to_fp16(qweight: torch.Tensor, qzeros: torch.Tensor, scales: torch.Tensor,
@@ -97,3 +101,26 @@ def awq_gemm_silu_mul_forward(x: torch.Tensor, qweight: torch.Tensor, qzeros: to
     N = scales.shape[1]
     out = awq_b200.gemm_silu_mul(x_flat, qweight, qzeros, scales, group_size)
     return out.view(*in_shape[:-1], N // 2)
+
+
+def awq_gemm_epilogue_forward(x: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor,
+                              scales: torch.Tensor, group_size: int = 128,
+                              bias: torch.Tensor | None = None, activation: str | None = None,
+                              residual: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(awq_gemm_forward(x, ...) + bias) + residual`` in one call: bias fp16 [N],
+    activation None, "relu", "silu", "gelu" or "gelu_tanh", residual fp16 of the output's
+    shape ``x.shape[:-1] + (N,)``; fp32 up to the single fp16 rounding."""
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if x.dim() < 1:
+        raise ValueError("x must have at least one dimension")
+    out_shape = (*x.shape[:-1], scales.shape[1])
+    if residual is not None:
+        if not isinstance(residual, torch.Tensor):
+            raise TypeError("residual must be a torch.Tensor")
+        if tuple(residual.shape) != out_shape:
+            raise ValueError(f"residual must be {out_shape}, got {tuple(residual.shape)}")
+        residual = residual.reshape(-1, out_shape[-1])
+    out = awq_b200.gemm_epilogue(x.reshape(-1, x.shape[-1]), qweight, qzeros, scales, group_size,
+                                 bias=bias, activation=activation, residual=residual)
+    return out.view(out_shape)
