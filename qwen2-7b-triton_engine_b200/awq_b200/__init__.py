@@ -350,7 +350,10 @@ def gemm_epilogue(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor
         need = _workspace_need(lib, dev, M, N, K, gs)
         ws = None
         if need and torch.cuda.is_current_stream_capturing():
-            ws = torch.zeros(need, dtype=torch.uint8, device=dev)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            # only the arrival counters at its head must start at zero
+            _lib.check(lib.awq_workspace_init(ws.data_ptr(), min(need, _lib.WS_COUNTER_BYTES),
+                                              stream.cuda_stream))
         elif need:
             ws = workspace_for(dev, need, stream)
         _lib.check(lib.awq_gemm_f16_epilogue(

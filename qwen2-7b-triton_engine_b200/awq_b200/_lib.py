@@ -25,6 +25,10 @@ AWQ_PATH_DECODE = 1
 AWQ_PATH_TC = 2
 AWQ_PATH_TS = 3
 
+# head of a split-K workspace that must start at zero (the arrival counters); the partial sums
+# behind it are always written before they are read
+WS_COUNTER_BYTES = 64 * 1024
+
 # activations of awq_gemm_f16_epilogue
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 

@@ -7,6 +7,9 @@
 //   o_G = ( sum_t (p_t s_tG) c_tG + sum_t p_t m_tG ) / sum_t p_t
 // so the tensor cores multiply fp16 queries, and fp16 weights p s, with the raw codes (fp16
 // subnormals, one AND per two codes), and scales and minima are applied per token in fp32.
+// The odd codes of a word sit four bits higher, times 2^-20; the queries they meet are scaled
+// by 1/16 for it, after an item's queries are scaled up together by a power of two so that
+// the largest lies just below fp16's limit and nothing that matters becomes subnormal.
 // The softmax reference M runs over log2(p s) rather than log2(p), so that the fp16 weights
 // stay below 2^8 and near the top of the range whatever the size of the value scales; sums,
 // statistics and accumulators are fp32.
@@ -16,8 +19,9 @@
 // query heads of a group waste one column in eight instead of nine rows in sixteen.
 //
 // Work split (kv4_attn_kernel): the (request, kv head, 8 NT query rows) items are cut into
-// tiles of 32 tokens, and the linear list of all tiles is dealt evenly to all warps of one
-// CTA per SM; ragged batches balance to within a tile.  A warp streams its tiles through
+// tiles of 64 tokens, and the linear list of all tiles is dealt evenly to all warps of one
+// CTA per SM; ragged batches balance to within a tile.  Every item has one empty tile more,
+// which stands for its fixed cost.  A warp streams its tiles through
 // its own ring of bulk copies (no CTA barrier in the loop).  Items that cross warps are
 // joined in the CTA at its end; items that cross CTAs by kv4_merge_kernel, in CTA order, so
 // results do not depend on timing.
@@ -36,7 +40,7 @@ namespace awq {
 
 namespace {
 
-constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kv4::kBlockTokens;
+constexpr int kTileBlocks = 4, kTileTokens = kTileBlocks * kv4::kBlockTokens;
 constexpr int kPrefixEntries = 1024;     // prefix sums held in shared memory
 constexpr int kDescInts = 8;
 
@@ -66,6 +70,42 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The scale / minimum half2 of a token's NG groups.
+template <int NG>
+__device__ __forceinline__ void load_params(uint32_t addr, uint32_t (&p)[NG]) {
+  if constexpr (NG == 4) {
+    const uint4 v = sm100::ld_shared_v4(addr);
+    p[0] = v.x, p[1] = v.y, p[2] = v.z, p[3] = v.w;
+  } else if constexpr (NG == 2) {
+    const uint2 v = sm100::ld_shared_v2(addr);
+    p[0] = v.x, p[1] = v.y;
+  } else {
+    p[0] = sm100::ld_shared_u32(addr);
+  }
+}
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t addr, uint32_t (&w)[W]) {
+  if constexpr (W == 4) {
+    const uint4 v = sm100::ld_shared_v4(addr);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = sm100::ld_shared_v2(addr);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -88,7 +128,7 @@ struct Geo {
   static constexpr int D = D_, GROUP = GROUP_, NT = NT_, WARPS = WARPS_;
   static constexpr int NG = D / GROUP, W = D / 32, ROWS = 8 * NT;
   static constexpr int BLK = kv4::block_bytes(D, GROUP), TILE = kTileBlocks * BLK;
-  static constexpr int BUDGET = 227 * 1024 - (kPrefixEntries + 1) * 4 - 4096;
+  static constexpr int BUDGET = 227 * 1024 - (kPrefixEntries + 8) * 4 - 3072;
   static constexpr int FIT = BUDGET / (WARPS * TILE);
   static constexpr int STAGES = FIT < 6 ? FIT : 6;
   static constexpr int SLOT = ROWS * (D + 2);          // floats: O [ROWS][D], M, l
@@ -96,7 +136,8 @@ struct Geo {
   static constexpr int OFF_BAR = OFF_PRE + (kPrefixEntries + 8) * 4 / 16 * 16;
   static constexpr int OFF_META = OFF_BAR + WARPS * STAGES * 8;
   static constexpr int OFF_ENT = (OFF_META + WARPS * STAGES * 4 + 15) / 16 * 16;
-  static constexpr int SMEM = OFF_ENT + WARPS * 2 * 40;
+  static constexpr int OFF_FAC = OFF_ENT + WARPS * 2 * 40;     // join: factor per part and column
+  static constexpr int SMEM = OFF_FAC + WARPS * 2 * ROWS * 4;
   static_assert(STAGES >= 2 && SLOT * 4 <= STAGES * TILE && SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -121,7 +162,7 @@ __device__ __forceinline__ Req request(const AttnArgs& a, int r) {
     x.q0 = r;
     x.n = 1;
   }
-  x.tiles = max(1, (x.L + kTileTokens - 1) / kTileTokens);
+  x.tiles = (x.L + kTileTokens - 1) / kTileTokens + 1;
   x.nrt = (x.n * a.G + ROWS - 1) / ROWS;
   return x;
 }
@@ -199,6 +240,7 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
   const uint32_t bar0 = sbase + G_::OFF_BAR + warp * STAGES * 8;
   __shared__ int wsum[WARPS];
   __shared__ int s_total;
+  __shared__ float top[ROWS];                            // join: largest M of the columns
 
   if (lane == 0) {
     for (int s = 0; s < STAGES; ++s) sm100::mbar_init(bar0 + 8 * s, 1);
@@ -253,42 +295,46 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
     lc.locate<ROWS>(a, pre, entries, shift, u0);
     Cursor cc = lc;
     const int bpp_shift = a.page_shift - 4;
-    auto page_of = [&](const Cursor& c, int b) -> int {   // page of block b of the tile
-      const int blk = c.tile * kTileBlocks + b;
-      if (blk * kv4::kBlockTokens >= c.vis) return -1;
+    // A tile's blocks lie in runs of `run` blocks, one page each; lane i < 4 / run copies run i.
+    const int run_shift = min(bpp_shift, 2);
+    auto page_of = [&](const Cursor& c) -> int {
+      const int blk = c.tile * kTileBlocks + (lane << run_shift);
+      if (lane >= (kTileBlocks >> run_shift) || blk * kv4::kBlockTokens >= c.vis) return -1;
       return a.table[c.r * a.table_rs + (blk >> bpp_shift)];
     };
-    int pid0 = page_of(lc, 0), pid1 = page_of(lc, 1);
-    int issued = u0;
+    int pid = page_of(lc);
+    int issued = u0, fill = 0;                          // fill: the next stage to fill
     auto issue = [&]() {
-      const int s = (issued - u0) % STAGES;
+      const int first = lane << run_shift;
+      const int nb = min(1 << run_shift, (lc.vis + kv4::kBlockTokens - 1) / kv4::kBlockTokens -
+                                             lc.tile * kTileBlocks - first);
+      const bool want = lane < (kTileBlocks >> run_shift) && nb > 0;
+      const bool have = want && pid >= 0 && pid < a.num_pages;
+      if (want && !have) atomicOr(a.status, kDevErrShape);
+      int ok = have ? ((1 << nb) - 1) << first : 0;      // blocks that arrive
+      ok |= __shfl_xor_sync(0xffffffffu, ok, 1);
+      ok |= __shfl_xor_sync(0xffffffffu, ok, 2);
+      const uint32_t bar = bar0 + 8 * fill;
       if (lane == 0) {
-        const int blk = lc.tile * kTileBlocks, nb = min(kTileBlocks, (lc.vis - blk * 16 + 15) / 16);
-        const int m = (1 << (a.page_shift - 4)) - 1;
-        const bool ok0 = nb > 0 && (unsigned long long)(long long)pid0 < (unsigned long long)a.num_pages;
-        const bool ok1 = nb > 1 && (unsigned long long)(long long)pid1 < (unsigned long long)a.num_pages;
-        if ((nb > 0 && !ok0) || (nb > 1 && !ok1)) atomicOr(a.status, kDevErrShape);
-        meta[s] = (int)ok0 | (int)ok1 << 1;
-        sm100::mbar_arrive_expect_tx(bar0 + 8 * s, ((int)ok0 + (int)ok1) * BLK);
-        const uint32_t dst = ring + s * TILE;
-        if (ok0)
-          bulk_load(dst, a.cache + ((((int64_t)pid0 * a.kv_heads + lc.h) << bpp_shift) + (blk & m)) * BLK,
-                    BLK, bar0 + 8 * s);
-        if (ok1)
-          bulk_load(dst + BLK,
-                    a.cache + ((((int64_t)pid1 * a.kv_heads + lc.h) << bpp_shift) + ((blk + 1) & m)) * BLK,
-                    BLK, bar0 + 8 * s);
+        meta[fill] = ok;
+        sm100::mbar_arrive_expect_tx(bar, __popc(ok) * BLK);
       }
-      ++issued;
-      if (issued < u1) {
+      __syncwarp();
+      if (have) {
+        const int at = (lc.tile * kTileBlocks + first) & ((1 << bpp_shift) - 1);
+        bulk_load(ring + fill * TILE + first * BLK,
+                  a.cache + ((((int64_t)pid * a.kv_heads + lc.h) << bpp_shift) + at) * BLK, nb * BLK, bar);
+      }
+      if (++fill == STAGES) fill = 0;
+      if (++issued < u1) {
         if (++lc.tile == lc.x.tiles) lc.next_item<ROWS>(a);
-        pid0 = page_of(lc, 0), pid1 = page_of(lc, 1);
+        pid = page_of(lc);
       }
     };
     for (int s = 0; s < STAGES && issued < u1; ++s) issue();
 
     bool dead = false;                                  // a wait ran out: stop working
-    int u = u0;
+    int u = u0, use = 0, phase = 0;                     // use: the stage to read next
     while (u < u1) {
       // ---- one item, or this warp's part of it ----------------------------------------
       const int rows = cc.x.n * a.G, row0 = cc.rt * ROWS;
@@ -296,6 +342,8 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
       uint32_t qa[NT][W][2], qb[NT][W][2];              // B operands: even / odd nibbles
       float qs[NT][NG][2];                              // scale * sum of q over the group
       int lim[NT][2];                                   // last visible token of the columns
+      uint4 qv[NT][W];
+      float big = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int row = row0 + nt * 8 + g;
@@ -303,18 +351,24 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
         const __half* qp = a.q + (in ? (int64_t)(cc.x.q0 + row / a.G) * a.q_ts +
                                            (int64_t)(cc.h * a.G + row % a.G) * a.q_hs
                                      : 0);
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          qv[nt][j] = make_uint4(0, 0, 0, 0);
+          if (in) qv[nt][j] = *reinterpret_cast<const uint4*>(qp + 8 * (4 * j + t));
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
         float sum[NG] = {};
 #pragma unroll
         for (int j = 0; j < W; ++j) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (in) v = *reinterpret_cast<const uint4*>(qp + 8 * (4 * j + t));
-          qa[nt][j][0] = __byte_perm(v.x, v.z, 0x5410);  // channels 0, 4
-          qb[nt][j][0] = __byte_perm(v.x, v.z, 0x7632);  // 1, 5
-          qa[nt][j][1] = __byte_perm(v.y, v.w, 0x5410);  // 2, 6
-          qb[nt][j][1] = __byte_perm(v.y, v.w, 0x7632);  // 3, 7
-          const float2 f0 = __half22float2(u32_as_h2(v.x)), f1 = __half22float2(u32_as_h2(v.y));
-          const float2 f2 = __half22float2(u32_as_h2(v.z)), f3 = __half22float2(u32_as_h2(v.w));
-          sum[j / GW] += ((f0.x + f0.y) + (f1.x + f1.y)) + ((f2.x + f2.y) + (f3.x + f3.y));
+          const uint32_t w4[4] = {qv[nt][j].x, qv[nt][j].y, qv[nt][j].z, qv[nt][j].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(u32_as_h2(w4[k]));
+            sum[j / GW] += f.x + f.y;
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
         }
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
@@ -328,177 +382,194 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
         for (int c = 0; c < 2; ++c)
           lim[nt][c] = cc.x.L - cc.x.n + (row0 + nt * 8 + 2 * t + c) / a.G;
       }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+      // 2^(15 - e) for the largest |q| in [2^e, 2^(e + 1)); 1 for zeros and infinities
+      const int e_big = (int)(__float_as_uint(big) >> 23) - 127;
+      const int up2 = big > 0.f && e_big <= 15 ? 15 - e_big : 0;
+      const float qmul = __uint_as_float((uint32_t)(127 + up2) << 23);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          const uint4 v = qv[nt][j];
+          const uint32_t even[2] = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410)};
+          const uint32_t odd[2] = {__byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x7632)};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {                  // channels (0, 4), (2, 6); (1, 5), (3, 7)
+            const float2 e = __half22float2(u32_as_h2(even[k])), o = __half22float2(u32_as_h2(odd[k]));
+            qa[nt][j][k] = h2_as_u32(__floats2half2_rn(e.x * qmul, e.y * qmul));
+            qb[nt][j][k] = h2_as_u32(__floats2half2_rn(o.x * (qmul * 0.0625f), o.y * (qmul * 0.0625f)));
+          }
+        }
       const int lim_all = cc.x.L - cc.x.n + row0 / a.G;  // every row sees tokens up to here
-      const float ksc = a.scale_log2 * 16777216.0f;      // codes enter the MMA times 2^-24
+      // codes enter the MMA times 2^-24, queries times qmul
+      const float ksc = a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - up2) << 23);
       float O[NT][2 * W][4] = {}, M[NT][2], l[NT][2] = {}, pm[NT][NG][2] = {};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) M[nt][0] = M[nt][1] = -CUDART_INF_F;
 
+      // One tile; EDGE: some of its tokens may be unseen (past a row's limit, or in a page the
+      // table does not name).
+      auto tile = [&](auto edge, uint32_t st, int tok0, int ok) {
+        constexpr bool EDGE = decltype(edge)::value;
+        float x[NT][kTileBlocks][4];                     // [block][token g / g + 8, column]
+        float ls[kTileBlocks][2];                        // log2 of a token's largest value scale
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) {
+          const uint32_t blk = st + b * BLK;
+          uint32_t k0[W], k1[W], p0[NG], p1[NG];
+          load_words<W>(blk + g * (D / 2) + t * (4 * W), k0);
+          load_words<W>(blk + (g + 8) * (D / 2) + t * (4 * W), k1);
+          load_params<NG>(blk + kv4::off_kp(D) + g * (4 * NG), p0);
+          load_params<NG>(blk + kv4::off_kp(D) + (g + 8) * (4 * NG), p1);
+#pragma unroll
+          for (int k = 0; k < NG; ++k) {
+            const float2 f0 = __half22float2(u32_as_h2(p0[k])), f1 = __half22float2(u32_as_h2(p1[k]));
+            const float s0 = f0.x * ksc, s1 = f1.x * ksc;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float acc[4];
+#pragma unroll
+              for (int j = k * GW; j < (k + 1) * GW; ++j) {
+                const uint32_t h0 = k0[j] >> 8, h1 = k1[j] >> 8;
+                if (j == k * GW)
+                  mma16816_first(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
+                                 qa[nt][j][0], qa[nt][j][1]);
+                else
+                  mma16816(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
+                           qa[nt][j][0], qa[nt][j][1]);
+                mma16816(acc, k0[j] & kHiMask, k1[j] & kHiMask, h0 & kHiMask, h1 & kHiMask,
+                         qb[nt][j][0], qb[nt][j][1]);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float m = i < 2 ? f0.y : f1.y, q1 = qs[nt][k][i & 1];
+                const float base = k == 0 ? m * q1 : fmaf(m, q1, x[nt][b][i]);
+                x[nt][b][i] = fmaf(acc[i], i < 2 ? s0 : s1, base);
+              }
+            }
+          }
+          if constexpr (EDGE) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (tok0 + b * 16 + g + (i / 2) * 8 > lim[nt][i & 1] || !((ok >> b) & 1))
+                  x[nt][b][i] = -CUDART_INF_F;
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t pv[NG];
+            load_params<NG>(blk + kv4::off_vp(D, G_::GROUP) + (g + 8 * e) * (4 * NG), pv);
+            float top = 5.9604645e-8f;                   // 2^-24, fp16's least scale
+#pragma unroll
+            for (int k = 0; k < NG; ++k) top = fmaxf(top, __low2float(u32_as_h2(pv[k])));
+            ls[b][e] = lg2(top);
+          }
+        }
+        // the softmax reference moves only when it is more than 2^8 behind (the fp16 weights
+        // then reach 2^8 at most); -inf + 8 = -inf, so the first visible token sets it
+        bool up = false;
+        float nm[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float m = fmaxf(x[nt][0][c] + ls[0][0], x[nt][0][2 + c] + ls[0][1]);
+#pragma unroll
+            for (int b = 1; b < kTileBlocks; ++b)
+              m = fmaxf(m, fmaxf(x[nt][b][c] + ls[b][0], x[nt][b][2 + c] + ls[b][1]));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            nm[nt][c] = m;
+            up |= m > M[nt][c] + 8.0f;
+          }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float m = fmaxf(M[nt][c], nm[nt][c]);
+              f[c] = M[nt][c] == m ? 1.0f : ex2(M[nt][c] - m);
+              M[nt][c] = m;
+              l[nt][c] *= f[c];
+#pragma unroll
+              for (int k = 0; k < NG; ++k) pm[nt][k][c] *= f[c];
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * W; ++i) {
+              O[nt][i][0] *= f[0], O[nt][i][1] *= f[1];
+              O[nt][i][2] *= f[0], O[nt][i][3] *= f[1];
+            }
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; ++b) {
+          const uint32_t blk = st + b * BLK;
+          uint32_t wb[NT][NG][2];                        // B operands: weights p s per group
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t pv[NG];
+            load_params<NG>(blk + kv4::off_vp(D, G_::GROUP) + (g + 8 * e) * (4 * NG), pv);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float p[2];
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                p[c] = ex2(x[nt][b][2 * e + c] - (EDGE && M[nt][c] == -CUDART_INF_F ? 0.f : M[nt][c]));
+                l[nt][c] += p[c];
+              }
+#pragma unroll
+              for (int k = 0; k < NG; ++k) {
+                const float2 f = __half22float2(u32_as_h2(pv[k]));
+                float w[2];
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  // an unseen token's scale and minimum may be anything: no 0 * NaN
+                  const bool seen = !EDGE || p[c] != 0.f;
+                  w[c] = seen ? p[c] * f.x : 0.f;
+                  pm[nt][k][c] = seen ? fmaf(p[c], f.y, pm[nt][k][c]) : pm[nt][k][c];
+                }
+                wb[nt][k][e] = movmatrix(h2_as_u32(__floats2half2_rn(w[0], w[1])));
+              }
+            }
+          }
+          uint32_t v0[W], v1[W];
+          load_words<W>(blk + kv4::off_v(D) + t * D + g * (4 * W), v0);
+          load_words<W>(blk + kv4::off_v(D) + (t + 4) * D + g * (4 * W), v1);
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            const uint32_t h0 = v0[i] >> 8, h1 = v1[i] >> 8;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816(O[nt][2 * i], v0[i] & kLoMask, h0 & kLoMask, v1[i] & kLoMask, h1 & kLoMask,
+                       wb[nt][i / GW][0], wb[nt][i / GW][1]);
+              mma16816(O[nt][2 * i + 1], v0[i] & kHiMask, h0 & kHiMask, v1[i] & kHiMask, h1 & kHiMask,
+                       wb[nt][i / GW][0], wb[nt][i / GW][1]);
+            }
+          }
+        }
+      };
+
       for (; u < ue; ++u) {
-        const int s = (u - u0) % STAGES;
         if (!dead) {                                     // one verdict for the whole warp
-          const bool got = sm100::mbar_wait_bounded(bar0 + 8 * s, ((u - u0) / STAGES) & 1, a.status);
+          const bool got = sm100::mbar_wait_bounded(bar0 + 8 * use, phase, a.status);
           dead = __any_sync(0xffffffffu, !got);
         }
         const int tok0 = cc.tile * kTileTokens;
-        const int ok = dead ? 0 : *(volatile int*)(meta + s);
+        const int ok = dead ? 0 : *(volatile int*)(meta + use);
         ++cc.tile;
         if (ok) {
-          const uint32_t st = ring + s * TILE;
-          float x[NT][2][4];                             // [block][token g / g + 8, column]
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t kp = st + b * BLK + g * (D / 2) + t * (4 * W);
-            uint32_t k0[W], k1[W];
-            if constexpr (W == 4) {
-              const uint4 v0 = sm100::ld_shared_v4(kp), v1 = sm100::ld_shared_v4(kp + 8 * (D / 2));
-              k0[0] = v0.x, k0[1] = v0.y, k0[2] = v0.z, k0[3] = v0.w;
-              k1[0] = v1.x, k1[1] = v1.y, k1[2] = v1.z, k1[3] = v1.w;
-            } else {
-              const uint2 v0 = sm100::ld_shared_v2(kp), v1 = sm100::ld_shared_v2(kp + 8 * (D / 2));
-              k0[0] = v0.x, k0[1] = v0.y, k1[0] = v1.x, k1[1] = v1.y;
-            }
-            const uint32_t pp = st + b * BLK + kv4::off_kp(D) + g * (4 * NG);
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-              const float2 p0 = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 4 * k)));
-              const float2 p1 = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 8 * 4 * NG + 4 * k)));
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float ea[4] = {}, od[4] = {};
-#pragma unroll
-                for (int j = k * GW; j < (k + 1) * GW; ++j) {
-                  const uint32_t s0 = k0[j] >> 8, s1 = k1[j] >> 8;
-                  mma16816(ea, k0[j] & kLoMask, k1[j] & kLoMask, s0 & kLoMask, s1 & kLoMask,
-                           qa[nt][j][0], qa[nt][j][1]);
-                  mma16816(od, k0[j] & kHiMask, k1[j] & kHiMask, s0 & kHiMask, s1 & kHiMask,
-                           qb[nt][j][0], qb[nt][j][1]);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 p = i < 2 ? p0 : p1;
-                  const float dot = fmaf(od[i], 0.0625f, ea[i]) * ksc;
-                  const float v = fmaf(dot, p.x, p.y * qs[nt][k][i & 1]);
-                  x[nt][b][i] = k == 0 ? v : x[nt][b][i] + v;
-                }
-              }
-            }
-          }
-          // tokens past a row's limit, or in a page the table does not name, are not seen
-          if (tok0 + kTileTokens - 1 > lim_all || ok != 3) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  if (tok0 + b * 16 + g + (i / 2) * 8 > lim[nt][i & 1] || !((ok >> b) & 1))
-                    x[nt][b][i] = -CUDART_INF_F;
-          }
-          // value scales and minima; the softmax reference follows x + log2(largest scale)
-          float2 vp[2][2][NG];
-          float ls[2][2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t pp = st + b * BLK + kv4::off_vp(D, G_::GROUP) + (g + 8 * e) * (4 * NG);
-              float big = 5.9604645e-8f;                 // 2^-24, fp16's least scale
-#pragma unroll
-              for (int k = 0; k < NG; ++k) {
-                vp[b][e][k] = __half22float2(u32_as_h2(sm100::ld_shared_u32(pp + 4 * k)));
-                big = fmaxf(big, vp[b][e][k].x);
-              }
-              ls[b][e] = __log2f(big);
-            }
-          bool up = false;
-          float nm[NT][2];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float m = fmaxf(fmaxf(x[nt][0][c] + ls[0][0], x[nt][0][2 + c] + ls[0][1]),
-                              fmaxf(x[nt][1][c] + ls[1][0], x[nt][1][2 + c] + ls[1][1]));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-              nm[nt][c] = m;
-              up |= m > M[nt][c] + 8.0f;
-            }
-          // the reference moves only when it is more than 2^8 behind (the fp16 weights then
-          // reach 2^8 at most); -inf + 8 = -inf, so the first visible token sets it
-          if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float f[2];
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                const float m = fmaxf(M[nt][c], nm[nt][c]);
-                f[c] = M[nt][c] == m ? 1.0f : ex2(M[nt][c] - m);
-                M[nt][c] = m;
-                l[nt][c] *= f[c];
-#pragma unroll
-                for (int k = 0; k < NG; ++k) pm[nt][k][c] *= f[c];
-              }
-#pragma unroll
-              for (int i = 0; i < 2 * W; ++i) {
-                O[nt][i][0] *= f[0], O[nt][i][1] *= f[1];
-                O[nt][i][2] *= f[0], O[nt][i][3] *= f[1];
-              }
-            }
-          }
-          uint32_t wb[NT][2][NG][2];                     // B operands: weights p s per group
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float p[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  p[c] = ex2(x[nt][b][2 * e + c] - (M[nt][c] == -CUDART_INF_F ? 0.f : M[nt][c]));
-                  l[nt][c] += p[c];
-                }
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                  // an unseen token's scale and minimum may be anything: no 0 * NaN
-                  float w[2];
-#pragma unroll
-                  for (int c = 0; c < 2; ++c) {
-                    const bool seen = p[c] != 0.f;
-                    w[c] = seen ? p[c] * vp[b][e][k].x : 0.f;
-                    pm[nt][k][c] += seen ? p[c] * vp[b][e][k].y : 0.f;
-                  }
-                  wb[nt][b][k][e] = movmatrix(h2_as_u32(__floats2half2_rn(w[0], w[1])));
-                }
-              }
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const uint32_t vq = st + b * BLK + kv4::off_v(D) + t * D + g * (4 * W);
-            uint32_t v0[W], v1[W];
-            if constexpr (W == 4) {
-              const uint4 y0 = sm100::ld_shared_v4(vq), y1 = sm100::ld_shared_v4(vq + 4 * D);
-              v0[0] = y0.x, v0[1] = y0.y, v0[2] = y0.z, v0[3] = y0.w;
-              v1[0] = y1.x, v1[1] = y1.y, v1[2] = y1.z, v1[3] = y1.w;
-            } else {
-              const uint2 y0 = sm100::ld_shared_v2(vq), y1 = sm100::ld_shared_v2(vq + 4 * D);
-              v0[0] = y0.x, v0[1] = y0.y, v1[0] = y1.x, v1[1] = y1.y;
-            }
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-              const uint32_t s0 = v0[i] >> 8, s1 = v1[i] >> 8;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816(O[nt][2 * i], v0[i] & kLoMask, s0 & kLoMask, v1[i] & kLoMask, s1 & kLoMask,
-                         wb[nt][b][i / GW][0], wb[nt][b][i / GW][1]);
-                mma16816(O[nt][2 * i + 1], v0[i] & kHiMask, s0 & kHiMask, v1[i] & kHiMask,
-                         s1 & kHiMask, wb[nt][b][i / GW][0], wb[nt][b][i / GW][1]);
-              }
-            }
-          }
+          if (tok0 + kTileTokens - 1 > lim_all || ok != (1 << kTileBlocks) - 1)
+            tile(std::true_type{}, ring + use * TILE, tok0, ok);
+          else
+            tile(std::false_type{}, ring + use * TILE, tok0, ok);
         }
         __syncwarp();                                    // the stage is read: refill it
+        if (++use == STAGES) use = 0, phase ^= 1;
         if (issued < u1 && !dead) issue();
       }
 
@@ -558,7 +629,7 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
       if (u < u1) cc.next_item<ROWS>(a);
     }
     if (dead)                                            // copies in flight land before the exit
-      for (int k = u0 > issued - STAGES ? u0 : issued - STAGES; k < issued; ++k)
+      for (int k = max(u0, issued - STAGES); k < issued; ++k)
         sm100::mbar_wait_bounded(bar0 + 8 * ((k - u0) % STAGES), ((k - u0) / STAGES) & 1, nullptr, 100000000ull);
   }
   sm100::grid_launch_dependents();
@@ -566,6 +637,7 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
 
   // ---- join the items that cross this CTA's warps, in order ------------------------------
   const int cs = first_unit((long long)cta * WARPS), ce = first_unit((long long)(cta + 1) * WARPS);
+  float* fac = reinterpret_cast<float*>(smem + G_::OFF_FAC);
   int span = 0;
   Entry head = {};
   int i = 0;
@@ -584,17 +656,30 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
       span = (int)(((long long)e0.ie * Wt - 1) / U / WARPS) - cta + 1;
       head = e0;
     }
+    // factors 2^(M_k - M) of the parts, one thread per (part, column)
+    for (int idx = tid; idx < (last - i + 1) * ROWS; idx += WARPS * 32) {
+      const int k = i + idx / ROWS, col = idx % ROWS;
+      float m = -CUDART_INF_F, mine = -CUDART_INF_F;
+      for (int n = i; n <= last; ++n)
+        if (ent[n].ptr) {
+          const float v = ent[n].ptr[ROWS * D + col];
+          m = fmaxf(m, v);
+          if (n == k) mine = v;
+        }
+      fac[idx] = mine == m ? 1.0f : ex2(mine - m);
+      if (k == i) top[col] = m;
+    }
+    __syncthreads();
     for (int idx = tid; idx < ROWS * (D / 4); idx += WARPS * 32) {
       const int col = idx / (D / 4), ch = (idx - col * (D / 4)) * 4, row = e0.row0 + col;
-      float m = -CUDART_INF_F;
-      for (int k = i; k <= last; ++k)
-        if (ent[k].ptr) m = fmaxf(m, ent[k].ptr[ROWS * D + col]);
+      const float m = top[col];
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       float l = 0.f;
+#pragma unroll 4
       for (int k = i; k <= last; ++k) {
         const float* p = ent[k].ptr;
         if (!p) continue;
-        const float mk = p[ROWS * D + col], f = mk == m ? 1.0f : ex2(mk - m);
+        const float f = fac[(k - i) * ROWS + col];
         const float4 v = *reinterpret_cast<const float4*>(p + col * D + ch);
         l = fmaf(f, p[ROWS * D + ROWS + col], l);
         o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y);
@@ -612,6 +697,7 @@ __global__ void __launch_bounds__(G_::WARPS * 32, 1) kv4_attn_kernel(const AttnA
         if (ch == 0) slot[ROWS * D + col] = m, slot[ROWS * D + ROWS + col] = l;
       }
     }
+    __syncthreads();                                     // fac is free again
     i = j;
   }
   if (tid == 0) {
@@ -672,7 +758,11 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const 
                                                       h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
 }
 
-constexpr int kWarps1 = 16, kWarps2 = 8;
+// Warps of a CTA: two 64-token stages each must fit shared memory (D = 128 in groups of 32:
+// 10 KB a stage), and 16 query rows need twice the accumulators.
+constexpr int kWarps1 = 12, kWarps1Wide = 10, kWarps2 = 8;
+// warp slots of either kernel, in rows
+constexpr int kSlotRows = kWarps1 * 8 > kWarps2 * 16 ? kWarps1 * 8 : kWarps2 * 16;
 
 template <class G_>
 cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
@@ -699,15 +789,16 @@ cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
 
 template <int D, int GROUP>
 cudaError_t launch_rows(const AttnArgs& a, int max_rows, int num_sms, cudaStream_t stream) {
-  if (max_rows <= 8) return launch_geo<Geo<D, GROUP, 1, kWarps1>>(a, num_sms, stream);
+  constexpr int warps1 = D / GROUP == 4 ? kWarps1Wide : kWarps1;
+  if (max_rows <= 8) return launch_geo<Geo<D, GROUP, 1, warps1>>(a, num_sms, stream);
   return launch_geo<Geo<D, GROUP, 2, kWarps2>>(a, num_sms, stream);
 }
 
 }  // namespace
 
 size_t kv4_attention_workspace(int head_dim, int num_sms) {
-  // descriptors, 2 slots per CTA and one per warp: 8 x 16 warps and 16 x 8 warps alike
-  const size_t slots = (size_t)num_sms * (2 * 16 + kWarps1 * 8);
+  // descriptors, 2 slots per CTA (up to 16 rows) and one per warp
+  const size_t slots = (size_t)num_sms * (2 * 16 + kSlotRows);
   return (size_t)num_sms * kDescInts * 4 + slots * (head_dim + 2) * 4;
 }
 
