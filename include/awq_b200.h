@@ -240,10 +240,11 @@ AWQ_API int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64
  * rows of a request (a hint for the choice of kernel).  Tokens in a page outside
  * 0 .. num_pages - 1 are not seen, kv_lens is clipped to the table, a request whose cu_q is
  * not ascending within 0 .. tokens is left out; each sets status bit 2.  The workspace
- * (awq_kv4_attention_workspace_bytes, 16-byte aligned) needs no initialisation; calls that
- * may overlap on the GPU need different ones.
+ * (awq_kv4_attention_workspace_bytes with max_rows = min(max_q, tokens) * q_heads / kv_heads,
+ * 16-byte aligned) needs no initialisation; calls that may overlap on the GPU need different
+ * ones.
  */
-AWQ_API size_t awq_kv4_attention_workspace_bytes(int64_t head_dim);
+AWQ_API size_t awq_kv4_attention_workspace_bytes(int64_t head_dim, int64_t max_rows);
 AWQ_API int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                               int64_t tokens, int64_t q_heads, const void* cache,
                               int64_t num_pages, int64_t kv_heads, int64_t head_dim,

@@ -74,7 +74,7 @@ SIGNATURES = {
     "awq_kv4_gather": ([_P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _P, _P, _P], _INT),
     "awq_kv4_pages_step": ([_P, _I64, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _P, _P,
                             _I64, _P, _P, _P, _P], _INT),
-    "awq_kv4_attention_workspace_bytes": ([_I64], _SZ),
+    "awq_kv4_attention_workspace_bytes": ([_I64, _I64], _SZ),
     "awq_kv4_attention": ([_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P,
                            _I64, _I64, _P, _P, _I64, _I64, ctypes.c_float, _P, _I64, _I64, _P,
                            _SZ, _P], _INT),

@@ -323,7 +323,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
         return out
     lib = _lib.load()
     with _core()._DeviceGuard(dev):
-        need = _attention_workspace(lib, dev, D)
+        need = _attention_workspace(lib, dev, D, min(max_q, T) * (H // cache.kv_heads))
         # a workspace of this call alone: graphs that replay at once must not share one
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         _lib.check(lib.awq_kv4_attention(
@@ -339,11 +339,11 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
 _attn_ws: dict = {}
 
 
-def _attention_workspace(lib, dev: torch.device, head_dim: int) -> int:
-    key = (dev.index, head_dim)
+def _attention_workspace(lib, dev: torch.device, head_dim: int, max_rows: int) -> int:
+    key = (dev.index, head_dim, max_rows)
     need = _attn_ws.get(key)
     if need is None:
-        need = int(lib.awq_kv4_attention_workspace_bytes(head_dim))
-        if need:
+        need = int(lib.awq_kv4_attention_workspace_bytes(head_dim, max_rows))
+        if need and len(_attn_ws) < 65536:
             _attn_ws[key] = need
     return need

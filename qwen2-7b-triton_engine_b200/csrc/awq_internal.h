@@ -202,6 +202,11 @@ struct Kv4PagesCall {
 };
 cudaError_t launch_kv4_pages(const Kv4PagesCall& c, cudaStream_t stream);
 
+namespace kv4 {
+struct AttnArgs;
+}
+cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, int head_dim, int group, int num_sms,
+                               cudaStream_t stream);
 struct Kv4AttnCall {
   Kv4Shape cache;
   const void* data;
@@ -218,7 +223,10 @@ struct Kv4AttnCall {
   float scale;
   void* workspace;
 };
-size_t kv4_attention_workspace(int head_dim, int num_sms);
+// Query rows per kv head (tokens x heads of a group) from which a request runs on the
+// tcgen05 kernel, and the rows of one of that kernel's items.
+constexpr int kKv4PrefillMinRows = 64, kKv4PrefillRows = 256;
+size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms);
 cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
                                  cudaStream_t stream);
 

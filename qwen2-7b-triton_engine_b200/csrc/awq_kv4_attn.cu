@@ -34,32 +34,16 @@
 #include "awq_common.cuh"
 #include "awq_internal.h"
 #include "awq_kv4.cuh"
+#include "awq_kv4_args.cuh"
 #include "awq_sm100.cuh"
 
 namespace awq {
 
 namespace {
 
-constexpr int kPrefixEntries = 1024;     // prefix sums held in shared memory
-constexpr int kDescInts = 8;
-
-struct AttnArgs {
-  const uint8_t* cache;
-  const __half* q;
-  __half* out;
-  const int32_t* table;
-  const int32_t* lens;
-  const int32_t* cu_q;
-  int64_t q_ts, q_hs, o_ts, o_hs, table_rs;
-  int64_t num_pages;
-  int64_t tokens;
-  float* part;        // [ctas][2] slots of items that cross CTAs
-  float* warp_part;   // [ctas][warps] slots of items that cross warps, not a warp's last
-  int* desc;          // [ctas][kDescInts]
-  int* status;
-  float scale_log2;
-  int R, width, page_shift, kv_heads, G;
-};
+using kv4::AttnArgs;
+using kv4::kDescInts;
+using kv4::kPrefixEntries;
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -156,6 +140,7 @@ __device__ __forceinline__ Req request(const AttnArgs& a, int r) {
     x.q0 = r;
     x.n = 1;
   }
+  if ((long long)x.n * a.G >= a.min_rows) x.n = 0;      // the prefill kernel's request
   x.tiles = (x.L + G_::TOKENS - 1) / G_::TOKENS + 1;
   x.nrt = (x.n * a.G + G_::ROWS - 1) / G_::ROWS;
   return x;
@@ -809,7 +794,7 @@ cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
 }
 
 template <int D, int GROUP>
-cudaError_t launch_rows(const AttnArgs& a, int max_rows, int num_sms, cudaStream_t stream) {
+cudaError_t launch_rows(const AttnArgs& a, int64_t max_rows, int num_sms, cudaStream_t stream) {
   // two stages must fit shared memory: 32-token tiles where a 64-token one takes 10 KB
   constexpr int tb = D / GROUP == 4 ? 2 : 4;
   if (max_rows <= 8) return launch_geo<Geo<D, GROUP, 1, tb, kWarps1>>(a, num_sms, stream);
@@ -818,10 +803,11 @@ cudaError_t launch_rows(const AttnArgs& a, int max_rows, int num_sms, cudaStream
 
 }  // namespace
 
-size_t kv4_attention_workspace(int head_dim, int num_sms) {
-  // descriptors, 2 slots per CTA (up to 16 rows) and one per warp
-  const size_t slots = (size_t)num_sms * (2 * 16 + kSlotRows);
-  return (size_t)num_sms * kDescInts * 4 + slots * (head_dim + 2) * 4;
+size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms) {
+  // descriptors, 2 slots per CTA (up to 16 rows) and one per warp; or the prefill kernel's 2
+  // slots of 256 rows per CTA (the two kernels of a call run one after the other)
+  const int rows = max_rows >= kKv4PrefillMinRows ? 2 * kKv4PrefillRows : 2 * 16 + kSlotRows;
+  return (size_t)num_sms * (kDescInts * 4 + (size_t)rows * (head_dim + 2) * 4);
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
@@ -839,8 +825,16 @@ cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_sta
   a.R = c.rows, a.width = c.width, a.kv_heads = c.cache.heads, a.G = c.q_heads / c.cache.heads;
   a.page_shift = 0;
   while ((1 << a.page_shift) < c.cache.page) ++a.page_shift;
-  const int max_rows = c.max_q * a.G;
+  int64_t max_rows = (int64_t)c.max_q * a.G;
   const int D = c.cache.dim, g = c.cache.group;
+  a.min_rows = 0x7fffffff;
+  if (max_rows >= kKv4PrefillMinRows) {
+    // requests with many query rows, then those with few, which share no output row
+    a.min_rows = kKv4PrefillMinRows;
+    const cudaError_t e = launch_kv4_prefill(a, D, g, num_sms, stream);
+    if (e != cudaSuccess) return e;
+    max_rows = a.G;                                      // decode rows are the ones to be fast
+  }
   if (D == 64 && g == 32) return launch_rows<64, 32>(a, max_rows, num_sms, stream);
   if (D == 64 && g == 64) return launch_rows<64, 64>(a, max_rows, num_sms, stream);
   if (D == 128 && g == 32) return launch_rows<128, 32>(a, max_rows, num_sms, stream);

@@ -1,0 +1,844 @@
+// awq_kv4_prefill.cu -- attention of many query rows over the paged 4-bit key/value cache, on
+// tcgen05.  Same mathematics as awq_kv4_attn.cu, for requests with many query rows per kv
+// head (prompt chunks), where the tensor work binds instead of the cache's bytes.
+//
+// One CTA works on 256 query rows (two row tiles A and B of 128) of a request's kv head, over
+// steps of NTOK = 128 / NG tokens (NG scale groups per head):
+//   S_g [128 x NTOK] = Q_g [128 x group] . C_g^T      codes as fp16 integers (subnormals)
+//   x = scale sum_g (s_tg S_g + m_tg sum q_g)          fp32, one thread per query row
+//   P_g = fp16(2^(x - M) v_tg)                         value scales, reference M as there
+//   O_g [128 x group] += P_g . C'_g
+// so keys and values are never rounded: scales and minima are applied in fp32.  One group
+// (NG = 1) is a plain flash step of 128 tokens; more groups trade tokens for accumulators, so
+// that S always takes 128 columns of tensor memory, P 64 of them (over S, once it is read)
+// and O head_dim: 2 x 256 columns in all.
+//
+// Roles (16 warps): two softmax warpgroups (one per row tile, one row per thread, so no
+// shuffles), one warpgroup that spreads the packed codes into the MMAs' K-major 128-byte
+// swizzled operands, a warp that issues the MMAs and one that fetches cache blocks with bulk
+// copies.  While one tile's softmax runs, the tensor core works on the other tile.
+//
+// Work split: items (request, kv head, 256 rows) are cut into steps, causal lengths counted
+// per item, and every CTA (one per SM) takes an equal share of the list of steps; items that
+// cross CTAs are joined by kv4_prefill_merge in CTA order.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+
+#include "awq_common.cuh"
+#include "awq_internal.h"
+#include "awq_kv4.cuh"
+#include "awq_kv4_args.cuh"
+#include "awq_sm100.cuh"
+
+namespace awq {
+
+namespace {
+
+using kv4::AttnArgs;
+using kv4::kDescInts;
+using kv4::kPrefixEntries;
+
+constexpr int kThreads = 512;
+constexpr int kRows = kKv4PrefillRows;   // 256: query rows of an item, two tiles of 128
+constexpr int kKvSlots = 3, kRawStages = 2, kParStages = 2;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+template <int D_, int GROUP_>
+struct Geo {
+  static constexpr int D = D_, GROUP = GROUP_, NG = D / GROUP;
+  static constexpr int NTOK = 128 / NG, NBLK = NTOK / 16, BLK = kv4::block_bytes(D, GROUP);
+  static constexpr int RAW = NBLK * BLK;               // a step's cache blocks
+  static constexpr int KA = D / 64;                    // 64-channel atoms of Q and K rows
+  static constexpr int VA = (NTOK + 63) / 64;          // 64-token atoms of V rows
+  static constexpr int QTILE = KA * 128 * 128, KSLOT = KA * NTOK * 128, VSLOT = VA * D * 128;
+  static constexpr int SLOT = KSLOT > VSLOT ? KSLOT : VSLOT;
+  static constexpr int PAR = 4 * 128 * 4 + NTOK * 4;   // ks, km, vs, vm [NG][NTOK], ls [NTOK]
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_KV = OFF_Q + 2 * QTILE;
+  static constexpr int OFF_RAW = OFF_KV + kKvSlots * SLOT;
+  static constexpr int OFF_PAR = OFF_RAW + kRawStages * RAW;
+  static constexpr int OFF_PRE = OFF_PAR + kParStages * PAR;
+  static constexpr int OFF_BAR = OFF_PRE + (kPrefixEntries + 8) * 4;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;    // + alignment slack
+  static_assert(SMEM <= 227 * 1024 && QTILE % 1024 == 0 && SLOT % 1024 == 0 && RAW % 16 == 0 &&
+                    PAR % 16 == 0, "shared memory");
+};
+enum Bar { RAW_FULL = 0, RAW_EMPTY = 2, KV_FULL = 4, KV_EMPTY = 7, PAR_FULL = 10, PAR_EMPTY = 12,
+           Q_READY = 14, S_FULL = 16, P_READY = 18, O_FULL = 20, DRAIN = 22, NBARS = 23 };
+
+// A request's items: nrt row tiles of 256 per kv head, each with its causal number of steps
+// and one empty step that stands for its fixed cost.
+struct Item {
+  int L, n, q0, nrt;
+  int r, h, rt, step;
+  int vis, steps;
+
+  template <class G_>
+  __device__ void request(const AttnArgs& a) {
+    const int cap = (int)min((long long)a.width << a.page_shift, 0x7fffff00LL);
+    L = min(max(a.lens[r], 0), cap);
+    n = q0 = 0;
+    if (a.cu_q) {
+      const int b = a.cu_q[r], e = a.cu_q[r + 1];
+      if (b >= 0 && e >= b && e <= a.tokens) q0 = b, n = e - b;
+    } else {
+      q0 = r, n = 1;
+    }
+    if ((long long)n * a.G < a.min_rows) n = 0;         // the other kernel's request
+    nrt = (int)(((long long)n * a.G + kRows - 1) / kRows);
+  }
+  template <class G_>
+  __device__ int steps_of(const AttnArgs& a, int tile, int* seen) const {
+    const int last = min(n - 1, (int)(((long long)(tile + 1) * kRows - 1) / a.G));
+    *seen = max(0, L - n + last + 1);
+    return (*seen + G_::NTOK - 1) / G_::NTOK + 1;
+  }
+  template <class G_>
+  __device__ int units(const AttnArgs& a) const {       // of one kv head
+    int s = 0, v;
+    for (int i = 0; i < nrt; ++i) s += steps_of<G_>(a, i, &v);
+    return s;
+  }
+  template <class G_>
+  __device__ void next(const AttnArgs& a) {
+    step = 0;
+    if (++rt == nrt) {
+      rt = 0;
+      if (++h == a.kv_heads) {
+        h = 0;
+        do {
+          if (++r >= a.R) return;
+          request<G_>(a);
+        } while (nrt == 0);
+      }
+    }
+    steps = steps_of<G_>(a, rt, &vis);
+  }
+};
+
+// This CTA's part of an item.
+struct Segment {
+  int k0, count;        // first step, steps with tokens
+  bool skip, whole, starts;
+  bool two;             // the second row tile has rows
+  __device__ Segment(const Item& it, const AttnArgs& a, int u, int u0, int u1) {
+    const int ib = u - it.step, real = it.steps - 1;
+    k0 = it.step;
+    count = max(0, min(real, k0 + u1 - u) - k0);
+    skip = real > 0 && count == 0;                       // only the empty step is left
+    starts = ib >= u0;
+    whole = starts && ib + max(1, real) <= u1;
+    two = (long long)it.n * a.G > (long long)it.rt * kRows + 128;
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// Two fp32 lanes in one instruction.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// Byte offset of 16-byte chunk c (0..7) of a 128-byte row under the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swz(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
+
+template <class G_>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs a) {
+  constexpr int D = G_::D, GROUP = G_::GROUP, NG = G_::NG, NTOK = G_::NTOK, NBLK = G_::NBLK;
+  constexpr int BLK = G_::BLK, PAR = G_::PAR;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (sm100::smem_u32(smem_raw) & 1023)) & 1023);
+  const uint32_t sbase = sm100::smem_u32(smem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  int* pre = reinterpret_cast<int*>(smem + G_::OFF_PRE);
+  const uint32_t bars = sbase + G_::OFF_BAR;
+  __shared__ int wsum[kThreads / 32];
+  __shared__ int s_total;
+  __shared__ volatile int s_abort;
+  __shared__ uint32_t s_tmem;
+  __shared__ Item s_first;
+  __shared__ int raw_ok[kRawStages], par_ok[kParStages];   // blocks of the step that are there
+
+  if (tid == 0) {
+    s_total = 0, s_abort = 0;
+    for (int i = 0; i < NBARS; ++i) {
+      int count = 1;                                     // bulk copies, MMA commits
+      if (i >= RAW_EMPTY && i < RAW_EMPTY + 2) count = 128;
+      if (i >= KV_FULL && i < KV_FULL + 3) count = 128;
+      if (i >= PAR_FULL && i < PAR_FULL + 2) count = 128;
+      if (i >= PAR_EMPTY && i < PAR_EMPTY + 2) count = 256;
+      if (i >= Q_READY && i < Q_READY + 2) count = 128;
+      if (i >= P_READY && i < P_READY + 2) count = 128;
+      sm100::mbar_init(bars + 8 * i, count);
+    }
+    sm100::fence_mbar_init();
+  }
+  // ---- prefix sums of the requests' steps -------------------------------------------------
+  int shift = 0;
+  while ((a.R >> shift) + 1 > kPrefixEntries) ++shift;
+  const int entries = (a.R + (1 << shift) - 1) >> shift;
+  for (int e0 = 0; e0 < entries; e0 += kThreads) {
+    const int e = e0 + tid;
+    int v = 0;
+    if (e < entries)
+      for (int r = e << shift; r < min(a.R, (e + 1) << shift); ++r) {
+        Item it;
+        it.r = r;
+        it.request<G_>(a);
+        v += a.kv_heads * it.units<G_>(a);
+      }
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int nb = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += nb;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    const int part = lane < kThreads / 32 ? wsum[lane] : 0;
+    const int before = s_total + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
+    const int all = __reduce_add_sync(0xffffffffu, part);
+    if (e < entries) pre[e] = before + inc - v;
+    __syncthreads();
+    if (tid == 0) s_total += all;
+    __syncthreads();
+  }
+  const int U = s_total;
+  const int cta = blockIdx.x, ctas = min((int)gridDim.x, U);
+  if (cta >= ctas) {
+    if (tid == 0) a.desc[cta * kDescInts] = 0;
+    return;
+  }
+  const int uq = U / ctas, ur = U - uq * ctas;
+  auto first_unit = [&](int c) { return uq * c + ur * c / ctas; };
+  const int u0 = first_unit(cta), u1 = first_unit(cta + 1);
+  if (warp == 0) {
+    sm100::tmem_alloc(sm100::smem_u32(&s_tmem), 512);
+    sm100::tmem_relinquish();
+  }
+  if (tid == 32) {
+    int lo = 0, hi = entries;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (pre[mid] <= u0) lo = mid; else hi = mid;
+    }
+    Item it = {};
+    int rem = u0 - pre[lo], per = 0;
+    it.r = lo << shift;
+    for (;;) {
+      it.request<G_>(a);
+      per = it.units<G_>(a);
+      if (rem < per * a.kv_heads || it.r + 1 >= a.R) break;
+      rem -= per * a.kv_heads;
+      ++it.r;
+    }
+    it.h = rem / per;
+    rem -= it.h * per;
+    for (it.rt = 0;; ++it.rt) {
+      it.steps = it.steps_of<G_>(a, it.rt, &it.vis);
+      if (rem < it.steps) break;
+      rem -= it.steps;
+    }
+    it.step = rem;
+    s_first = it;
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  auto bar = [&](int i) { return bars + 8 * i; };
+  // Waits end the CTA's work when they run out or when another role's has.
+  auto wait = [&](int b, uint32_t parity) {
+    if (s_abort) return false;
+    if (sm100::mbar_wait_bounded(bar(b), parity, a.status, kWaitNs)) return true;
+    s_abort = 1;
+    return false;
+  };
+  Item it = s_first;
+
+  if (warp < 8) {
+    // ---- softmax: warpgroup T has row tile T, thread = row ---------------------------------
+    sm100::setmaxnreg_inc<192>();
+    const int T = warp >> 2, rloc = (warp & 3) * 32 + lane;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lanes + T * 128, tO = tmem + lanes + 256 + T * 128;
+    const uint32_t qs_base = sbase + G_::OFF_Q + T * G_::QTILE;
+    int np = 0, ns = 0, nq = 0;                          // steps, this tile's steps, segments
+    bool live = true;
+    for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+      const Segment sg(it, a, u, u0, u1);
+      if (sg.skip) continue;
+      const int row = it.rt * kRows + T * 128 + rloc;
+      const bool in = row < it.n * a.G;
+      const int head = it.h * a.G + row % a.G, tokq = it.q0 + row / a.G;
+      const bool mine = T == 0 || sg.two;
+      float qs[NG], ksc = 0.f, M = -CUDART_INF_F;
+      F2 l2 = pack2(0.f, 0.f), pm2[NG];
+#pragma unroll
+      for (int k = 0; k < NG; ++k) qs[k] = 0.f, pm2[k] = pack2(0.f, 0.f);
+      const int lim = in ? it.L - it.n + row / a.G : -1;
+      if (sg.count > 0 && mine) {
+        // queries into the A operand: the codes' order within an octet, odd channels / 16,
+        // scaled up to just below fp16's limit
+        uint4 v[D / 8];
+        float big = 0.f;
+        const __half* qp = a.q + (in ? (int64_t)tokq * a.q_ts + (int64_t)head * a.q_hs : 0);
+#pragma unroll
+        for (int o = 0; o < D / 8; ++o) {
+          v[o] = make_uint4(0, 0, 0, 0);
+          if (in) v[o] = *reinterpret_cast<const uint4*>(qp + 8 * o);
+        }
+#pragma unroll
+        for (int o = 0; o < D / 8; ++o) {
+          const uint32_t w[4] = {v[o].x, v[o].y, v[o].z, v[o].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(u32_as_h2(w[k]));
+            qs[o * 8 / GROUP] += f.x + f.y;
+            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+        }
+        const int e_big = (int)(__float_as_uint(big) >> 23) - 127;
+        const int up2 = big > 0.f && e_big <= 15 ? 15 - e_big : 0;
+        const float qmul = __uint_as_float((uint32_t)(127 + up2) << 23), qodd = qmul * 0.0625f;
+        // x = ksc (s S + m qs): codes enter the MMA times 2^-24, queries times qmul
+        ksc = a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - up2) << 23);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) qs[k] *= qmul * 5.9604645e-8f;
+#pragma unroll
+        for (int o = 0; o < D / 8; ++o) {
+          const uint32_t ev[2] = {__byte_perm(v[o].x, v[o].z, 0x5410), __byte_perm(v[o].y, v[o].w, 0x5410)};
+          const uint32_t od[2] = {__byte_perm(v[o].x, v[o].z, 0x7632), __byte_perm(v[o].y, v[o].w, 0x7632)};
+          uint32_t c[4];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2 e = __half22float2(u32_as_h2(ev[k])), f = __half22float2(u32_as_h2(od[k]));
+            c[2 * k] = h2_as_u32(__floats2half2_rn(e.x * qmul, e.y * qmul));
+            c[2 * k + 1] = h2_as_u32(__floats2half2_rn(f.x * qodd, f.y * qodd));
+          }
+          sm100::st_shared_v4(qs_base + (o / 8) * (128 * 128) + swz(rloc, o & 7), c[0], c[1], c[2], c[3]);
+        }
+        sm100::fence_proxy_async_smem();
+        sm100::mbar_arrive(bar(Q_READY + T));
+      }
+      const int lim_lo = it.L - it.n + (it.rt * kRows + T * 128) / a.G;   // all rows see these
+      for (int k = 0; k < sg.count; ++k, ++np) {
+        const int ps = np % kParStages;
+        if (!(live = wait(PAR_FULL + ps, (np / kParStages) & 1))) break;
+        if (!mine) {
+          sm100::mbar_arrive(bar(PAR_EMPTY + ps));
+          continue;
+        }
+        if (!(live = wait(S_FULL + T, ns & 1))) break;
+        ++ns;
+        sm100::tc_fence_after();
+        const int tok0 = (sg.k0 + k) * NTOK;
+        const int ok = par_ok[ps];
+        const float* par = reinterpret_cast<const float*>(smem + G_::OFF_PAR + ps * PAR);
+        const float* ls = par + 512;
+        uint32_t x[128];                                 // S_g, then x in [0, NTOK)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          sm100::tmem_ld_32x32b_x32(tS + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
+        sm100::tmem_ld_wait();
+        const bool edge = tok0 + NTOK - 1 > lim_lo || ok != (1 << NBLK) - 1;
+        float top = -CUDART_INF_F;
+        const F2 ksc2 = pack2(ksc, ksc);
+#pragma unroll
+        for (int t = 0; t < NTOK; t += 4) {
+          F2 y[2];
+#pragma unroll
+          for (int g = 0; g < NG; ++g) {
+            const float4 s4 = *reinterpret_cast<const float4*>(par + g * NTOK + t);
+            const float4 m4 = *reinterpret_cast<const float4*>(par + 128 + g * NTOK + t);
+            const F2 q2 = pack2(qs[g], qs[g]);
+            const uint32_t* S = x + g * NTOK + t;
+            const F2 a0 = pack2(__uint_as_float(S[0]), __uint_as_float(S[1]));
+            const F2 a1 = pack2(__uint_as_float(S[2]), __uint_as_float(S[3]));
+            y[0] = fma2(a0, pack2(s4.x, s4.y), g == 0 ? mul2(pack2(m4.x, m4.y), q2) : fma2(pack2(m4.x, m4.y), q2, y[0]));
+            y[1] = fma2(a1, pack2(s4.z, s4.w), g == 0 ? mul2(pack2(m4.z, m4.w), q2) : fma2(pack2(m4.z, m4.w), q2, y[1]));
+          }
+          const float4 l4 = *reinterpret_cast<const float4*>(ls + t);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 xv = unpack2(y[i]);
+            x[t + 2 * i] = __float_as_uint(xv.x), x[t + 2 * i + 1] = __float_as_uint(xv.y);
+            float2 yv = unpack2(fma2(y[i], ksc2, i == 0 ? pack2(l4.x, l4.y) : pack2(l4.z, l4.w)));
+            if (edge) {
+              const int tk = t + 2 * i;
+              const bool there = (ok >> (tk / 16)) & 1;
+              if (tok0 + tk > lim || !there) yv.x = -CUDART_INF_F;
+              if (tok0 + tk + 1 > lim || !there) yv.y = -CUDART_INF_F;
+            }
+            top = fmaxf(top, fmaxf(yv.x, yv.y));
+          }
+        }
+        // the reference moves when it is more than 2^8 behind
+        if (__any_sync(0xffffffffu, top > M + 8.0f)) {
+          const float m = fmaxf(M, top), f = M == m ? 1.0f : ex2(M - m);
+          M = m;
+          const F2 f2 = pack2(f, f);
+          l2 = mul2(l2, f2);
+#pragma unroll
+          for (int g = 0; g < NG; ++g) pm2[g] = mul2(pm2[g], f2);
+          if (k > 0) {                                   // the step before is in O already
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              sm100::tmem_ld_32x32b_x32(tO + 32 * c, o);
+              sm100::tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              sm100::tmem_st_32x32b_x32(tO + 32 * c, o);
+            }
+          }
+        }
+        const float Mu = M == -CUDART_INF_F ? 0.f : M;
+        const F2 negM = pack2(-Mu, -Mu);
+        // P over S: 16 columns per 32 tokens and group
+#pragma unroll
+        for (int c = 0; c < NTOK / 32; ++c) {
+          uint32_t w[NG][16];
+#pragma unroll
+          for (int t = 32 * c; t < 32 * c + 32; t += 4) {
+            F2 p2[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 e = unpack2(fma2(pack2(__uint_as_float(x[t + 2 * i]), __uint_as_float(x[t + 2 * i + 1])),
+                                            ksc2, negM));
+              float2 p = make_float2(ex2(e.x), ex2(e.y));
+              if (edge) {
+                const int tk = t + 2 * i;
+                const bool there = (ok >> (tk / 16)) & 1;
+                if (tok0 + tk > lim || !there) p.x = 0.f;
+                if (tok0 + tk + 1 > lim || !there) p.y = 0.f;
+              }
+              p2[i] = pack2(p.x, p.y);
+              l2 = add2(l2, p2[i]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+              float4 s4 = *reinterpret_cast<const float4*>(par + 256 + g * NTOK + t);
+              float4 m4 = *reinterpret_cast<const float4*>(par + 384 + g * NTOK + t);
+              if (edge) {                                // unseen tokens may hold anything
+                const bool there = (ok >> (t / 16)) & 1;
+                if (tok0 + t > lim || !there) s4.x = m4.x = 0.f;
+                if (tok0 + t + 1 > lim || !there) s4.y = m4.y = 0.f;
+                if (tok0 + t + 2 > lim || !there) s4.z = m4.z = 0.f;
+                if (tok0 + t + 3 > lim || !there) s4.w = m4.w = 0.f;
+              }
+              pm2[g] = fma2(p2[0], pack2(m4.x, m4.y), pm2[g]);
+              pm2[g] = fma2(p2[1], pack2(m4.z, m4.w), pm2[g]);
+              const float2 w0 = unpack2(mul2(p2[0], pack2(s4.x, s4.y)));
+              const float2 w1 = unpack2(mul2(p2[1], pack2(s4.z, s4.w)));
+              w[g][(t - 32 * c) / 2] = h2_as_u32(__floats2half2_rn(w0.x, w0.y));
+              w[g][(t - 32 * c) / 2 + 1] = h2_as_u32(__floats2half2_rn(w1.x, w1.y));
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < NG; ++g) sm100::tmem_st_32x32b_x16(tS + g * (NTOK / 2) + 16 * c, w[g]);
+        }
+        sm100::mbar_arrive(bar(PAR_EMPTY + ps));
+        sm100::tmem_st_wait();
+        sm100::tc_fence_before();
+        sm100::mbar_arrive(bar(P_READY + T));
+      }
+      if (!live) break;
+      if (!mine) continue;
+      // ---- the rows' result ------------------------------------------------------------------
+      if (sg.count > 0) {
+        if (!(live = wait(O_FULL + T, nq & 1))) break;
+        ++nq;
+        sm100::tc_fence_after();
+      }
+      const float2 lv = unpack2(l2);
+      const float l = lv.x + lv.y;
+      float pm[NG];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        const float2 v = unpack2(pm2[g]);
+        pm[g] = v.x + v.y;
+      }
+      const float inv = l == 0.f ? 0.f : 1.0f / l;
+      __half* op = a.out + (in ? (int64_t)tokq * a.o_ts + (int64_t)head * a.o_hs : 0);
+      float* slot = a.part + (size_t)(cta * 2 + (sg.starts ? 1 : 0)) * (kRows * (D + 2));
+      const int srow = T * 128 + rloc;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = 0;
+        if (sg.count > 0) {
+          sm100::tmem_ld_32x32b_x32(tO + 32 * c, o);
+          sm100::tmem_ld_wait();
+        }
+        float f[32];
+        const float m = pm[c * 32 / GROUP];
+#pragma unroll
+        for (int j = 0; j < 32; ++j)                     // odd channels' codes entered times 2^-20
+          f[j] = fmaf(__uint_as_float(o[j]), (j & 1) ? 1048576.f : 16777216.f, m);
+        if (!sg.whole) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(slot + (size_t)srow * D + 32 * c + j) =
+                make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+        } else if (in) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<uint2*>(op + 32 * c + j) =
+                make_uint2(h2_as_u32(__floats2half2_rn(f[j] * inv, f[j + 1] * inv)),
+                           h2_as_u32(__floats2half2_rn(f[j + 2] * inv, f[j + 3] * inv)));
+        }
+      }
+      if (!sg.whole) {
+        slot[kRows * D + srow] = M;
+        slot[kRows * D + kRows + srow] = l;
+      }
+      sm100::tc_fence_before();
+    }
+  } else if (warp < 12) {
+    // ---- codes into operands ------------------------------------------------------------------
+    sm100::setmaxnreg_dec<64>();
+    const int i = tid - 256;
+    int n = 0, kv = 0;                                   // steps, operand slots filled
+    bool live = true;
+    for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+      const Segment sg(it, a, u, u0, u1);
+      for (int k = 0; k < sg.count; ++k, ++n) {
+        const int rs = n % kRawStages, ps = n % kParStages;
+        if (!(live = wait(RAW_FULL + rs, (n / kRawStages) & 1))) break;
+        const uint8_t* raw = smem + G_::OFF_RAW + rs * G_::RAW;
+        // scales and minima as fp32, per group and token
+        if (n >= kParStages && !(live = wait(PAR_EMPTY + ps, (n / kParStages - 1) & 1))) break;
+        {
+          float* par = reinterpret_cast<float*>(smem + G_::OFF_PAR + ps * PAR);
+          const int tok = i / NG, g = i % NG;
+          const uint8_t* blk = raw + (tok / 16) * BLK;
+          const float2 kp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_kp(D))[(tok % 16) * NG + g]);
+          const float2 vp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_vp(D, GROUP))[(tok % 16) * NG + g]);
+          par[g * NTOK + tok] = kp.x, par[128 + g * NTOK + tok] = kp.y;
+          par[256 + g * NTOK + tok] = vp.x, par[384 + g * NTOK + tok] = vp.y;
+          float big = fmaxf(vp.x, 5.9604645e-8f);        // 2^-24, fp16's least scale
+#pragma unroll
+          for (int o = 1; o < NG; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          if (g == 0) par[512 + tok] = lg2(big);
+          if (i == 0) par_ok[ps] = raw_ok[rs];
+        }
+        sm100::mbar_arrive(bar(PAR_FULL + ps));
+        // K: rows of tokens.  A quad of lanes reads a token's row; rows r and r ^ 5 in a
+        // phase of eight lanes meet neither each other's banks nor swizzled chunks.
+        int slot = kv % kKvSlots;
+        if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
+        uint32_t dst = sbase + G_::OFF_KV + slot * G_::SLOT;
+#pragma unroll 1
+        for (int unit = i; unit < NTOK * 4; unit += 128) {
+          const int t = unit & 3, half = (unit >> 2) & 1, pair = (unit >> 3) & 3, oct = unit >> 5;
+          const int tok = oct * 8 + (half ? pair ^ 5 : pair);
+          const uint8_t* src = raw + (tok / 16) * BLK + (tok % 16) * (D / 2) + t * (D / 8);
+          uint32_t w[D / 32];
+          if constexpr (D == 128) {
+            const uint4 y = *reinterpret_cast<const uint4*>(src);
+            w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
+          } else {
+            const uint2 y = *reinterpret_cast<const uint2*>(src);
+            w[0] = y.x, w[1] = y.y;
+          }
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const int o = 4 * j + t;                     // octet of the token's row
+            const uint32_t h = w[j] >> 8;
+            sm100::st_shared_v4(dst + (o / 8) * (NTOK * 128) + swz(tok, o & 7), w[j] & kLoMask,
+                                w[j] & kHiMask, h & kLoMask, h & kHiMask);
+          }
+        }
+        sm100::fence_proxy_async_smem();
+        sm100::mbar_arrive(bar(KV_FULL + slot));
+        ++kv;
+        // V: rows of channels.  A thread turns 8 tokens of D / 32 quads of channels; a phase
+        // of eight lanes has four runs of 8 tokens and two quads.
+        slot = kv % kKvSlots;
+        if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
+        dst = sbase + G_::OFF_KV + slot * G_::SLOT;
+#pragma unroll 1
+        for (int unit = i; unit < NTOK; unit += 128) {   // 8 x (NTOK / 8) units
+          const int run = (unit & 3) + 4 * (unit >> 5), h8 = (unit >> 2) & 7;
+          const uint8_t* src = raw + (run / 2) * BLK + kv4::off_v(D) + (run & 1) * 4 * D + h8 * (D / 8);
+          uint32_t w[4][D / 32];
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            if constexpr (D == 128) {
+              const uint4 y = *reinterpret_cast<const uint4*>(src + p * D);
+              w[p][0] = y.x, w[p][1] = y.y, w[p][2] = y.z, w[p][3] = y.w;
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2*>(src + p * D);
+              w[p][0] = y.x, w[p][1] = y.y;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < D / 32; ++j) {
+            const int ch = 4 * (8 * j + h8);             // first of the quad's channels
+            const uint32_t at = dst + (run / 8) * (D * 128);
+            uint32_t e[4], o[4];
+#pragma unroll
+            for (int p = 0; p < 4; ++p) e[p] = w[p][j] & kLoMask, o[p] = w[p][j] & kHiMask;
+            sm100::st_shared_v4(at + swz(ch, run & 7), e[0], e[1], e[2], e[3]);
+            sm100::st_shared_v4(at + swz(ch + 1, run & 7), o[0], o[1], o[2], o[3]);
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint32_t hw = w[p][j] >> 8;
+              e[p] = hw & kLoMask, o[p] = hw & kHiMask;
+            }
+            sm100::st_shared_v4(at + swz(ch + 2, run & 7), e[0], e[1], e[2], e[3]);
+            sm100::st_shared_v4(at + swz(ch + 3, run & 7), o[0], o[1], o[2], o[3]);
+          }
+        }
+        sm100::mbar_arrive(bar(RAW_EMPTY + rs));
+        sm100::fence_proxy_async_smem();
+        sm100::mbar_arrive(bar(KV_FULL + slot));
+        ++kv;
+      }
+    }
+  } else {
+    sm100::setmaxnreg_dec<64>();
+    if (warp == 12 && lane == 0) {
+      // ---- MMA issue ---------------------------------------------------------------------------
+      constexpr uint32_t idS = sm100::idesc_f16_f32(128, NTOK, 0, 0);
+      constexpr uint32_t idO = sm100::idesc_f16_f32(128, GROUP, 0, 0);
+      int kv = 0, np[2] = {0, 0}, nq[2] = {0, 0};
+      bool live = true;
+      auto issue_s = [&](int T, int slot) {
+        const uint32_t q = sbase + G_::OFF_Q + T * G_::QTILE, kk0 = sbase + G_::OFF_KV + slot * G_::SLOT;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t ad = sm100::umma_desc_sw128(q + (kk / 4) * (128 * 128) + (kk & 3) * 32, 16, 1024);
+          const uint64_t bd = sm100::umma_desc_sw128(kk0 + (kk / 4) * (NTOK * 128) + (kk & 3) * 32, 16, 1024);
+          sm100::umma_f16(tmem + T * 128 + (kk * 16 / GROUP) * NTOK, ad, bd, idS, kk * 16 % GROUP != 0);
+        }
+        sm100::umma_commit(bar(S_FULL + T));
+      };
+      auto issue_o = [&](int T, int slot, bool first) {
+        const uint32_t v = sbase + G_::OFF_KV + slot * G_::SLOT;
+#pragma unroll
+        for (int g = 0; g < NG; ++g)
+#pragma unroll
+          for (int kk = 0; kk < NTOK / 16; ++kk) {
+            const uint64_t bd = sm100::umma_desc_sw128(v + (kk / 4) * (D * 128) + g * GROUP * 128 + (kk & 3) * 32, 16, 1024);
+            sm100::umma_f16_ts(tmem + 256 + T * 128 + g * GROUP, tmem + T * 128 + g * (NTOK / 2) + kk * 8, bd,
+                               idO, !first || kk != 0);
+          }
+      };
+      for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+        const Segment sg(it, a, u, u0, u1);
+        if (sg.count == 0) continue;
+        const int tiles = sg.two ? 2 : 1;
+        // S of the first step
+        if (!(live = wait(KV_FULL + kv % kKvSlots, (kv / kKvSlots) & 1))) break;
+        for (int T = 0; T < tiles && live; ++T) {
+          if (!(live = wait(Q_READY + T, nq[T] & 1))) break;
+          ++nq[T];
+          sm100::tc_fence_after();
+          issue_s(T, kv % kKvSlots);
+        }
+        if (!live) break;
+        sm100::umma_commit(bar(KV_EMPTY + kv % kKvSlots));
+        ++kv;
+        for (int k = 0; k < sg.count && live; ++k) {
+          const int vs = kv % kKvSlots, vp = (kv / kKvSlots) & 1;
+          ++kv;
+          const int ks = kv % kKvSlots, kp = (kv / kKvSlots) & 1;
+          const bool more = k + 1 < sg.count;
+          if (!(live = wait(KV_FULL + vs, vp))) break;
+          for (int T = 0; T < tiles; ++T) {
+            if (!(live = wait(P_READY + T, np[T] & 1))) break;
+            ++np[T];
+            sm100::tc_fence_after();
+            issue_o(T, vs, k == 0);
+            if (T == tiles - 1) sm100::umma_commit(bar(KV_EMPTY + vs));
+            if (more) {
+              if (T == 0 && !(live = wait(KV_FULL + ks, kp))) break;
+              sm100::tc_fence_after();
+              issue_s(T, ks);
+              if (T == tiles - 1) sm100::umma_commit(bar(KV_EMPTY + ks));
+            } else {
+              sm100::umma_commit(bar(O_FULL + T));
+            }
+          }
+          if (more) ++kv;
+        }
+      }
+      if (s_abort) {                                     // MMAs in flight finish before TMEM goes back
+        sm100::umma_commit(bar(DRAIN));
+        sm100::mbar_wait_bounded(bar(DRAIN), 0, nullptr, 100000000ull);
+      }
+    } else if (warp == 13) {
+      // ---- cache blocks of a step: lane b copies block b ---------------------------------------
+      const int bpp_shift = a.page_shift - 4;
+      int n = 0;
+      bool live = true;
+      for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+        const Segment sg(it, a, u, u0, u1);
+        auto page = [&](int k) {
+          const int blk = (sg.k0 + k) * NBLK + lane;
+          return lane < NBLK && k < sg.count && blk * 16 < it.vis
+                     ? a.table[it.r * a.table_rs + (blk >> bpp_shift)] : -2;
+        };
+        int pid = page(0);
+        for (int k = 0; k < sg.count; ++k, ++n) {
+          const int rs = n % kRawStages;
+          if (n >= kRawStages) live = wait(RAW_EMPTY + rs, (n / kRawStages - 1) & 1);
+          live = __all_sync(0xffffffffu, live);
+          if (!live) break;
+          const bool have = pid >= 0 && pid < a.num_pages;
+          if (pid != -2 && !have) atomicOr(a.status, kDevErrShape);
+          const uint32_t ok = __ballot_sync(0xffffffffu, have);
+          if (lane == 0) {
+            raw_ok[rs] = (int)ok;
+            sm100::mbar_arrive_expect_tx(bar(RAW_FULL + rs), __popc(ok) * BLK);
+          }
+          __syncwarp();
+          if (have) {
+            const int blk = (sg.k0 + k) * NBLK + lane;
+            bulk_load(sbase + G_::OFF_RAW + rs * G_::RAW + lane * BLK,
+                      a.cache + ((((int64_t)pid * a.kv_heads + it.h) << bpp_shift) +
+                                 (blk & ((1 << bpp_shift) - 1))) * BLK,
+                      BLK, bar(RAW_FULL + rs));
+          }
+          pid = page(k + 1);
+        }
+      }
+      __syncwarp();
+      if (lane == 0 && s_abort)                          // copies in flight land before the exit
+        for (int k = max(0, n - kRawStages); k < n; ++k)
+          sm100::mbar_wait_bounded(bar(RAW_FULL + k % kRawStages), (k / kRawStages) & 1, nullptr, 100000000ull);
+    }
+    __syncwarp();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  sm100::grid_launch_dependents();
+  if (tid == 0) {
+    // the item that starts here and goes on in the next CTAs, if there is one
+    int* d = a.desc + cta * kDescInts;
+    int span = 0;
+    Item x = s_first;
+    for (int u = u0; u < u1; u += x.steps - x.step, x.next<G_>(a)) {
+      const Segment sg(x, a, u, u0, u1);
+      if (!sg.whole && sg.starts) {
+        const int end = u - x.step + max(1, x.steps - 1);     // past the last step with tokens
+        span = (int)(((double)end * ctas - 1.0) / U) - cta + 1;
+        d[1] = x.q0, d[2] = x.rt * kRows, d[3] = x.n * a.G, d[4] = x.h;
+      }
+    }
+    d[0] = span;
+  }
+  if (warp == 0) sm100::tmem_dealloc(tmem, 512);
+}
+
+// Joins an item that crosses CTAs: block (c, y) takes rows [8 y, 8 y + 8) of the item that
+// starts in CTA c, over the slots of CTAs c .. c + span - 1 in order, 32 lanes a row.
+template <int D>
+__global__ void __launch_bounds__(256) kv4_prefill_merge(const AttnArgs a) {
+  sm100::grid_dependency_wait();
+  const int cta = blockIdx.x, tid = threadIdx.x;
+  const int* d = a.desc + cta * kDescInts;
+  const int span = d[0];
+  if (span == 0) return;
+  const int r = blockIdx.y * 8 + tid / 32, ch = (tid & 31) * (D / 32), row = d[2] + r;
+  if (row >= d[3]) return;
+  constexpr size_t kSlot = (size_t)kRows * (D + 2);
+  auto part = [&](int k) { return a.part + (size_t)((cta + k) * 2 + (k == 0)) * kSlot; };
+  float m = -CUDART_INF_F;
+  for (int k = 0; k < span; ++k) m = fmaxf(m, part(k)[kRows * D + r]);
+  float o[D / 32] = {}, l = 0.f;
+  for (int k = 0; k < span; ++k) {
+    const float* p = part(k);
+    const float mk = p[kRows * D + r], f = mk == m ? 1.0f : ex2(mk - m);
+    l = fmaf(f, p[kRows * D + kRows + r], l);
+#pragma unroll
+    for (int j = 0; j < D / 32; j += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(p + (size_t)r * D + ch + j);
+      o[j] = fmaf(f, v.x, o[j]), o[j + 1] = fmaf(f, v.y, o[j + 1]);
+    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  __half* op = a.out + (int64_t)(d[1] + row / a.G) * a.o_ts + (int64_t)(d[4] * a.G + row % a.G) * a.o_hs + ch;
+#pragma unroll
+  for (int j = 0; j < D / 32; j += 2)
+    *reinterpret_cast<__half2*>(op + j) = __floats2half2_rn(o[j] * inv, o[j + 1] * inv);
+}
+
+template <int D, int GROUP>
+cudaError_t launch_geo(const AttnArgs& a, int num_sms, cudaStream_t stream) {
+  using G_ = Geo<D, GROUP>;
+  static PerDeviceOnce attr_once;
+  const cudaError_t attr = attr_once.run([] {
+    return cudaFuncSetAttribute(kv4_prefill_kernel<G_>, cudaFuncAttributeMaxDynamicSharedMemorySize, G_::SMEM);
+  });
+  if (attr != cudaSuccess) return attr;
+  kv4_prefill_kernel<G_><<<num_sms, kThreads, G_::SMEM, stream>>>(a);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms, kRows / 8, 1);
+  cfg.blockDim = dim3(256, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv4_prefill_merge<D>, a);
+}
+
+}  // namespace
+
+cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, int head_dim, int group, int num_sms,
+                               cudaStream_t stream) {
+  if (head_dim == 64 && group == 32) return launch_geo<64, 32>(a, num_sms, stream);
+  if (head_dim == 64 && group == 64) return launch_geo<64, 64>(a, num_sms, stream);
+  if (head_dim == 128 && group == 32) return launch_geo<128, 32>(a, num_sms, stream);
+  if (head_dim == 128 && group == 64) return launch_geo<128, 64>(a, num_sms, stream);
+  if (head_dim == 128 && group == 128) return launch_geo<128, 128>(a, num_sms, stream);
+  return cudaErrorInvalidValue;
+}
+
+}  // namespace awq

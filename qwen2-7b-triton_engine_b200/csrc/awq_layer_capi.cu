@@ -129,10 +129,10 @@ int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64_t max_b
   return AWQ_OK;
 }
 
-size_t awq_kv4_attention_workspace_bytes(int64_t head_dim) {
+size_t awq_kv4_attention_workspace_bytes(int64_t head_dim, int64_t max_rows) {
   int sms = 0, *status = nullptr;
   if ((head_dim != 64 && head_dim != 128) || awq::device_context(&sms, &status)) return 0;
-  return awq::kv4_attention_workspace((int)head_dim, sms);
+  return awq::kv4_attention_workspace((int)head_dim, max_rows, sms);
 }
 
 int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int64_t tokens,
@@ -172,7 +172,8 @@ int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
     return fail(AWQ_ERR_UNSUPPORTED, "tokens x max_blocks x page_size is too large for one call");
   int sms = 0, *status = nullptr;
   if ((rc = awq::device_context(&sms, &status))) return rc;
-  const size_t need = awq::kv4_attention_workspace((int)head_dim, sms);
+  a.max_q = (int)(max_q < tokens ? max_q : tokens);
+  const size_t need = awq::kv4_attention_workspace((int)head_dim, (int64_t)a.max_q * (q_heads / kv_heads), sms);
   if (!workspace || workspace_bytes < need)
     return fail(AWQ_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
   if (!aligned(workspace, 16)) return fail(AWQ_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
@@ -180,7 +181,6 @@ int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   a.out = out, a.o_ts = out_token_stride, a.o_hs = out_head_stride;
   a.table = block_table, a.table_rs = table_stride, a.lens = kv_lens, a.cu_q = cu_q;
   a.tokens = tokens, a.rows = (int)requests, a.width = (int)max_blocks, a.q_heads = (int)q_heads;
-  a.max_q = (int)(max_q < tokens ? max_q : tokens);
   a.scale = scale, a.workspace = workspace;
   const cudaError_t e = awq::launch_kv4_attention(a, sms, status, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return fail_cuda(e, "kv4 attention launch");

@@ -404,3 +404,64 @@ def test_attention_graph_and_streams(cuda):
                     g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, ref) for _, _, out in graphs)
+
+
+@pytest.mark.parametrize("D,group,H,Hk", [(128, 128, 7, 1), (128, 64, 8, 2), (128, 32, 4, 4),
+                                          (64, 64, 14, 2), (64, 32, 2, 1)])
+@pytest.mark.parametrize("lens,qs,page", [([300], [300], 64), ([700, 90], [37, 90], 16),
+                                          ([1030], [65], 32), ([64, 1500, 10], [64, 3, 10], 128),
+                                          ([50, 129], [70, 129], 16)])
+def test_attention_prompt_chunks(cuda, D, group, H, Hk, lens, qs, page):
+    """Many query rows (tcgen05 kernel) beside few, steps that end inside blocks, more query
+    tokens than cached ones."""
+    check_attention(np.random.default_rng(sum(lens)), lens, qs, H, Hk, D, group, page, pad=2)
+
+
+def test_attention_prompt_scale_and_small_values(cuda):
+    rng = np.random.default_rng(21)
+    for kw in (dict(small=True), dict(scale=2.0), dict(scale=-0.3), dict(scale=0.0)):
+        check_attention(rng, [200], [100], 4, 2, 128, 64, 32, **kw)
+
+
+def test_attention_prompt_bad_pages_and_nan(cuda):
+    rng = np.random.default_rng(22)
+    cache, table, KV, _, kv = make_cache(rng, [200], 1, 128, 64, 16)
+    q = rng.standard_normal((90, 2, 128)).astype(np.float16)
+    lens, cu = dev(np.array([200])).int(), dev(np.array([0, 90])).int()
+    page1 = int(table[0, 1])
+    table[0, 1] = -1
+    got = awq_b200.kv4_attention(dev(q), cache, table, lens, cu, 90).double().cpu().numpy()
+    assert awq_b200.device_status() == 2
+    keep = [*range(16), *range(32, 200)]
+    K, V = (x[keep] for x in KV[0])
+    ref = L.attention(q, K, V, 128 ** -0.5)
+    assert np.abs(got - ref).max() <= 2e-3 * np.abs(V).max()
+    table[0, 1] = page1                                 # rows 40.. see token 150, others do not
+    k = torch.full((1, 1, 128), float("nan"), dtype=torch.float16, device="cuda")
+    awq_b200.kv4_append(k, k, dev(kv[0][2][150:151]), cache)
+    got = awq_b200.kv4_attention(dev(q), cache, table, lens, cu, 90)
+    bad = torch.isnan(got).flatten(1)
+    assert bad[40:].all() and not bad[:40].any()
+
+
+def test_attention_prompt_graph_with_other_lengths(cuda):
+    rng = np.random.default_rng(23)
+    lens = [300, 260]
+    cache, table, KV, _, _ = make_cache(rng, lens, 2, 128, 128, 32)
+    q = dev(rng.standard_normal((220, 4, 128)).astype(np.float16))
+    live, cu = dev(np.array(lens)).int(), dev(np.array([0, 100, 220])).int()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = awq_b200.kv4_attention(q, cache, table, live, cu, 220)
+    for new_lens, new_cu in (([300, 260], [0, 100, 220]), ([31, 260], [0, 1, 180]), ([0, 0], [0, 0, 220])):
+        live.copy_(dev(np.array(new_lens)))
+        cu.copy_(dev(np.array(new_cu)))
+        want = awq_b200.kv4_attention(q, cache, table, live, cu, 220)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:new_cu[-1]], want[:new_cu[-1]])
+    assert awq_b200.device_status() == 0
