@@ -25,6 +25,8 @@
 #include <cuda_runtime.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "awq_common.cuh"
 #include "awq_internal.h"
 #include "awq_kv4.cuh"
@@ -53,7 +55,8 @@ struct Geo {
   static constexpr int VA = (NTOK + 63) / 64;          // 64-token atoms of V rows
   static constexpr int QTILE = KA * 128 * 128, KSLOT = KA * NTOK * 128, VSLOT = VA * D * 128;
   static constexpr int SLOT = KSLOT > VSLOT ? KSLOT : VSLOT;
-  static constexpr int PAR = 4 * 128 * 4 + NTOK * 4;   // ks, km, vs, vm [NG][NTOK], ls [NTOK]
+  // ks, km, vs, vm [NG][NTOK], log2 of a token's largest vs [NTOK], largest and least [4]
+  static constexpr int PAR = 4 * 128 * 4 + NTOK * 4 + 32;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_KV = OFF_Q + 2 * QTILE;
   static constexpr int OFF_RAW = OFF_KV + kKvSlots * SLOT;
@@ -177,6 +180,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
       ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 4) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+}
 // Byte offset of 16-byte chunk c (0..7) of a 128-byte row under the 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int row, int c) { return row * 128 + ((c ^ (row & 7)) << 4); }
 
@@ -296,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
 
   if (warp < 8) {
     // ---- softmax: warpgroup T has row tile T, thread = row ---------------------------------
-    sm100::setmaxnreg_inc<192>();
+    sm100::setmaxnreg_inc<168>();
     const int T = warp >> 2, rloc = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tmem + lanes + T * 128, tO = tmem + lanes + 256 + T * 128;
@@ -338,9 +351,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         }
         const int e_big = (int)(__float_as_uint(big) >> 23) - 127;
         const int up2 = big > 0.f && e_big <= 15 ? 15 - e_big : 0;
-        const float qmul = __uint_as_float((uint32_t)(127 + up2) << 23), qodd = qmul * 0.0625f;
+        // (a negative scale turns the queries: the largest x is then the largest score)
+        const float qmul = copysignf(__uint_as_float((uint32_t)(127 + up2) << 23), a.scale_log2);
+        const float qodd = qmul * 0.0625f;
         // x = ksc (s S + m qs): codes enter the MMA times 2^-24, queries times qmul
-        ksc = a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - up2) << 23);
+        ksc = fmaxf(fabsf(a.scale_log2), 1e-30f) * 16777216.0f * __uint_as_float((uint32_t)(127 - up2) << 23);
 #pragma unroll
         for (int k = 0; k < NG; ++k) qs[k] *= qmul * 5.9604645e-8f;
 #pragma unroll
@@ -374,43 +389,66 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         const int ok = par_ok[ps];
         const float* par = reinterpret_cast<const float*>(smem + G_::OFF_PAR + ps * PAR);
         const float* ls = par + 512;
-        uint32_t x[128];                                 // S_g, then x in [0, NTOK)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          sm100::tmem_ld_32x32b_x32(tS + 32 * c, reinterpret_cast<uint32_t(&)[32]>(x[32 * c]));
-        sm100::tmem_ld_wait();
-        const bool edge = tok0 + NTOK - 1 > lim_lo || ok != (1 << NBLK) - 1;
+        // One step.  SLOW: some of its tokens may be unseen (past a row's limit, or in a page
+        // the table does not name), or their value scales differ by more than 2^8, so that
+        // the reference has to look at every token's scale instead of the step's largest.
+        const float4 hi4 = *reinterpret_cast<const float4*>(ls + NTOK);
+        const float4 lo4 = *reinterpret_cast<const float4*>(ls + NTOK + 4);
+        const float v_hi = fmaxf(fmaxf(hi4.x, hi4.y), fmaxf(hi4.z, hi4.w));
+        const float v_lo = fminf(fminf(lo4.x, lo4.y), fminf(lo4.z, lo4.w));
+        auto softmax_step = [&](auto slow) {
+        constexpr bool SLOW = decltype(slow)::value;
+        constexpr int CT = 32 / NG, NC = NTOK / CT;      // tokens of a chunk: 32 registers of S
+        auto unseen = [&](int t) { return tok0 + t > lim || !((ok >> (t / 16)) & 1); };
         float top = -CUDART_INF_F;
-        const F2 ksc2 = pack2(ksc, ksc);
+        {
+          // first pass: x / ksc of every token, back into the columns of S_0, and the largest
+          uint32_t buf[2][NG][CT];
+          auto load = [&](int b, int c) {
 #pragma unroll
-        for (int t = 0; t < NTOK; t += 4) {
-          F2 y[2];
+            for (int g = 0; g < NG; ++g) sm100::tmem_ld_32x32b<CT>(tS + g * NTOK + c * CT, buf[b][g]);
+          };
+          load(0, 0);
 #pragma unroll
-          for (int g = 0; g < NG; ++g) {
-            const float4 s4 = *reinterpret_cast<const float4*>(par + g * NTOK + t);
-            const float4 m4 = *reinterpret_cast<const float4*>(par + 128 + g * NTOK + t);
-            const F2 q2 = pack2(qs[g], qs[g]);
-            const uint32_t* S = x + g * NTOK + t;
-            const F2 a0 = pack2(__uint_as_float(S[0]), __uint_as_float(S[1]));
-            const F2 a1 = pack2(__uint_as_float(S[2]), __uint_as_float(S[3]));
-            y[0] = fma2(a0, pack2(s4.x, s4.y), g == 0 ? mul2(pack2(m4.x, m4.y), q2) : fma2(pack2(m4.x, m4.y), q2, y[0]));
-            y[1] = fma2(a1, pack2(s4.z, s4.w), g == 0 ? mul2(pack2(m4.z, m4.w), q2) : fma2(pack2(m4.z, m4.w), q2, y[1]));
-          }
-          const float4 l4 = *reinterpret_cast<const float4*>(ls + t);
+          for (int c = 0; c < NC; ++c) {
+            sm100::tmem_ld_wait();
+            if (c + 1 < NC) load((c + 1) & 1, c + 1);
+            uint32_t x[CT];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 xv = unpack2(y[i]);
-            x[t + 2 * i] = __float_as_uint(xv.x), x[t + 2 * i + 1] = __float_as_uint(xv.y);
-            float2 yv = unpack2(fma2(y[i], ksc2, i == 0 ? pack2(l4.x, l4.y) : pack2(l4.z, l4.w)));
-            if (edge) {
-              const int tk = t + 2 * i;
-              const bool there = (ok >> (tk / 16)) & 1;
-              if (tok0 + tk > lim || !there) yv.x = -CUDART_INF_F;
-              if (tok0 + tk + 1 > lim || !there) yv.y = -CUDART_INF_F;
+            for (int t0 = 0; t0 < CT; t0 += 4) {
+              const int t = c * CT + t0;
+              F2 y[2];
+#pragma unroll
+              for (int g = 0; g < NG; ++g) {
+                const float4 s4 = *reinterpret_cast<const float4*>(par + g * NTOK + t);
+                const float4 m4 = *reinterpret_cast<const float4*>(par + 128 + g * NTOK + t);
+                const F2 q2 = pack2(qs[g], qs[g]);
+                const uint32_t* S = buf[c & 1][g] + t0;
+                const F2 a0 = pack2(__uint_as_float(S[0]), __uint_as_float(S[1]));
+                const F2 a1 = pack2(__uint_as_float(S[2]), __uint_as_float(S[3]));
+                const F2 b0 = pack2(m4.x, m4.y), b1 = pack2(m4.z, m4.w);
+                y[0] = fma2(a0, pack2(s4.x, s4.y), g == 0 ? mul2(b0, q2) : fma2(b0, q2, y[0]));
+                y[1] = fma2(a1, pack2(s4.z, s4.w), g == 0 ? mul2(b1, q2) : fma2(b1, q2, y[1]));
+              }
+              float2 y0 = unpack2(y[0]), y1 = unpack2(y[1]);
+              if constexpr (SLOW) {
+                if (unseen(t)) y0.x = -CUDART_INF_F;
+                if (unseen(t + 1)) y0.y = -CUDART_INF_F;
+                if (unseen(t + 2)) y1.x = -CUDART_INF_F;
+                if (unseen(t + 3)) y1.y = -CUDART_INF_F;
+                const float4 l4 = *reinterpret_cast<const float4*>(ls + t);
+                top = fmaxf(top, fmaxf(fmaxf(fmaf(y0.x, ksc, l4.x), fmaf(y0.y, ksc, l4.y)),
+                                       fmaxf(fmaf(y1.x, ksc, l4.z), fmaf(y1.y, ksc, l4.w))));
+              } else {
+                top = fmaxf(top, fmaxf(fmaxf(y0.x, y0.y), fmaxf(y1.x, y1.y)));
+              }
+              x[t0] = __float_as_uint(y0.x), x[t0 + 1] = __float_as_uint(y0.y);
+              x[t0 + 2] = __float_as_uint(y1.x), x[t0 + 3] = __float_as_uint(y1.y);
             }
-            top = fmaxf(top, fmaxf(yv.x, yv.y));
+            sm100::tmem_st_32x32b<CT>(tS + c * CT, x);
           }
         }
+        if constexpr (!SLOW) top = fmaf(top, ksc, lg2(v_hi));
         // the reference moves when it is more than 2^8 behind
         if (__any_sync(0xffffffffu, top > M + 8.0f)) {
           const float m = fmaxf(M, top), f = M == m ? 1.0f : ex2(M - m);
@@ -420,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
 #pragma unroll
           for (int g = 0; g < NG; ++g) pm2[g] = mul2(pm2[g], f2);
           if (k > 0) {                                   // the step before is in O already
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
               uint32_t o[32];
               sm100::tmem_ld_32x32b_x32(tO + 32 * c, o);
@@ -432,50 +470,52 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
           }
         }
         const float Mu = M == -CUDART_INF_F ? 0.f : M;
-        const F2 negM = pack2(-Mu, -Mu);
-        // P over S: 16 columns per 32 tokens and group
+        const F2 negM = pack2(-Mu, -Mu), ksc2 = pack2(ksc, ksc);
+        sm100::tmem_st_wait();
+        // second pass: weights, sums, and P_g over columns that have been read: 16 per chunk
+        // of 32 tokens in the columns of S_g
+        constexpr int PT = NTOK < 32 ? NTOK : 32;
+        uint32_t xb[2][PT];
+        sm100::tmem_ld_32x32b<PT>(tS, xb[0]);
 #pragma unroll
-        for (int c = 0; c < NTOK / 32; ++c) {
-          uint32_t w[NG][16];
+        for (int c = 0; c < NTOK / PT; ++c) {
+          sm100::tmem_ld_wait();
+          if (c + 1 < NTOK / PT) sm100::tmem_ld_32x32b<PT>(tS + (c + 1) * PT, xb[(c + 1) & 1]);
+          uint32_t w[NG][PT / 2];
 #pragma unroll
-          for (int t = 32 * c; t < 32 * c + 32; t += 4) {
-            F2 p2[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const float2 e = unpack2(fma2(pack2(__uint_as_float(x[t + 2 * i]), __uint_as_float(x[t + 2 * i + 1])),
-                                            ksc2, negM));
-              float2 p = make_float2(ex2(e.x), ex2(e.y));
-              if (edge) {
-                const int tk = t + 2 * i;
-                const bool there = (ok >> (tk / 16)) & 1;
-                if (tok0 + tk > lim || !there) p.x = 0.f;
-                if (tok0 + tk + 1 > lim || !there) p.y = 0.f;
-              }
-              p2[i] = pack2(p.x, p.y);
-              l2 = add2(l2, p2[i]);
-            }
+          for (int t0 = 0; t0 < PT; t0 += 4) {
+            const int t = c * PT + t0;
+            const uint32_t* x = xb[c & 1] + t0;
+            const float2 e0 = unpack2(fma2(pack2(__uint_as_float(x[0]), __uint_as_float(x[1])), ksc2, negM));
+            const float2 e1 = unpack2(fma2(pack2(__uint_as_float(x[2]), __uint_as_float(x[3])), ksc2, negM));
+            const F2 p0 = pack2(ex2(e0.x), ex2(e0.y)), p1 = pack2(ex2(e1.x), ex2(e1.y));
+            l2 = add2(l2, add2(p0, p1));
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
               float4 s4 = *reinterpret_cast<const float4*>(par + 256 + g * NTOK + t);
               float4 m4 = *reinterpret_cast<const float4*>(par + 384 + g * NTOK + t);
-              if (edge) {                                // unseen tokens may hold anything
-                const bool there = (ok >> (t / 16)) & 1;
-                if (tok0 + t > lim || !there) s4.x = m4.x = 0.f;
-                if (tok0 + t + 1 > lim || !there) s4.y = m4.y = 0.f;
-                if (tok0 + t + 2 > lim || !there) s4.z = m4.z = 0.f;
-                if (tok0 + t + 3 > lim || !there) s4.w = m4.w = 0.f;
+              if constexpr (SLOW) {                      // unseen tokens may hold anything
+                if (unseen(t)) s4.x = m4.x = 0.f;
+                if (unseen(t + 1)) s4.y = m4.y = 0.f;
+                if (unseen(t + 2)) s4.z = m4.z = 0.f;
+                if (unseen(t + 3)) s4.w = m4.w = 0.f;
               }
-              pm2[g] = fma2(p2[0], pack2(m4.x, m4.y), pm2[g]);
-              pm2[g] = fma2(p2[1], pack2(m4.z, m4.w), pm2[g]);
-              const float2 w0 = unpack2(mul2(p2[0], pack2(s4.x, s4.y)));
-              const float2 w1 = unpack2(mul2(p2[1], pack2(s4.z, s4.w)));
-              w[g][(t - 32 * c) / 2] = h2_as_u32(__floats2half2_rn(w0.x, w0.y));
-              w[g][(t - 32 * c) / 2 + 1] = h2_as_u32(__floats2half2_rn(w1.x, w1.y));
+              pm2[g] = fma2(p0, pack2(m4.x, m4.y), pm2[g]);
+              pm2[g] = fma2(p1, pack2(m4.z, m4.w), pm2[g]);
+              const float2 w0 = unpack2(mul2(p0, pack2(s4.x, s4.y)));
+              const float2 w1 = unpack2(mul2(p1, pack2(s4.z, s4.w)));
+              w[g][t0 / 2] = h2_as_u32(__floats2half2_rn(w0.x, w0.y));
+              w[g][t0 / 2 + 1] = h2_as_u32(__floats2half2_rn(w1.x, w1.y));
             }
           }
 #pragma unroll
-          for (int g = 0; g < NG; ++g) sm100::tmem_st_32x32b_x16(tS + g * (NTOK / 2) + 16 * c, w[g]);
+          for (int g = 0; g < NG; ++g) sm100::tmem_st_32x32b<PT / 2>(tS + g * NTOK + c * (PT / 2), w[g]);
         }
+        };
+        if (tok0 + NTOK - 1 > lim_lo || ok != (1 << NBLK) - 1 || !(v_hi <= 256.f * v_lo))
+          softmax_step(std::true_type{});
+        else
+          softmax_step(std::false_type{});
         sm100::mbar_arrive(bar(PAR_EMPTY + ps));
         sm100::tmem_st_wait();
         sm100::tc_fence_before();
@@ -536,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     }
   } else if (warp < 12) {
     // ---- codes into operands ------------------------------------------------------------------
-    sm100::setmaxnreg_dec<64>();
+    sm100::setmaxnreg_dec<88>();
     const int i = tid - 256;
     int n = 0, kv = 0;                                   // steps, operand slots filled
     bool live = true;
@@ -546,88 +586,79 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         const int rs = n % kRawStages, ps = n % kParStages;
         if (!(live = wait(RAW_FULL + rs, (n / kRawStages) & 1))) break;
         const uint8_t* raw = smem + G_::OFF_RAW + rs * G_::RAW;
+        // every load of the step's raw blocks first: K rows by quads of lanes (a phase of eight
+        // lanes has rows r and r ^ 5, which meet neither in banks nor in swizzled chunks), V
+        // in units of 8 tokens x D / 32 quads of channels (four runs of 8 tokens and two
+        // quads in a phase)
+        constexpr int KU = NTOK * 4 / 128;
+        uint32_t kw[KU][D / 32], vw[4][D / 32];
+        const int t = i & 3, pair = (i >> 3) & 3;
+        const int tok_in = (i & 4) ? pair ^ 5 : pair;    // of the 8 tokens of an oct
+#pragma unroll
+        for (int x = 0; x < KU; ++x) {
+          const int tok = ((i >> 5) + 4 * x) * 8 + tok_in;
+          load_words<D / 32>(raw + (tok / 16) * BLK + (tok % 16) * (D / 2) + t * (D / 8), kw[x]);
+        }
+        const int run = (i & 3) + 4 * (i >> 5), h8 = (i >> 2) & 7;
+        if (i < NTOK) {
+          const uint8_t* src = raw + (run / 2) * BLK + kv4::off_v(D) + (run & 1) * 4 * D + h8 * (D / 8);
+#pragma unroll
+          for (int p = 0; p < 4; ++p) load_words<D / 32>(src + p * D, vw[p]);
+        }
         // scales and minima as fp32, per group and token
+        const int ptok = i / NG, pg = i % NG;
+        const uint8_t* pblk = raw + (ptok / 16) * BLK;
+        const float2 kp = __half22float2(reinterpret_cast<const __half2*>(pblk + kv4::off_kp(D))[(ptok % 16) * NG + pg]);
+        const float2 vp = __half22float2(reinterpret_cast<const __half2*>(pblk + kv4::off_vp(D, GROUP))[(ptok % 16) * NG + pg]);
+        const int ok = raw_ok[rs];
         if (n >= kParStages && !(live = wait(PAR_EMPTY + ps, (n / kParStages - 1) & 1))) break;
         {
           float* par = reinterpret_cast<float*>(smem + G_::OFF_PAR + ps * PAR);
-          const int tok = i / NG, g = i % NG;
-          const uint8_t* blk = raw + (tok / 16) * BLK;
-          const float2 kp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_kp(D))[(tok % 16) * NG + g]);
-          const float2 vp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_vp(D, GROUP))[(tok % 16) * NG + g]);
-          par[g * NTOK + tok] = kp.x, par[128 + g * NTOK + tok] = kp.y;
-          par[256 + g * NTOK + tok] = vp.x, par[384 + g * NTOK + tok] = vp.y;
+          par[pg * NTOK + ptok] = kp.x, par[128 + pg * NTOK + ptok] = kp.y;
+          par[256 + pg * NTOK + ptok] = vp.x, par[384 + pg * NTOK + ptok] = vp.y;
           float big = fmaxf(vp.x, 5.9604645e-8f);        // 2^-24, fp16's least scale
 #pragma unroll
           for (int o = 1; o < NG; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
-          if (g == 0) par[512 + tok] = lg2(big);
-          if (i == 0) par_ok[ps] = raw_ok[rs];
+          if (pg == 0) par[512 + ptok] = lg2(big);
+          // positive floats order as their bits
+          const uint32_t hi = __reduce_max_sync(0xffffffffu, __float_as_uint(big));
+          const uint32_t lo = __reduce_min_sync(0xffffffffu, __float_as_uint(big));
+          if (lane == 0) par[512 + NTOK + i / 32] = __uint_as_float(hi), par[516 + NTOK + i / 32] = __uint_as_float(lo);
+          if (i == 0) par_ok[ps] = ok;
         }
         sm100::mbar_arrive(bar(PAR_FULL + ps));
-        // K: rows of tokens.  A quad of lanes reads a token's row; rows r and r ^ 5 in a
-        // phase of eight lanes meet neither each other's banks nor swizzled chunks.
         int slot = kv % kKvSlots;
         if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
         uint32_t dst = sbase + G_::OFF_KV + slot * G_::SLOT;
-#pragma unroll 1
-        for (int unit = i; unit < NTOK * 4; unit += 128) {
-          const int t = unit & 3, half = (unit >> 2) & 1, pair = (unit >> 3) & 3, oct = unit >> 5;
-          const int tok = oct * 8 + (half ? pair ^ 5 : pair);
-          const uint8_t* src = raw + (tok / 16) * BLK + (tok % 16) * (D / 2) + t * (D / 8);
-          uint32_t w[D / 32];
-          if constexpr (D == 128) {
-            const uint4 y = *reinterpret_cast<const uint4*>(src);
-            w[0] = y.x, w[1] = y.y, w[2] = y.z, w[3] = y.w;
-          } else {
-            const uint2 y = *reinterpret_cast<const uint2*>(src);
-            w[0] = y.x, w[1] = y.y;
-          }
+        // K: rows of tokens
+#pragma unroll
+        for (int x = 0; x < KU; ++x) {
+          const int tok = ((i >> 5) + 4 * x) * 8 + tok_in;
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const int o = 4 * j + t;                     // octet of the token's row
-            const uint32_t h = w[j] >> 8;
-            sm100::st_shared_v4(dst + (o / 8) * (NTOK * 128) + swz(tok, o & 7), w[j] & kLoMask,
-                                w[j] & kHiMask, h & kLoMask, h & kHiMask);
+            const uint32_t w = kw[x][j], h = w >> 8;
+            sm100::st_shared_v4(dst + (o / 8) * (NTOK * 128) + swz(tok, o & 7), w & kLoMask, w & kHiMask,
+                                h & kLoMask, h & kHiMask);
           }
         }
         sm100::fence_proxy_async_smem();
         sm100::mbar_arrive(bar(KV_FULL + slot));
         ++kv;
-        // V: rows of channels.  A thread turns 8 tokens of D / 32 quads of channels; a phase
-        // of eight lanes has four runs of 8 tokens and two quads.
+        // V: rows of channels
         slot = kv % kKvSlots;
         if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
-        dst = sbase + G_::OFF_KV + slot * G_::SLOT;
-#pragma unroll 1
-        for (int unit = i; unit < NTOK; unit += 128) {   // 8 x (NTOK / 8) units
-          const int run = (unit & 3) + 4 * (unit >> 5), h8 = (unit >> 2) & 7;
-          const uint8_t* src = raw + (run / 2) * BLK + kv4::off_v(D) + (run & 1) * 4 * D + h8 * (D / 8);
-          uint32_t w[4][D / 32];
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            if constexpr (D == 128) {
-              const uint4 y = *reinterpret_cast<const uint4*>(src + p * D);
-              w[p][0] = y.x, w[p][1] = y.y, w[p][2] = y.z, w[p][3] = y.w;
-            } else {
-              const uint2 y = *reinterpret_cast<const uint2*>(src + p * D);
-              w[p][0] = y.x, w[p][1] = y.y;
-            }
-          }
+        dst = sbase + G_::OFF_KV + slot * G_::SLOT + (run / 8) * (D * 128);
+        if (i < NTOK) {
 #pragma unroll
           for (int j = 0; j < D / 32; ++j) {
             const int ch = 4 * (8 * j + h8);             // first of the quad's channels
-            const uint32_t at = dst + (run / 8) * (D * 128);
-            uint32_t e[4], o[4];
-#pragma unroll
-            for (int p = 0; p < 4; ++p) e[p] = w[p][j] & kLoMask, o[p] = w[p][j] & kHiMask;
-            sm100::st_shared_v4(at + swz(ch, run & 7), e[0], e[1], e[2], e[3]);
-            sm100::st_shared_v4(at + swz(ch + 1, run & 7), o[0], o[1], o[2], o[3]);
-#pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const uint32_t hw = w[p][j] >> 8;
-              e[p] = hw & kLoMask, o[p] = hw & kHiMask;
-            }
-            sm100::st_shared_v4(at + swz(ch + 2, run & 7), e[0], e[1], e[2], e[3]);
-            sm100::st_shared_v4(at + swz(ch + 3, run & 7), o[0], o[1], o[2], o[3]);
+            const uint32_t a0 = vw[0][j], a1 = vw[1][j], a2 = vw[2][j], a3 = vw[3][j];
+            sm100::st_shared_v4(dst + swz(ch, run & 7), a0 & kLoMask, a1 & kLoMask, a2 & kLoMask, a3 & kLoMask);
+            sm100::st_shared_v4(dst + swz(ch + 1, run & 7), a0 & kHiMask, a1 & kHiMask, a2 & kHiMask, a3 & kHiMask);
+            const uint32_t b0 = a0 >> 8, b1 = a1 >> 8, b2 = a2 >> 8, b3 = a3 >> 8;
+            sm100::st_shared_v4(dst + swz(ch + 2, run & 7), b0 & kLoMask, b1 & kLoMask, b2 & kLoMask, b3 & kLoMask);
+            sm100::st_shared_v4(dst + swz(ch + 3, run & 7), b0 & kHiMask, b1 & kHiMask, b2 & kHiMask, b3 & kHiMask);
           }
         }
         sm100::mbar_arrive(bar(RAW_EMPTY + rs));
@@ -637,33 +668,33 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
       }
     }
   } else {
-    sm100::setmaxnreg_dec<64>();
+    sm100::setmaxnreg_dec<88>();
     if (warp == 12 && lane == 0) {
       // ---- MMA issue ---------------------------------------------------------------------------
       constexpr uint32_t idS = sm100::idesc_f16_f32(128, NTOK, 0, 0);
       constexpr uint32_t idO = sm100::idesc_f16_f32(128, GROUP, 0, 0);
       int kv = 0, np[2] = {0, 0}, nq[2] = {0, 0};
       bool live = true;
+      // descriptors differ in their start address (low bits, in 16-byte units) only
+      const uint64_t dq = sm100::umma_desc_sw128(sbase + G_::OFF_Q, 16, 1024);
+      const uint64_t dkv = sm100::umma_desc_sw128(sbase + G_::OFF_KV, 16, 1024);
       auto issue_s = [&](int T, int slot) {
-        const uint32_t q = sbase + G_::OFF_Q + T * G_::QTILE, kk0 = sbase + G_::OFF_KV + slot * G_::SLOT;
+        const uint64_t q = dq + (uint32_t)(T * (G_::QTILE / 16)), kd = dkv + (uint32_t)(slot * (G_::SLOT / 16));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t ad = sm100::umma_desc_sw128(q + (kk / 4) * (128 * 128) + (kk & 3) * 32, 16, 1024);
-          const uint64_t bd = sm100::umma_desc_sw128(kk0 + (kk / 4) * (NTOK * 128) + (kk & 3) * 32, 16, 1024);
-          sm100::umma_f16(tmem + T * 128 + (kk * 16 / GROUP) * NTOK, ad, bd, idS, kk * 16 % GROUP != 0);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)
+          sm100::umma_f16(tmem + T * 128 + (kk * 16 / GROUP) * NTOK, q + ((kk / 4) * (128 * 128) + (kk & 3) * 32) / 16,
+                          kd + ((kk / 4) * (NTOK * 128) + (kk & 3) * 32) / 16, idS, kk * 16 % GROUP != 0);
         sm100::umma_commit(bar(S_FULL + T));
       };
       auto issue_o = [&](int T, int slot, bool first) {
-        const uint32_t v = sbase + G_::OFF_KV + slot * G_::SLOT;
+        const uint64_t vd = dkv + (uint32_t)(slot * (G_::SLOT / 16));
 #pragma unroll
         for (int g = 0; g < NG; ++g)
 #pragma unroll
-          for (int kk = 0; kk < NTOK / 16; ++kk) {
-            const uint64_t bd = sm100::umma_desc_sw128(v + (kk / 4) * (D * 128) + g * GROUP * 128 + (kk & 3) * 32, 16, 1024);
-            sm100::umma_f16_ts(tmem + 256 + T * 128 + g * GROUP, tmem + T * 128 + g * (NTOK / 2) + kk * 8, bd,
-                               idO, !first || kk != 0);
-          }
+          for (int kk = 0; kk < NTOK / 16; ++kk)
+            sm100::umma_f16_ts(tmem + 256 + T * 128 + g * GROUP, tmem + T * 128 + g * NTOK + kk * 8,
+                               vd + ((kk / 4) * (D * 128) + g * GROUP * 128 + (kk & 3) * 32) / 16, idO,
+                               !first || kk != 0);
       };
       for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
         const Segment sg(it, a, u, u0, u1);
