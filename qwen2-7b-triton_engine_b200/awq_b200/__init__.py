@@ -294,6 +294,10 @@ def gemm_epilogue(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor
     ``residual`` (the residual stream updated in place); otherwise it must overlap no input.
     Outside graph capture the split-K workspace is the one of the current stream; a captured
     call gets its own, so that graphs may replay at the same time."""
+    if _ext is not None and all(t is None or isinstance(t, torch.Tensor)
+                                for t in (x2d, qweight, qzeros, scales, bias, residual, out)):
+        return _ext.gemm_epilogue(x2d, qweight, qzeros, scales, int(group_size), bias, activation,
+                                  residual, out)
     K, N, qweight, qzeros, scales = _prepared_weights(qweight, qzeros, scales, group_size)
     _require_cuda(x2d, "x")
     if x2d.dtype != torch.float16:

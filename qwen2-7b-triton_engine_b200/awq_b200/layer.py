@@ -18,6 +18,7 @@ formats and refusals: include/awq_b200.h.
 from __future__ import annotations
 
 import ctypes
+import sys
 from dataclasses import dataclass
 
 import torch
@@ -29,8 +30,18 @@ __all__ = ["KV4Cache", "rope_axes", "kv4_pages_step", "kv4_append", "kv4_gather"
 
 
 def _core():
-    import awq_b200
-    return awq_b200
+    return sys.modules[__package__]
+
+
+def _ext():
+    """The C++ host glue (the same steps as the functions below), or None."""
+    return _core()._ext
+
+
+def _tensors(*args) -> bool:
+    """Whether all arguments are tensors (or None): what the C++ signatures take.  Others go
+    through the Python path, which names them."""
+    return all(a is None or isinstance(a, torch.Tensor) for a in args)
 
 
 def _need(t, name: str, dtype, ndim: int, device=None) -> None:
@@ -126,6 +137,10 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
     i % axes while that axis has sections left, else to axis 0.  Angles keep full accuracy at
     any position.  Returns (out_q, out_k): new dense tensors, or those given, which may be q
     and k themselves (in place)."""
+    ext = _ext()
+    if ext is not None and _tensors(q, k, positions, inv_freq, out_q, out_k):
+        return ext.rope_axes(q, k, positions, inv_freq, [int(x) for x in sections],
+                             bool(interleaved), out_q, out_k)
     _need(q, "q", torch.float16, 3)
     dev = q.device
     _need(k, "k", torch.float16, 3, dev)
@@ -198,6 +213,11 @@ def kv4_pages_step(block_table: torch.Tensor, held: torch.Tensor, free_pages: to
     where each new token goes and its position, request after request, -1 and 0 behind the
     last one.  status 0; n > 0: n pages short; -1: a length out of range.  A refused step
     (status not 0) changes nothing and has no tokens.  At most 8192 requests."""
+    ext = _ext()
+    if ext is not None and _tensors(block_table, held, free_pages, free_count, kv_lens,
+                                    new_tokens, reset):
+        return ext.kv4_pages_step(block_table, held, free_pages, free_count, kv_lens, new_tokens,
+                                  int(page_size), int(max_tokens), reset)
     _need(block_table, "block_table", torch.int32, 2)
     dev = block_table.device
     R, width = block_table.shape
@@ -233,6 +253,10 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KV4
     """Quantize k and v [T, kv_heads, head_dim] (fp16, strided views are read in place) into
     the cache's slots (int64 [T], page * page_size + offset; negative: skipped).  The slots of
     a call must differ, as those of ``kv4_pages_step`` do."""
+    ext = _ext()
+    if ext is not None and _tensors(k, v, slots):
+        return ext.kv4_append(k, v, slots, cache.data, cache.head_dim, cache.page_size,
+                              cache.group_size)
     dev = cache._check()
     _need(k, "k", torch.float16, 3, dev)
     _need(v, "v", torch.float16, 3, dev)
@@ -255,6 +279,9 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: KV4
 def kv4_gather(cache: KV4Cache, slots: torch.Tensor):
     """(k, v) fp16 [T, kv_heads, head_dim] of the cache's slots (int64 [T]; zeros where a slot
     is negative): what attention reads, rounded to fp16."""
+    ext = _ext()
+    if ext is not None and _tensors(slots):
+        return ext.kv4_gather(cache.data, cache.head_dim, cache.page_size, cache.group_size, slots)
     dev = cache._check()
     _need(slots, "slots", torch.int64, 1, dev)
     T = slots.shape[0]
@@ -283,6 +310,10 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
     on it).  Query head h reads kv head h // (q_heads / kv_heads).  scale defaults to
     head_dim ** -0.5.  Rows that see no token are zeros.  Rows behind cu_q[R] are left as they
     are in ``out`` and are zeros in a new tensor."""
+    ext = _ext()
+    if ext is not None and _tensors(q, block_table, kv_lens, cu_q, out):
+        return ext.kv4_attention(q, cache.data, cache.head_dim, cache.page_size, cache.group_size,
+                                 block_table, kv_lens, cu_q, int(max_q), scale, out)
     dev = cache._check()
     _need(q, "q", torch.float16, 3, dev)
     T, H, D = q.shape

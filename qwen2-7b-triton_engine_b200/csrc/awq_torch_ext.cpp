@@ -15,9 +15,14 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <cmath>
+#include <cstdlib>
 #include <map>
 #include <mutex>
+#include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/awq_b200.h"
 
@@ -175,6 +180,323 @@ at::Tensor forward_impl(const at::Tensor& x, const at::Tensor& qw, const at::Ten
   return out.view(shape);
 }
 
+// ---- the operators between the products (awq_b200/layer.py has the same steps in Python) ----
+
+using OptTensor = c10::optional<at::Tensor>;
+
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+void need(const at::Tensor& t, const char* name, at::ScalarType dtype, int64_t ndim,
+          const at::Device* dev = nullptr) {
+  require_cuda(t, name);
+  TORCH_CHECK_TYPE(t.scalar_type() == dtype, name, " must be ", c10::toString(dtype), ", got ",
+                   t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == ndim, name, " must be ", ndim, "-D, got shape ", t.sizes());
+  if (dev) TORCH_CHECK_VALUE(t.device() == *dev, name, " is on ", t.device().str(), ", expected ", dev->str());
+}
+
+// A contiguous tensor of exactly this shape (state and outputs, never copied).
+void need_dense(const at::Tensor& t, const char* name, at::ScalarType dtype, at::IntArrayRef shape,
+                const at::Device& dev) {
+  need(t, name, dtype, (int64_t)shape.size(), &dev);
+  TORCH_CHECK_VALUE(t.sizes() == shape && t.is_contiguous(), name, " must be a contiguous ", shape,
+                    " tensor, got ", t.sizes());
+}
+
+at::Tensor last_dense(const at::Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+// Whether the address ranges of two tensors overlap.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  auto span = [](const at::Tensor& t) {
+    int64_t last = t.numel() ? 0 : -1;
+    if (t.numel())
+      for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * std::abs(t.stride(d));
+    const char* p = static_cast<const char*>(t.data_ptr());
+    return std::make_pair(p, p + (last + 1) * t.element_size());
+  };
+  const auto x = span(a), y = span(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+// Different columns of the same rows (views of one fused q/k/v tensor).
+bool apart(const at::Tensor& o, const at::Tensor& y) {
+  if (o.stride(0) != y.stride(0) || o.stride(0) <= 0 || o.stride(1) < 0 || y.stride(1) < 0) return false;
+  const int64_t row = o.stride(0) * 2;
+  auto cols = [](const at::Tensor& t) { return (t.size(1) - 1) * t.stride(1) * 2 + t.size(2) * 2; };
+  int64_t d = (static_cast<const char*>(y.data_ptr()) - static_cast<const char*>(o.data_ptr())) % row;
+  if (d < 0) d += row;
+  return cols(o) <= d && d + cols(y) <= row;
+}
+
+uintptr_t address(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); }
+
+void check(int rc) {
+  if (rc != AWQ_OK) raise_awq(rc);
+}
+
+int activation_code(const c10::optional<std::string>& name) {
+  static const std::map<std::string, int> codes = {{"none", AWQ_ACT_NONE}, {"relu", AWQ_ACT_RELU},
+                                                   {"silu", AWQ_ACT_SILU}, {"gelu", AWQ_ACT_GELU},
+                                                   {"gelu_tanh", AWQ_ACT_GELU_TANH}};
+  if (!name.has_value()) return AWQ_ACT_NONE;
+  const auto it = codes.find(*name);
+  TORCH_CHECK_VALUE(it != codes.end(), "activation '", *name,
+                    "' is none of gelu, gelu_tanh, none, relu, silu");
+  return it->second;
+}
+
+at::Tensor gemm_epilogue(at::Tensor x, at::Tensor qw, at::Tensor qz, at::Tensor s, int64_t gs,
+                         OptTensor bias_opt, const c10::optional<std::string>& activation,
+                         OptTensor res_opt, OptTensor out_opt) {
+  auto [K, N] = check_weights(qw, qz, s, gs);
+  qw = dense16(qw);
+  qz = dense16(qz);
+  s = dense16(s);
+  require_cuda(x, "x");
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kHalf, "x must be float16, got ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) == K, "x must be [M, K=", K, "], got ", x.sizes());
+  TORCH_CHECK_VALUE(x.device() == qw.device(), "x and the weights must be on one device");
+  const at::Device dev = x.device();
+  const int64_t M = x.size(0);
+  const int act = activation_code(activation);
+  at::Tensor bias, res;
+  if (given(bias_opt)) {
+    bias = *bias_opt;
+    need(bias, "bias", at::kHalf, 1, &dev);
+    TORCH_CHECK_VALUE(bias.size(0) == N, "bias must be [", N, "], got ", bias.sizes());
+  }
+  if (given(res_opt)) {
+    res = *res_opt;
+    need(res, "residual", at::kHalf, 2, &dev);
+    TORCH_CHECK_VALUE(res.size(0) == M && res.size(1) == N, "residual must be [", M, ", ", N, "], got ", res.sizes());
+  }
+  at::Tensor out;
+  if (given(out_opt)) {
+    out = *out_opt;
+    need(out, "out", at::kHalf, 2, &dev);
+    TORCH_CHECK_VALUE(out.size(0) == M && out.size(1) == N && out.stride(1) == 1 &&
+                          (M <= 1 || out.stride(0) >= N) && address(out) % 16 == 0 && out.stride(0) % 8 == 0,
+                      "out must be a [", M, ", ", N, "] tensor with dense, 16-byte aligned rows");
+    const bool same = res.defined() && out.data_ptr() == res.data_ptr() && out.strides() == res.strides();
+    TORCH_CHECK_VALUE(!overlap(out, x) && !(bias.defined() && overlap(out, bias)) &&
+                          !(res.defined() && !same && overlap(out, res)),
+                      "out overlaps an input (it may only be the residual itself)");
+  } else {
+    out = at::empty({M, N}, x.options());
+  }
+  if (M == 0) return out;
+  if (bias.defined()) bias = bias.contiguous();
+  if (res.defined() && (res.stride(1) != 1 || (M > 1 && res.stride(0) < N))) res = res.contiguous();
+  if (x.stride(1) != 1 || address(x) % 16 || (x.stride(0) * 2) % 16 || (M > 1 && x.stride(0) < K)) {
+    x = x.contiguous();
+    if (address(x) % 16) x = x.clone();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
+  const size_t nb = workspace_need(dev.index(), M, N, K, gs, false);
+  at::Tensor ws;
+  if (nb) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    TORCH_CHECK(cudaStreamIsCapturing(st, &cap) == cudaSuccess, "cudaStreamIsCapturing failed");
+    if (cap == cudaStreamCaptureStatusNone) {
+      ws = workspace_for(dev, st, nb);
+    } else {
+      // a captured call has a workspace of its own: graphs may replay at the same time; only
+      // the arrival counters at its head must start at zero
+      ws = at::empty({(int64_t)nb}, x.options().dtype(at::kByte));
+      check(awq_workspace_init(ws.data_ptr(), nb < 65536 ? nb : 65536, st));
+    }
+  }
+  check(awq_gemm_f16_epilogue(x.data_ptr(), std::max(x.stride(0), K), qw.data_ptr<int32_t>(),
+                              qz.data_ptr<int32_t>(), s.data_ptr(), bias.defined() ? bias.data_ptr() : nullptr,
+                              act, res.defined() ? res.data_ptr() : nullptr,
+                              res.defined() ? std::max(res.stride(0), N) : 0, out.data_ptr(),
+                              std::max(out.stride(0), N), M, N, K, gs, ws.defined() ? ws.data_ptr() : nullptr,
+                              ws.defined() ? (size_t)ws.numel() : 0, st));
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Tensor pos,
+                                             const at::Tensor& inv_freq, const std::vector<int64_t>& sections,
+                                             bool interleaved, OptTensor out_q, OptTensor out_k) {
+  need(q, "q", at::kHalf, 3);
+  const at::Device dev = q.device();
+  need(k, "k", at::kHalf, 3, &dev);
+  const int64_t T = q.size(0), D = q.size(2), A = (int64_t)sections.size();
+  TORCH_CHECK_VALUE(k.size(0) == T && k.size(2) == D, "k ", k.sizes(), " does not match q ", q.sizes());
+  int64_t half = 0;
+  bool ok = A >= 1 && A <= 4;
+  int32_t sec[4] = {};
+  for (int64_t i = 0; i < A && ok; ++i) {
+    ok = sections[i] >= 0 && sections[i] <= D;
+    sec[i] = (int32_t)sections[i];
+    half += sections[i];
+  }
+  TORCH_CHECK_VALUE(ok && half >= 1 && 2 * half <= D, "sections=", sections,
+                    " must be 1 to 4 counts that rotate 2 to ", D, " channels");
+  require_cuda(pos, "positions");
+  if (pos.dim() == 1) pos = pos.unsqueeze(0);
+  TORCH_CHECK_TYPE(pos.scalar_type() == at::kLong || pos.scalar_type() == at::kInt,
+                   "positions must be int64 or int32, got ", pos.scalar_type());
+  need(pos, "positions", pos.scalar_type(), 2, &dev);
+  TORCH_CHECK_VALUE(pos.size(0) == A && pos.size(1) == T, "positions must be [", A, ", ", T, "], got ", pos.sizes());
+  need_dense(inv_freq, "inv_freq", at::kFloat, {half}, dev);
+  if (T) pos = last_dense(pos);
+  if (T) q = last_dense(q), k = last_dense(k);
+  at::Tensor outs[2];
+  const OptTensor* asked[2] = {&out_q, &out_k};
+  const at::Tensor ins[2] = {q, k};
+  for (int i = 0; i < 2; ++i) {
+    if (!given(*asked[i])) {
+      outs[i] = at::empty(ins[i].sizes(), ins[i].options());
+      continue;
+    }
+    const char* name = i ? "out_k" : "out_q";
+    const at::Tensor& o = **asked[i];
+    need(o, name, at::kHalf, 3, &dev);
+    TORCH_CHECK_VALUE(o.sizes() == ins[i].sizes() && (D == 1 || o.stride(2) == 1), name, " must be ",
+                      ins[i].sizes(), " with a dense last dimension");
+    const bool same = o.data_ptr() == ins[i].data_ptr() && o.strides() == ins[i].strides();
+    for (int j = 0; j < 2; ++j)
+      TORCH_CHECK_VALUE(!overlap(o, ins[j]) || (same && i == j) || apart(o, ins[j]), name,
+                        " overlaps an input other than as that input itself");
+    outs[i] = o;
+  }
+  if (T == 0) return {outs[0], outs[1]};
+  const c10::cuda::CUDAGuard guard(dev);
+  check(awq_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), q.size(1), k.data_ptr(), k.stride(0), k.stride(1),
+                      k.size(1), T, D, pos.data_ptr(), pos.scalar_type() == at::kLong, pos.stride(0),
+                      inv_freq.data_ptr<float>(), sec, (int)A, interleaved, outs[0].data_ptr(), outs[0].stride(0),
+                      outs[0].stride(1), outs[1].data_ptr(), outs[1].stride(0), outs[1].stride(1),
+                      at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {outs[0], outs[1]};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> kv4_pages_step(
+    const at::Tensor& table, const at::Tensor& held, const at::Tensor& free_pages, const at::Tensor& free_count,
+    const at::Tensor& kv_lens, const at::Tensor& new_tokens, int64_t page_size, int64_t max_tokens,
+    OptTensor reset) {
+  need(table, "block_table", at::kInt, 2);
+  const at::Device dev = table.device();
+  const int64_t R = table.size(0), width = table.size(1);
+  TORCH_CHECK_VALUE((!width || width == 1 || table.stride(1) == 1) && (R <= 1 || table.stride(0) >= width),
+                    "block_table must have dense, non-overlapping rows");
+  need_dense(held, "held", at::kInt, {R}, dev);
+  need(free_pages, "free_pages", at::kInt, 1, &dev);
+  TORCH_CHECK_VALUE(free_pages.is_contiguous(), "free_pages must be contiguous");
+  need_dense(free_count, "free_count", at::kInt, {1}, dev);
+  need_dense(kv_lens, "kv_lens", at::kInt, {R}, dev);
+  need_dense(new_tokens, "new_tokens", at::kInt, {R}, dev);
+  if (given(reset)) {
+    require_cuda(*reset, "reset");
+    TORCH_CHECK_TYPE(reset->scalar_type() == at::kBool || reset->scalar_type() == at::kByte,
+                     "reset must be bool or uint8, got ", reset->scalar_type());
+    need_dense(*reset, "reset", reset->scalar_type(), {R}, dev);
+  }
+  TORCH_CHECK_VALUE(page_size >= 1 && max_tokens >= 0, "page_size must be positive and max_tokens not negative");
+  at::Tensor slots = at::empty({max_tokens}, table.options().dtype(at::kLong));
+  at::Tensor ints = at::empty({max_tokens + 2 * R + 2}, table.options());
+  int32_t* p = ints.data_ptr<int32_t>();
+  const c10::cuda::CUDAGuard guard(dev);
+  check(awq_kv4_pages_step(table.data_ptr<int32_t>(), R > 1 ? table.stride(0) : width, width,
+                           held.data_ptr<int32_t>(), free_pages.data_ptr<int32_t>(), free_pages.numel(),
+                           free_count.data_ptr<int32_t>(), kv_lens.data_ptr<int32_t>(),
+                           new_tokens.data_ptr<int32_t>(),
+                           given(reset) ? static_cast<const uint8_t*>(reset->data_ptr()) : nullptr, R, page_size,
+                           slots.data_ptr<int64_t>(), p, max_tokens, p + max_tokens, p + max_tokens + R + 1,
+                           p + max_tokens + 2 * R + 1, at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {slots, ints.narrow(0, 0, max_tokens), ints.narrow(0, max_tokens, R + 1),
+          ints.narrow(0, max_tokens + R + 1, R), ints.narrow(0, max_tokens + 2 * R + 1, 1)};
+}
+
+void kv4_append(at::Tensor k, at::Tensor v, at::Tensor slots, const at::Tensor& data, int64_t D, int64_t page,
+                int64_t group) {
+  require_cuda(data, "cache.data");
+  const at::Device dev = data.device();
+  need(k, "k", at::kHalf, 3, &dev);
+  need(v, "v", at::kHalf, 3, &dev);
+  need(slots, "slots", at::kLong, 1, &dev);
+  const int64_t T = slots.size(0), H = data.size(1);
+  const int64_t want[3] = {T, H, D};
+  TORCH_CHECK_VALUE(k.sizes() == at::IntArrayRef(want, 3) && v.sizes() == at::IntArrayRef(want, 3), "k ", k.sizes(),
+                    " and v ", v.sizes(), " must be [", T, ", ", H, ", ", D, "]");
+  if (T == 0) return;
+  k = last_dense(k);
+  v = last_dense(v);
+  slots = slots.contiguous();
+  const c10::cuda::CUDAGuard guard(dev);
+  check(awq_kv4_append(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                       slots.data_ptr<int64_t>(), T, data.data_ptr(), data.size(0), H, D, group, page,
+                       at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+}
+
+std::tuple<at::Tensor, at::Tensor> kv4_gather(const at::Tensor& data, int64_t D, int64_t page, int64_t group,
+                                              at::Tensor slots) {
+  require_cuda(data, "cache.data");
+  const at::Device dev = data.device();
+  need(slots, "slots", at::kLong, 1, &dev);
+  const int64_t T = slots.size(0), H = data.size(1);
+  at::Tensor k = at::empty({T, H, D}, data.options().dtype(at::kHalf)), v = at::empty_like(k);
+  if (T == 0) return {k, v};
+  slots = slots.contiguous();
+  const c10::cuda::CUDAGuard guard(dev);
+  check(awq_kv4_gather(data.data_ptr(), data.size(0), H, D, group, page, slots.data_ptr<int64_t>(), T, k.data_ptr(),
+                       v.data_ptr(), at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return {k, v};
+}
+
+at::Tensor kv4_attention(at::Tensor q, const at::Tensor& data, int64_t D, int64_t page, int64_t group,
+                         at::Tensor table, const at::Tensor& kv_lens, OptTensor cu_q, int64_t max_q,
+                         c10::optional<double> scale, OptTensor out_opt) {
+  require_cuda(data, "cache.data");
+  const at::Device dev = data.device();
+  need(q, "q", at::kHalf, 3, &dev);
+  const int64_t T = q.size(0), H = q.size(1), Hk = data.size(1);
+  TORCH_CHECK_VALUE(q.size(2) == D, "q has head_dim ", q.size(2), ", the cache ", D);
+  TORCH_CHECK_VALUE(H >= 1 && H % Hk == 0, H, " query heads do not group over ", Hk, " kv heads");
+  need(table, "block_table", at::kInt, 2, &dev);
+  const int64_t R = table.size(0), width = table.size(1);
+  if ((width > 1 && table.stride(1) != 1) || (R > 1 && table.stride(0) < width)) table = table.contiguous();
+  need_dense(kv_lens, "kv_lens", at::kInt, {R}, dev);
+  const bool ragged = given(cu_q);
+  if (!ragged) {
+    TORCH_CHECK_VALUE(T == R && max_q == 1, "without cu_q every request has one query row: ", T, " rows, ", R,
+                      " requests, max_q=", max_q);
+  } else {
+    need_dense(*cu_q, "cu_q", at::kInt, {R + 1}, dev);
+    TORCH_CHECK_VALUE(max_q >= 1, "max_q must be positive");
+  }
+  if (q.numel() && (q.stride(2) != 1 || address(q) % 16 || q.stride(0) % 8 || q.stride(1) % 8)) {
+    q = q.contiguous();
+    if (address(q) % 16) q = q.clone();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  at::Tensor out;
+  if (given(out_opt)) {
+    out = *out_opt;
+    need(out, "out", at::kHalf, 3, &dev);
+    TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.stride(2) == 1 && address(out) % 8 == 0 &&
+                          out.stride(0) % 4 == 0 && out.stride(1) % 4 == 0,
+                      "out must be ", q.sizes(), " with a dense last dimension, 8-byte aligned rows");
+    TORCH_CHECK_VALUE(!overlap(out, q), "out overlaps q");
+  } else {
+    out = ragged ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());
+  }
+  if (T == 0 || R == 0) return out;
+  const size_t nb = awq_kv4_attention_workspace_bytes(D, std::min(max_q, T) * (H / Hk));
+  // a workspace of this call alone: graphs that replay at once must not share one
+  at::Tensor ws = at::empty({(int64_t)nb}, data.options());
+  check(awq_kv4_attention(q.data_ptr(), q.stride(0), q.stride(1), T, H, data.data_ptr(), data.size(0), Hk, D, group,
+                          page, table.data_ptr<int32_t>(), R > 1 ? table.stride(0) : width, width,
+                          kv_lens.data_ptr<int32_t>(), ragged ? cu_q->data_ptr<int32_t>() : nullptr, R, max_q,
+                          (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)D)), out.data_ptr(),
+                          out.stride(0), out.stride(1), ws.data_ptr(), nb,
+                          at::cuda::getCurrentCUDAStream(dev.index()).stream()));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -204,4 +526,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                const at::Tensor& s, int64_t gs) {
           return forward_impl(x, qw, qz, s, gs, c10::nullopt, true);
         });
+  m.def("gemm_epilogue", &gemm_epilogue);
+  m.def("rope_axes", &rope_axes);
+  m.def("kv4_pages_step", &kv4_pages_step);
+  m.def("kv4_append", &kv4_append);
+  m.def("kv4_gather", &kv4_gather);
+  m.def("kv4_attention", &kv4_attention);
 }
