@@ -28,140 +28,179 @@ struct Kv4IoArgs {
   __half* out_k;                    // gather: [T, H, D] contiguous
   __half* out_v;
   int64_t T, capacity;              // tokens; num_pages * page_size
-  int H, page;
+  int H, page_shift;
   int* status;
 };
 
-// Round-to-nearest-even of the exact (x - m) / s, 0..15.  The fp32 quotient is within
-// 2^-21 of the exact one here (three roundings of 2^-24 each, quotient below 2^5), so only
-// results that close to a tie take the double division, which decides every tie: x - m is
-// exact in double, and an fp16 / fp16-difference quotient that is not a tie lies further
-// than 2^-46 from one.
-__device__ __forceinline__ uint32_t quant1(float x, float m, float s, float inv) {
-  const float t = (x - m) * inv;
-  float r = rintf(t);
-  if (fabsf(t - r) > 0.4999f) r = (float)rint(((double)x - (double)m) / (double)s);
-  return (uint32_t)fminf(fmaxf(r, 0.f), 15.f);
+__device__ __forceinline__ uint32_t hmin2_u32(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("min.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmax2_u32(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
-// The four codes of a lane's channels (nibble p = channel p), its group's scale and
-// minimum.  LG lanes of four channels form a group.
+// fp16((hi - lo) / 15), rounded once.  The fp32 quotient is within 2^-22 of the exact one; where
+// both ends of that interval round to the same fp16 value that is the result, otherwise (about
+// one group in a thousand) the double quotient decides: hi - lo is exact in double, and an
+// integer multiple of a power of two over 15 that is not a tie is far further than 2^-50 from
+// one.
+__device__ __forceinline__ __half scale_of(float lo, float hi) {
+  const float q = (hi - lo) * (1.0f / 15.0f);
+  const __half a = __float2half_rn(q * (1.0f - 0x1p-21f)), b = __float2half_rn(q * (1.0f + 0x1p-21f));
+  if (__half_as_ushort(a) == __half_as_ushort(b)) return a;
+  return __double2half(((double)hi - (double)lo) / 15.0);
+}
+
+// The codes of a lane's octet of channels (nibble p = channel p), its group's scale and minimum.
+// LG lanes form a group; u: the eight fp16 values.  Every lane of the warp calls it.
+//
+// A code is the round-to-nearest-even of the exact (x - m) / s, at most 15.  The fp32 quotient
+// is within 2^-18 of the exact one (three roundings of 2^-24 and a reciprocal of 2^-23, quotient
+// below 2^5), so only results within 10^-5 of a tie take the double division, which decides
+// every tie (x - m is exact in double).  So do groups whose scale is subnormal: elsewhere the
+// scale's own rounding (2^-11) leaves the quotient below 15.5.
 template <int LG>
-__device__ __forceinline__ uint32_t quant_quad(const float (&x)[4], __half& sh, __half& mh) {
-  float lo = fminf(fminf(x[0], x[1]), fminf(x[2], x[3]));
-  float hi = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-  // a sum of differences that is not zero marks a NaN or an infinity
-  bool bad = !((x[0] - x[0]) + (x[1] - x[1]) + (x[2] - x[2]) + (x[3] - x[3]) == 0.f);
+__device__ __forceinline__ uint32_t quant_octet(const uint4 u, int lane, __half& sh, __half& mh) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  // (minimum, -maximum) of the group in one register
+  const uint32_t lo2 = hmin2_u32(hmin2_u32(w[0], w[1]), hmin2_u32(w[2], w[3]));
+  const uint32_t hi2 = hmax2_u32(hmax2_u32(w[0], w[1]), hmax2_u32(w[2], w[3])) ^ 0x80008000u;
+  uint32_t v = hmin2_u32(__byte_perm(lo2, hi2, 0x5410), __byte_perm(lo2, hi2, 0x7632));
 #pragma unroll
-  for (int o = LG / 2; o > 0; o >>= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    bad |= (bool)__shfl_xor_sync(0xffffffffu, (int)bad, o);
-  }
-  lo += 0.f, hi += 0.f;                              // one zero: -0 is stored as +0
-  sh = __double2half(((double)hi - (double)lo) / 15.0);
-  mh = __float2half_rn(lo);                          // exact: lo is one of the inputs
-  if (bad) sh = mh = __ushort_as_half(0x7FFF);
+  for (int o = LG / 2; o > 0; o >>= 1) v = hmin2_u32(v, __shfl_xor_sync(0xffffffffu, v, o));
+  // an exponent of all ones marks an infinity or a NaN
+  uint32_t odd = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) odd |= (w[k] & 0x7FFF7FFFu) + 0x04000400u;
+  const uint32_t group = ((1u << LG) - 1u) << (lane & ~(LG - 1));
+  const bool bad = (__ballot_sync(0xffffffffu, (odd & 0x80008000u) != 0) & group) != 0;
+  const float2 mm = __half22float2(u32_as_h2(v));
+  const float lo = mm.x + 0.f, hi = 0.f - mm.y;      // one zero: -0 is stored as +0
+  sh = bad ? __ushort_as_half(0x7FFF) : scale_of(lo, hi);
+  mh = bad ? __ushort_as_half(0x7FFF) : __float2half_rn(lo);
   const float s = __half2float(sh);
   if (!(s > 0.f)) return 0;
-  const float inv = 1.0f / s;
-  uint32_t c = 0;
+  const float inv = __fdividef(1.0f, s);
+  float x[8];
 #pragma unroll
-  for (int p = 0; p < 4; ++p) c |= quant1(x[p], lo, s, inv) << (4 * p);
+  for (int k = 0; k < 4; ++k) {
+    const float2 f = __half22float2(u32_as_h2(w[k]));
+    x[2 * k] = f.x, x[2 * k + 1] = f.y;
+  }
+  // t + 1.5 * 2^23 rounds t to an integer (ties to even) in the low bits of the float
+  uint32_t b[8];
+  float worst = 0.f;
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const float t = (x[p] - lo) * inv, m = t + 12582912.f;
+    b[p] = __float_as_uint(m);
+    worst = fmaxf(worst, fabsf(t - (m - 12582912.f)));
+  }
+  if (worst > 0.49999f || s < 6.1035156e-5f) {
+#pragma unroll 1
+    for (int p = 0; p < 8; ++p) {
+      const uint32_t c = (uint32_t)fmin(rint(((double)__half2float(__ushort_as_half(
+                             (uint16_t)(w[p >> 1] >> (16 * (p & 1))))) - (double)lo) / (double)s), 15.0);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (q == p) b[q] = 0x4B400000u + c;
+    }
+  }
+  // 1.5 * 2^23 is 0x4B400000: of sum b[p] 16^p, 0x4B400000 (1 + 16 + 256) is the floats' own
+  uint32_t c = b[0] - 0x4B400000u * 273u;
+#pragma unroll
+  for (int p = 1; p < 8; ++p) c += b[p] << (4 * p);
   return c;
 }
 
-__device__ __forceinline__ void load_quad(const __half* p, bool vec, float (&x)[4]) {
-  if (vec) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-    const float2 a = __half22float2(u32_as_h2(u.x)), b = __half22float2(u32_as_h2(u.y));
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __half2float(p[i]);
-  }
+__device__ __forceinline__ uint4 load_octet(const __half* p, bool vec) {
+  if (vec) return *reinterpret_cast<const uint4*>(p);
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16,
+                    h[6] | (uint32_t)h[7] << 16);
 }
 
-// D/4 lanes per (token, head); grid-stride over the T * H rows, whole warps at a time so
-// that the shuffles always see 32 lanes.
+// D/8 lanes per token, one kv head per blockIdx.y; whole warps at a time, so that the shuffles
+// always see 32 lanes.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(256)
 kv4_append_kernel(const Kv4IoArgs a, const int vec_k, const int vec_v) {
-  constexpr int L = D / 4, ROWS = 32 / L, NG = D / GROUP;
-  const int lane = threadIdx.x & 31, c = lane % L;
-  const int64_t rows = a.T * a.H;
-  const int64_t step = (int64_t)gridDim.x * (blockDim.x / 32) * ROWS;
-  for (int64_t r0 = ((int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32) * ROWS; r0 < rows;
-       r0 += step) {
-    const int64_t row = r0 + lane / L;
-    const bool in = row < rows;
-    const int64_t tok = in ? row / a.H : 0;
-    const int h = in ? (int)(row - tok * a.H) : 0;
+  constexpr int L = D / 8, ROWS = 32 / L, NG = D / GROUP;
+  const int lane = threadIdx.x & 31, o = lane % L, h = blockIdx.y;
+  const int64_t step = (int64_t)gridDim.x * 8 * ROWS;
+  for (int64_t t0 = ((int64_t)blockIdx.x * 8 + threadIdx.x / 32) * ROWS; t0 < a.T; t0 += step) {
+    const int64_t tok = t0 + lane / L;
+    const bool in = tok < a.T;
     const int64_t slot = in ? a.slots[tok] : -1;
-    float kx[4] = {}, vx[4] = {};
+    uint4 ku = make_uint4(0, 0, 0, 0), vu = ku;
     if (in) {
-      load_quad(a.k + tok * a.k_ts + h * a.k_hs + 4 * c, vec_k, kx);
-      load_quad(a.v + tok * a.v_ts + h * a.v_hs + 4 * c, vec_v, vx);
+      ku = load_octet(a.k + tok * a.k_ts + h * a.k_hs + 8 * o, vec_k);
+      vu = load_octet(a.v + tok * a.v_ts + h * a.v_hs + 8 * o, vec_v);
     }
     __half ks, km, vs, vm;
-    const uint32_t kc = quant_quad<GROUP / 4>(kx, ks, km);
-    const uint32_t vc = quant_quad<GROUP / 4>(vx, vs, vm);
-    const uint32_t kn = __shfl_down_sync(0xffffffffu, kc, 1);
+    const uint32_t kc = quant_octet<GROUP / 8>(ku, lane, ks, km);
+    const uint32_t vc = quant_octet<GROUP / 8>(vu, lane, vs, vm);
     if (slot < 0) continue;                          // padding: nothing is written
     if (slot >= a.capacity) {
-      if (c == 0) atomicOr(a.status, kDevErrShape);
+      if (o == 0) atomicOr(a.status, kDevErrShape);
       continue;
     }
-    const int64_t page = slot / a.page;
-    const int at = (int)(slot - page * a.page), b = at & 15;
-    uint8_t* blk = a.cache + ((page * a.H + h) * (a.page / 16) + at / 16) * kv4::block_bytes(D, GROUP);
-    if ((c & 1) == 0)
-      *reinterpret_cast<uint32_t*>(blk + b * (D / 2) + 4 * kv4::k_word(D, c / 2)) = kc | kn << 16;
-    *reinterpret_cast<uint16_t*>(blk + kv4::off_v(D) + (b / 2) * D + 4 * kv4::v_word(D, c) + 2 * (b & 1)) =
-        (uint16_t)vc;
-    if (c % (GROUP / 4) == 0) {
-      const int gi = c / (GROUP / 4);
+    const int64_t page = slot >> a.page_shift;
+    const int at = (int)slot & ((1 << a.page_shift) - 1), b = at & 15;
+    uint8_t* blk = a.cache + (((page * a.H + h) << (a.page_shift - 4)) + (at >> 4)) * kv4::block_bytes(D, GROUP);
+    *reinterpret_cast<uint32_t*>(blk + b * (D / 2) + 4 * kv4::k_word(D, o)) = kc;
+    uint8_t* vrow = blk + kv4::off_v(D) + (b / 2) * D + 2 * (b & 1);
+    *reinterpret_cast<uint16_t*>(vrow + 4 * kv4::v_word(D, 2 * o)) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t*>(vrow + 4 * kv4::v_word(D, 2 * o + 1)) = (uint16_t)(vc >> 16);
+    if (o % (GROUP / 8) == 0) {
+      const int gi = o / (GROUP / 8);
       reinterpret_cast<__half2*>(blk + kv4::off_kp(D))[b * NG + gi] = __halves2half2(ks, km);
       reinterpret_cast<__half2*>(blk + kv4::off_vp(D, GROUP))[b * NG + gi] = __halves2half2(vs, vm);
     }
   }
 }
 
-// fp16(code * scale + minimum) of the slots' keys and values; a negative slot reads as 0.
+// fp16(code * scale + minimum) of the slots' keys and values; a negative slot reads as 0.  One
+// thread per octet of channels of a token's K and V rows.
 template <int D, int GROUP>
 __global__ void __launch_bounds__(256) kv4_gather_kernel(const Kv4IoArgs a) {
-  constexpr int L = D / 4, NG = D / GROUP;
-  const int64_t total = a.T * a.H * L;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t row = i / L, tok = row / a.H;
-    const int c = (int)(i - row * L), h = (int)(row - tok * a.H);
+  constexpr int L = D / 8, NG = D / GROUP;
+  const int o = threadIdx.x % L, h = blockIdx.y;
+  const int64_t step = (int64_t)gridDim.x * (256 / L);
+  for (int64_t tok = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L; tok < a.T; tok += step) {
     const int64_t slot = a.slots[tok];
-    uint2 ko = make_uint2(0, 0), vo = make_uint2(0, 0);
+    uint4 ko = make_uint4(0, 0, 0, 0), vo = make_uint4(0, 0, 0, 0);
     if (slot >= a.capacity) {
-      if (c == 0) atomicOr(a.status, kDevErrShape);
+      if (o == 0) atomicOr(a.status, kDevErrShape);
     } else if (slot >= 0) {
-      const int64_t page = slot / a.page;
-      const int at = (int)(slot - page * a.page), b = at & 15;
-      const uint8_t* blk = a.cache + ((page * a.H + h) * (a.page / 16) + at / 16) * kv4::block_bytes(D, GROUP);
-      const uint32_t kc = *reinterpret_cast<const uint16_t*>(
-          blk + b * (D / 2) + 4 * kv4::k_word(D, c / 2) + 2 * (c & 1));
-      const uint32_t vc = *reinterpret_cast<const uint16_t*>(
-          blk + kv4::off_v(D) + (b / 2) * D + 4 * kv4::v_word(D, c) + 2 * (b & 1));
-      const int gi = c / (GROUP / 4);
+      const int64_t page = slot >> a.page_shift;
+      const int at = (int)slot & ((1 << a.page_shift) - 1), b = at & 15;
+      const uint8_t* blk = a.cache + (((page * a.H + h) << (a.page_shift - 4)) + (at >> 4)) * kv4::block_bytes(D, GROUP);
+      const uint32_t kc = *reinterpret_cast<const uint32_t*>(blk + b * (D / 2) + 4 * kv4::k_word(D, o));
+      const uint8_t* vrow = blk + kv4::off_v(D) + (b / 2) * D + 2 * (b & 1);
+      const uint32_t vc = *reinterpret_cast<const uint16_t*>(vrow + 4 * kv4::v_word(D, 2 * o)) |
+                          (uint32_t)*reinterpret_cast<const uint16_t*>(vrow + 4 * kv4::v_word(D, 2 * o + 1)) << 16;
+      const int gi = o / (GROUP / 8);
       const float2 kp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_kp(D))[b * NG + gi]);
       const float2 vp = __half22float2(reinterpret_cast<const __half2*>(blk + kv4::off_vp(D, GROUP))[b * NG + gi]);
-      float kf[4], vf[4];
+      uint32_t kw[4], vw[4];
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
-        kf[p] = fmaf((float)((kc >> (4 * p)) & 15u), kp.x, kp.y);
-        vf[p] = fmaf((float)((vc >> (4 * p)) & 15u), vp.x, vp.y);
+        kw[p] = h2_as_u32(__floats2half2_rn(fmaf((float)((kc >> (8 * p)) & 15u), kp.x, kp.y),
+                                            fmaf((float)((kc >> (8 * p + 4)) & 15u), kp.x, kp.y)));
+        vw[p] = h2_as_u32(__floats2half2_rn(fmaf((float)((vc >> (8 * p)) & 15u), vp.x, vp.y),
+                                            fmaf((float)((vc >> (8 * p + 4)) & 15u), vp.x, vp.y)));
       }
-      ko = make_uint2(h2_as_u32(__floats2half2_rn(kf[0], kf[1])), h2_as_u32(__floats2half2_rn(kf[2], kf[3])));
-      vo = make_uint2(h2_as_u32(__floats2half2_rn(vf[0], vf[1])), h2_as_u32(__floats2half2_rn(vf[2], vf[3])));
+      ko = make_uint4(kw[0], kw[1], kw[2], kw[3]);
+      vo = make_uint4(vw[0], vw[1], vw[2], vw[3]);
     }
-    *reinterpret_cast<uint2*>(a.out_k + row * D + 4 * c) = ko;
-    *reinterpret_cast<uint2*>(a.out_v + row * D + 4 * c) = vo;
+    const int64_t out = (tok * a.H + h) * D + 8 * o;
+    *reinterpret_cast<uint4*>(a.out_k + out) = ko;
+    *reinterpret_cast<uint4*>(a.out_v + out) = vo;
   }
 }
 
@@ -188,7 +227,7 @@ struct PagesArgs {
   int64_t max_tokens;
   int R, width, capacity, page;
 };
-constexpr int kPagesThreads = 512;
+constexpr int kPagesThreads = 1024, kPagesFew = 256;
 
 __device__ __forceinline__ long long warp_scan(long long v, int lane) {
 #pragma unroll
@@ -199,119 +238,145 @@ __device__ __forceinline__ long long warp_scan(long long v, int lane) {
   return v;
 }
 
-// Largest r with pre[r] <= j (pre[0] = 0, ascending).
-__device__ __forceinline__ int row_of(const int* pre, int R, int j) {
-  int lo = 0, hi = R;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (pre[mid] <= j) lo = mid; else hi = mid;
-  }
-  return lo;
+// Rows of N elements at once (the bisections overlap): the largest r with pre[r] <= j[n]
+// (pre[0] = 0, ascending).
+template <int N>
+__device__ __forceinline__ void rows_of(const int* pre, int R, const int (&j)[N], int (&row)[N]) {
+  int hi[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) row[n] = 0, hi[n] = R;
+  for (int span = R; span > 1; span = (span + 1) >> 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int mid = (row[n] + hi[n]) >> 1;
+      if (hi[n] - row[n] > 1) {
+        if (pre[mid] <= j[n]) row[n] = mid; else hi[n] = mid;
+      }
+    }
 }
 
-__global__ void __launch_bounds__(kPagesThreads) kv4_pages_kernel(const PagesArgs a) {
+// THREADS a CTA, up to PER rows a thread (THREADS = 256: one CTA, which needs no cluster).
+template <int THREADS, int PER>
+__global__ void __launch_bounds__(THREADS) kv4_pages_kernel(const PagesArgs a) {
   namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
-  extern __shared__ int sm[];                        // pre[3][R + 1]
-  __shared__ long long wsum[3][kPagesThreads / 32];
-  __shared__ long long carry[3];
+  constexpr bool kAlone = THREADS == kPagesFew;
+  auto everyone = [] {                               // all threads that share the step
+    if constexpr (kAlone) __syncthreads();
+    else cg::this_cluster().sync();
+  };
+  extern __shared__ int sm[];                        // pre[3][R + 1], kept [R], len [R]
+  __shared__ long long wsum[3][THREADS / 32];
   __shared__ int s_bad;
   int* pre_gone = sm;
   int* pre_need = sm + (a.R + 1);
   int* pre_tok = sm + 2 * (a.R + 1);
+  int* s_kept = sm + 3 * (a.R + 1);                  // pages the row keeps through the release
+  int* s_len = s_kept + a.R;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
-  if (tid < 3) carry[tid] = 0;
   if (tid == 0) s_bad = 0;
-  __syncthreads();
   const int count = *a.free_count;
-  for (int base = 0; base < a.R; base += kPagesThreads) {
-    const int r = base + tid;
-    long long v[3] = {0, 0, 0};
-    if (r < a.R) {
+  __syncthreads();
+  // a thread has `per` neighbouring rows, so that one scan over the block is enough
+  const int per = (a.R + THREADS - 1) / THREADS;
+  int g[PER], nd[PER], nw[PER];
+  long long sum[3] = {0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = tid * per + i;
+    g[i] = nd[i] = nw[i] = 0;
+    if (i < per && r < a.R) {
       const long long h = a.held[r], len = a.lens[r], n = a.fresh_tokens[r];
       const bool rs = a.reset && a.reset[r];
       const long long need = (len + n + a.page - 1) / a.page, kept = rs ? 0 : h;
       if (h < 0 || h > a.width || len < 0 || n < 0 || len + n > 0x7fffffffLL || need > a.width)
         s_bad = 1;
-      v[0] = rs ? h : 0;
-      v[1] = need > kept ? need - kept : 0;
-      v[2] = n;
+      g[i] = rs ? (int)h : 0;
+      nd[i] = need > kept ? (int)(need - kept) : 0;
+      nw[i] = (int)n;
+      s_kept[r] = (int)kept;
+      s_len[r] = (int)len;
+      sum[0] += g[i], sum[1] += nd[i], sum[2] += nw[i];
     }
-    long long inc[3];
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      inc[k] = warp_scan(v[k], lane);
-      if (lane == 31) wsum[k][warp] = inc[k];
-    }
-    __syncthreads();
-    if (warp == 0) {
-#pragma unroll
-      for (int k = 0; k < 3; ++k) {
-        const long long w = lane < kPagesThreads / 32 ? wsum[k][lane] : 0;
-        const long long i = warp_scan(w, lane), before = carry[k];
-        __syncwarp();                                // every lane has read the carry
-        if (lane < kPagesThreads / 32) wsum[k][lane] = before + i - w;
-        if (lane == 31) carry[k] = before + i;
-      }
-    }
-    __syncthreads();
-    // a sum past 32 bits is refused below, before any prefix is used
-    if (r < a.R) {
-      pre_gone[r] = (int)(wsum[0][warp] + inc[0] - v[0]);
-      pre_need[r] = (int)(wsum[1][warp] + inc[1] - v[1]);
-      pre_tok[r] = (int)(wsum[2][warp] + inc[2] - v[2]);
-    }
-    __syncthreads();
   }
-  const long long gone = carry[0], need = carry[1], tokens = carry[2];
+  long long inc[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    inc[k] = warp_scan(sum[k], lane);
+    if (lane == 31) wsum[k][warp] = inc[k];
+  }
+  __syncthreads();
+  long long total[3], base[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const long long w = warp_scan(lane < THREADS / 32 ? wsum[k][lane] : 0, lane);
+    total[k] = __shfl_sync(0xffffffffu, w, 31);
+    const long long before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+    base[k] = (warp ? before : 0) + inc[k] - sum[k];
+  }
+  const long long gone = total[0], need = total[1], tokens = total[2];
   int status = 0;
   if (s_bad || count < 0 || count + gone > a.capacity || tokens > a.max_tokens) status = -1;
   else if (need > count + gone) status = (int)(need - count - gone);
+  const bool ok = status == 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int r = tid * per + i;
+    if (i < per && r < a.R) {
+      pre_gone[r] = (int)base[0], pre_need[r] = (int)base[1], pre_tok[r] = (int)base[2];
+      base[0] += g[i], base[1] += nd[i], base[2] += nw[i];
+    }
+  }
   if (tid == 0) pre_gone[a.R] = (int)gone, pre_need[a.R] = (int)need, pre_tok[a.R] = (int)tokens;
   __syncthreads();
-  const bool ok = status == 0;
   const int top = ok ? count + (int)gone : 0;        // stack height between push and pop
-  const int gt = (int)cluster.block_rank() * kPagesThreads + tid;
-  const int gn = (int)cluster.num_blocks() * kPagesThreads;
+  const int gt = (int)blockIdx.x * THREADS + tid, gn = (int)gridDim.x * THREADS;
   if (ok)
     for (int j = gt; j < (int)gone; j += gn) {       // push: the first released page on top
-      const int r = row_of(pre_gone, a.R, j);
-      int32_t* e = a.table + r * a.table_rs + (j - pre_gone[r]);
+      int at[1] = {j}, r[1];
+      rows_of(pre_gone, a.R, at, r);
+      int32_t* e = a.table + r[0] * a.table_rs + (j - pre_gone[r[0]]);
       a.free_pages[top - 1 - j] = *e;
       *e = -1;
     }
-  cluster.sync();
+  everyone();
   if (ok)
     for (int j = gt; j < (int)need; j += gn) {       // pop into the rows' next columns
-      const int r = row_of(pre_need, a.R, j);
-      const int kept = (a.reset && a.reset[r]) ? 0 : a.held[r];
-      a.table[r * a.table_rs + kept + (j - pre_need[r])] = __ldcg(a.free_pages + top - 1 - j);
+      int at[1] = {j}, r[1];
+      rows_of(pre_need, a.R, at, r);
+      a.table[r[0] * a.table_rs + s_kept[r[0]] + (j - pre_need[r[0]])] = __ldcg(a.free_pages + top - 1 - j);
     }
-  for (int64_t t = gt; t < a.max_tokens; t += gn) {
-    int64_t slot = -1;
-    int pos = 0;
-    if (ok && t < tokens) {
-      const int r = row_of(pre_tok, a.R, (int)t);
-      const int kept = (a.reset && a.reset[r]) ? 0 : a.held[r];
-      pos = a.lens[r] + ((int)t - pre_tok[r]);
-      const int col = pos / a.page;
-      const int pg = col < kept ? a.table[r * a.table_rs + col]
-                                : __ldcg(a.free_pages + top - 1 - (pre_need[r] + col - kept));
-      slot = pg < 0 ? -1 : (int64_t)pg * a.page + (pos - col * a.page);
+  constexpr int N = 4;
+  for (int64_t t0 = gt; t0 < a.max_tokens; t0 += (int64_t)N * gn) {
+    int at[N], r[N], pos[N], pg[N], col[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) at[n] = (int)min((long long)t0 + (long long)n * gn, ok && tokens ? tokens - 1 : 0LL);
+    if (ok && tokens) {
+      rows_of(pre_tok, a.R, at, r);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        pos[n] = s_len[r[n]] + (at[n] - pre_tok[r[n]]);
+        col[n] = pos[n] / a.page;
+        const int kept = s_kept[r[n]];
+        pg[n] = col[n] < kept ? a.table[r[n] * a.table_rs + col[n]]
+                              : __ldcg(a.free_pages + top - 1 - (pre_need[r[n]] + col[n] - kept));
+      }
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t t = t0 + (int64_t)n * gn;
+      if (t >= a.max_tokens) continue;
+      const bool live = ok && t < tokens;
+      a.slots[t] = live && pg[n] >= 0 ? (int64_t)pg[n] * a.page + (pos[n] - col[n] * a.page) : -1;
+      a.positions[t] = live ? pos[n] : 0;
+    }
   }
   for (int r = gt; r <= a.R; r += gn) {
     a.cu_q[r] = ok ? pre_tok[r] : 0;
-    if (r < a.R) a.new_lens[r] = a.lens[r] + (ok ? a.fresh_tokens[r] : 0);
+    if (r < a.R) a.new_lens[r] = s_len[r] + (ok ? pre_tok[r + 1] - pre_tok[r] : 0);
   }
-  cluster.sync();                                    // every reader of held and the stack is done
+  everyone();                                    // every reader of the stack and the state is done
   if (ok) {
-    for (int r = gt; r < a.R; r += gn) {
-      const int kept = (a.reset && a.reset[r]) ? 0 : a.held[r];
-      a.held[r] = kept + (pre_need[r + 1] - pre_need[r]);
-    }
+    for (int r = gt; r < a.R; r += gn) a.held[r] = s_kept[r] + (pre_need[r + 1] - pre_need[r]);
     for (int j = gt; j < (int)need; j += gn) a.free_pages[top - 1 - j] = -1;
   }
   if (gt == 0) {
@@ -330,8 +395,14 @@ cudaError_t dispatch(int D, int group, F&& f) {
   return cudaErrorInvalidValue;
 }
 
-bool vec8(const void* p, int64_t ts, int64_t hs) {
-  return (reinterpret_cast<uintptr_t>(p) & 7) == 0 && ts % 4 == 0 && hs % 4 == 0;
+int log2_of(int n) {
+  int b = 0;
+  while ((1 << b) < n) ++b;
+  return b;
+}
+
+bool vec16(const void* p, int64_t ts, int64_t hs) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ts % 8 == 0 && hs % 8 == 0;
 }
 
 }  // namespace
@@ -344,14 +415,14 @@ cudaError_t launch_kv4_append(const Kv4Shape& c, const void* k, int64_t k_ts, in
   a.k = static_cast<const __half*>(k), a.v = static_cast<const __half*>(v);
   a.k_ts = k_ts, a.k_hs = k_hs, a.v_ts = v_ts, a.v_hs = v_hs;
   a.slots = slots, a.cache = static_cast<uint8_t*>(cache);
-  a.T = T, a.capacity = c.num_pages * c.page, a.H = c.heads, a.page = c.page;
+  a.T = T, a.capacity = c.num_pages * c.page, a.H = c.heads, a.page_shift = log2_of(c.page);
   a.status = dev_status;
-  const int vk = vec8(k, k_ts, k_hs), vv = vec8(v, v_ts, v_hs);
+  const int vk = vec16(k, k_ts, k_hs), vv = vec16(v, v_ts, v_hs);
   return dispatch(c.dim, c.group, [&](auto d, auto g) {
-    constexpr int kRows = 32 / (d.value / 4) * 8;    // (token, head) rows per block
-    int64_t blocks = (T * c.heads + kRows - 1) / kRows;
-    if (blocks > (int64_t)num_sms * 32) blocks = (int64_t)num_sms * 32;
-    kv4_append_kernel<d.value, g.value><<<(unsigned)blocks, 256, 0, stream>>>(a, vk, vv);
+    constexpr int kTokens = 32 / (d.value / 8) * 8;  // of a block
+    int64_t blocks = (T + kTokens - 1) / kTokens;
+    if (blocks > (int64_t)num_sms * 64) blocks = (int64_t)num_sms * 64;
+    kv4_append_kernel<d.value, g.value><<<dim3((unsigned)blocks, c.heads), 256, 0, stream>>>(a, vk, vv);
     return cudaGetLastError();
   });
 }
@@ -362,12 +433,13 @@ cudaError_t launch_kv4_gather(const Kv4Shape& c, const void* cache, const int64_
   Kv4IoArgs a = {};
   a.slots = slots, a.cache = static_cast<uint8_t*>(const_cast<void*>(cache));
   a.out_k = static_cast<__half*>(out_k), a.out_v = static_cast<__half*>(out_v);
-  a.T = T, a.capacity = c.num_pages * c.page, a.H = c.heads, a.page = c.page;
+  a.T = T, a.capacity = c.num_pages * c.page, a.H = c.heads, a.page_shift = log2_of(c.page);
   a.status = dev_status;
   return dispatch(c.dim, c.group, [&](auto d, auto g) {
-    int64_t blocks = (T * c.heads * (d.value / 4) + 255) / 256;
-    if (blocks > (int64_t)num_sms * 32) blocks = (int64_t)num_sms * 32;
-    kv4_gather_kernel<d.value, g.value><<<(unsigned)blocks, 256, 0, stream>>>(a);
+    constexpr int kTokens = 256 / (d.value / 8);
+    int64_t blocks = (T + kTokens - 1) / kTokens;
+    if (blocks > (int64_t)num_sms * 64) blocks = (int64_t)num_sms * 64;
+    kv4_gather_kernel<d.value, g.value><<<dim3((unsigned)blocks, c.heads), 256, 0, stream>>>(a);
     return cudaGetLastError();
   });
 }
@@ -380,25 +452,31 @@ cudaError_t launch_kv4_pages(const Kv4PagesCall& c, cudaStream_t stream) {
   a.slots = c.slots, a.positions = c.positions, a.cu_q = c.cu_q, a.new_lens = c.new_lens;
   a.status = c.status, a.max_tokens = c.max_tokens;
   a.R = c.rows, a.width = c.width, a.capacity = c.capacity, a.page = c.page;
-  const size_t smem = 3 * (size_t)(c.rows + 1) * sizeof(int);
+  const size_t smem = (3 * (size_t)(c.rows + 1) + 2 * (size_t)c.rows) * sizeof(int);
+  // One small CTA where its threads have a row and a few tokens each at most: a decode step of
+  // 64 requests of which three are replaced takes 7 us on it, 10 us on 1024 threads.
+  if (c.rows <= kPagesFew && c.max_tokens <= 4 * kPagesFew) {
+    kv4_pages_kernel<kPagesFew, 1><<<1, kPagesFew, smem, stream>>>(a);
+    return cudaGetLastError();
+  }
   static PerDeviceOnce attr_once;
   const cudaError_t attr = attr_once.run([] {
-    return cudaFuncSetAttribute(kv4_pages_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                3 * (kKv4MaxRows + 1) * (int)sizeof(int));
+    return cudaFuncSetAttribute(kv4_pages_kernel<kPagesThreads, kKv4MaxRows / kPagesThreads>,
+                                cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                (5 * kKv4MaxRows + 3) * (int)sizeof(int));
   });
   if (attr != cudaSuccess) return attr;
   cudaLaunchConfig_t cfg = {};
-  const int ctas = c.rows <= kPagesThreads && c.max_tokens <= 4 * kPagesThreads ? 1 : 8;
-  cfg.gridDim = dim3(ctas, 1, 1);
+  cfg.gridDim = dim3(8, 1, 1);
   cfg.blockDim = dim3(kPagesThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = ctas, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  at[0].val.clusterDim.x = 8, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_pages_kernel, a);
+  return cudaLaunchKernelEx(&cfg, kv4_pages_kernel<kPagesThreads, kKv4MaxRows / kPagesThreads>, a);
 }
 
 }  // namespace awq

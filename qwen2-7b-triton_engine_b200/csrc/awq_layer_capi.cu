@@ -37,7 +37,7 @@ int check_shape(int64_t num_pages, int64_t kv_heads, int64_t head_dim, int64_t g
   if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
     return fail(AWQ_ERR_UNSUPPORTED, "page_size=%lld must be a power of two from 16 to 1024",
                 (long long)page_size);
-  if (num_pages < 1 || num_pages > 0x7fffffffLL || kv_heads < 1 || kv_heads > 65536)
+  if (num_pages < 1 || num_pages > 0x7fffffffLL || kv_heads < 1 || kv_heads > 4096)
     return fail(AWQ_ERR_INVALID_ARG, "num_pages=%lld or kv_heads=%lld out of range",
                 (long long)num_pages, (long long)kv_heads);
   c->num_pages = num_pages;

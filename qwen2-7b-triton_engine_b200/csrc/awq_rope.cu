@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kRopeThreads = 256;
 constexpr int kRopeMaxHalf = 256;
+constexpr int kTokens = 4;             // of a block
 
 __device__ __forceinline__ int axis_of(const RopeCall& c, int i) {
   if (c.interleaved) {
@@ -32,54 +33,94 @@ __device__ __forceinline__ int axis_of(const RopeCall& c, int i) {
   return a;
 }
 
+// Where piece idx of a head lies: 8 pairs of channels (VEC) or one, from channel i of head h.
+struct Piece {
+  const __half* x;
+  __half* y;
+  int64_t xs, ys;      // token strides
+  int i;
+};
+template <bool VEC>
+__device__ __forceinline__ Piece piece(const RopeCall& c, int idx, int per) {
+  Piece p;
+  const int h = idx / per;
+  p.i = (idx - h * per) * (VEC ? 8 : 1);
+  const bool isq = h < c.q_heads;
+  const int hk = h - c.q_heads;
+  p.x = isq ? static_cast<const __half*>(c.q) + h * c.q_hs : static_cast<const __half*>(c.k) + hk * c.k_hs;
+  p.y = isq ? static_cast<__half*>(c.out_q) + h * c.oq_hs : static_cast<__half*>(c.out_k) + hk * c.ok_hs;
+  p.xs = isq ? c.q_ts : c.k_ts, p.ys = isq ? c.oq_ts : c.ok_ts;
+  return p;
+}
+
+// A block turns kTokens neighbouring tokens.  The loads of a thread's first piece are under way
+// while the block makes the tokens' sines and cosines.
 template <bool VEC>
 __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeCall c) {
-  __shared__ float s_cos[kRopeMaxHalf], s_sin[kRopeMaxHalf];
-  const int heads = c.q_heads + c.k_heads;
-  for (int64_t t = blockIdx.x; t < c.T; t += gridDim.x) {
-    for (int i = threadIdx.x; i < c.half; i += kRopeThreads) {
-      const int64_t at = axis_of(c, i) * c.pos_as + t;
-      const double pos = c.pos_is_64 ? (double)static_cast<const int64_t*>(c.positions)[at]
-                                     : (double)static_cast<const int32_t*>(c.positions)[at];
-      const double turns = pos * ((double)c.inv_freq[i] * 0.15915494309189533577);
-      sincospif((float)(2.0 * (turns - rint(turns))), &s_sin[i], &s_cos[i]);
-    }
-    __syncthreads();
-    const int per = VEC ? c.half / 8 : c.half;
-    for (int idx = threadIdx.x; idx < heads * per; idx += kRopeThreads) {
-      const int h = idx / per, i = (idx - h * per) * (VEC ? 8 : 1);
-      const bool isq = h < c.q_heads;
-      const __half* x = isq ? static_cast<const __half*>(c.q) + t * c.q_ts + h * c.q_hs
-                            : static_cast<const __half*>(c.k) + t * c.k_ts + (h - c.q_heads) * c.k_hs;
-      __half* y = isq ? static_cast<__half*>(c.out_q) + t * c.oq_ts + h * c.oq_hs
-                      : static_cast<__half*>(c.out_k) + t * c.ok_ts + (h - c.q_heads) * c.ok_hs;
-      if constexpr (VEC) {
-        const uint4 va = *reinterpret_cast<const uint4*>(x + i);
-        const uint4 vb = *reinterpret_cast<const uint4*>(x + i + c.half);
-        uint4 oa, ob;
-        const __half2* a = reinterpret_cast<const __half2*>(&va);
-        const __half2* b = reinterpret_cast<const __half2*>(&vb);
-        __half2* ya = reinterpret_cast<__half2*>(&oa);
-        __half2* yb = reinterpret_cast<__half2*>(&ob);
+  __shared__ __align__(16) float s_cos[kTokens][kRopeMaxHalf], s_sin[kTokens][kRopeMaxHalf];
+  const int heads = c.q_heads + c.k_heads, rest = c.dim - 2 * c.half;
+  const int per = VEC ? c.half / 8 : c.half, pieces = heads * per;
+  const int64_t t0 = (int64_t)blockIdx.x * kTokens;
+  const int tokens = (int)(c.T - t0 < kTokens ? c.T - t0 : kTokens);
+  Piece p = {};
+  uint4 va[kTokens], vb[kTokens];
+  auto fetch = [&](int idx) {
+    p = piece<VEC>(c, idx, per);
+    if constexpr (VEC) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 fa = __half22float2(a[j]), fb = __half22float2(b[j]);
-          const float c0 = s_cos[i + 2 * j], c1 = s_cos[i + 2 * j + 1];
-          const float s0 = s_sin[i + 2 * j], s1 = s_sin[i + 2 * j + 1];
-          ya[j] = __floats2half2_rn(fa.x * c0 - fb.x * s0, fa.y * c1 - fb.y * s1);
-          yb[j] = __floats2half2_rn(fb.x * c0 + fa.x * s0, fb.y * c1 + fa.y * s1);
+      for (int k = 0; k < kTokens; ++k)
+        if (k < tokens) {
+          const __half* x = p.x + (t0 + k) * p.xs + p.i;
+          va[k] = *reinterpret_cast<const uint4*>(x);
+          vb[k] = *reinterpret_cast<const uint4*>(x + c.half);
         }
-        *reinterpret_cast<uint4*>(y + i) = oa;
-        *reinterpret_cast<uint4*>(y + i + c.half) = ob;
+    }
+  };
+  if ((int)threadIdx.x < pieces) fetch(threadIdx.x);
+  for (int n = threadIdx.x; n < tokens * c.half; n += kRopeThreads) {
+    const int k = n / c.half, i = n - k * c.half;
+    const int64_t at = axis_of(c, i) * c.pos_as + t0 + k;
+    const double pos = c.pos_is_64 ? (double)static_cast<const int64_t*>(c.positions)[at]
+                                   : (double)static_cast<const int32_t*>(c.positions)[at];
+    const double turns = pos * ((double)c.inv_freq[i] * 0.15915494309189533577);
+    sincospif((float)(2.0 * (turns - rint(turns))), &s_sin[k][i], &s_cos[k][i]);
+  }
+  __syncthreads();
+  for (int idx = threadIdx.x; idx < pieces; idx += kRopeThreads) {
+    if (idx != (int)threadIdx.x) fetch(idx);
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      if (k >= tokens) break;
+      const float *cs = s_cos[k] + p.i, *sn = s_sin[k] + p.i;
+      __half* y = p.y + (t0 + k) * p.ys + p.i;
+      if constexpr (VEC) {
+        const uint32_t a[4] = {va[k].x, va[k].y, va[k].z, va[k].w}, b[4] = {vb[k].x, vb[k].y, vb[k].z, vb[k].w};
+        uint32_t ya[4], yb[4];
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const float4 c4 = *reinterpret_cast<const float4*>(cs + 2 * j);
+          const float4 s4 = *reinterpret_cast<const float4*>(sn + 2 * j);
+          const float2 a0 = __half22float2(u32_as_h2(a[j])), a1 = __half22float2(u32_as_h2(a[j + 1]));
+          const float2 b0 = __half22float2(u32_as_h2(b[j])), b1 = __half22float2(u32_as_h2(b[j + 1]));
+          ya[j] = h2_as_u32(__floats2half2_rn(a0.x * c4.x - b0.x * s4.x, a0.y * c4.y - b0.y * s4.y));
+          yb[j] = h2_as_u32(__floats2half2_rn(b0.x * c4.x + a0.x * s4.x, b0.y * c4.y + a0.y * s4.y));
+          ya[j + 1] = h2_as_u32(__floats2half2_rn(a1.x * c4.z - b1.x * s4.z, a1.y * c4.w - b1.y * s4.w));
+          yb[j + 1] = h2_as_u32(__floats2half2_rn(b1.x * c4.z + a1.x * s4.z, b1.y * c4.w + a1.y * s4.w));
+        }
+        *reinterpret_cast<uint4*>(y) = make_uint4(ya[0], ya[1], ya[2], ya[3]);
+        *reinterpret_cast<uint4*>(y + c.half) = make_uint4(yb[0], yb[1], yb[2], yb[3]);
       } else {
-        const float fa = __half2float(x[i]), fb = __half2float(x[i + c.half]);
-        y[i] = __float2half_rn(fa * s_cos[i] - fb * s_sin[i]);
-        y[i + c.half] = __float2half_rn(fb * s_cos[i] + fa * s_sin[i]);
+        const __half* x = p.x + (t0 + k) * p.xs + p.i;
+        const float fa = __half2float(x[0]), fb = __half2float(x[c.half]);
+        y[0] = __float2half_rn(fa * cs[0] - fb * sn[0]);
+        y[c.half] = __float2half_rn(fb * cs[0] + fa * sn[0]);
       }
     }
-    const int rest = c.dim - 2 * c.half;
-    for (int idx = threadIdx.x; idx < heads * rest; idx += kRopeThreads) {
-      const int h = idx / rest, i = 2 * c.half + idx - h * rest;
+  }
+  if (rest > 0)
+    for (int idx = threadIdx.x; idx < tokens * heads * rest; idx += kRopeThreads) {
+      const int k = idx / (heads * rest), at = idx - k * heads * rest, h = at / rest;
+      const int64_t t = t0 + k, i = 2 * c.half + at - h * rest;
       if (h < c.q_heads)
         static_cast<__half*>(c.out_q)[t * c.oq_ts + h * c.oq_hs + i] =
             static_cast<const __half*>(c.q)[t * c.q_ts + h * c.q_hs + i];
@@ -87,8 +128,6 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeCall c) {
         static_cast<__half*>(c.out_k)[t * c.ok_ts + (h - c.q_heads) * c.ok_hs + i] =
             static_cast<const __half*>(c.k)[t * c.k_ts + (h - c.q_heads) * c.k_hs + i];
     }
-    __syncthreads();
-  }
 }
 
 bool vec16(const void* p, int64_t ts, int64_t hs) {
@@ -100,8 +139,7 @@ bool vec16(const void* p, int64_t ts, int64_t hs) {
 cudaError_t launch_rope(const RopeCall& c, int num_sms, cudaStream_t stream) {
   const bool q_ok = c.q_heads == 0 || (vec16(c.q, c.q_ts, c.q_hs) && vec16(c.out_q, c.oq_ts, c.oq_hs));
   const bool k_ok = c.k_heads == 0 || (vec16(c.k, c.k_ts, c.k_hs) && vec16(c.out_k, c.ok_ts, c.ok_hs));
-  const int64_t most = (int64_t)num_sms * 64;
-  const unsigned blocks = (unsigned)(c.T < most ? c.T : most);
+  const unsigned blocks = (unsigned)((c.T + kTokens - 1) / kTokens);
   if (c.half % 8 == 0 && q_ok && k_ok)
     rope_kernel<true><<<blocks, kRopeThreads, 0, stream>>>(c);
   else
