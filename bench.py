@@ -40,7 +40,8 @@ the ranks by the library's all-reduce over NVLink peer memory (decode: fused int
 product kernel; prefill: a separate all-reduce kernel after the product), else NCCL
 (strong scaling: the token's total bytes are fixed).
 ``--impl reference`` times the reference's own CPU path (oracle port) instead.
-``--stack`` runs only the config-5 leg (see stack_bench).
+``--stack`` runs only the config-5 leg (see stack_bench); with ``--attention`` the layers
+attend over a paged 4-bit key/value cache instead of passing the query columns on.
 """
 from __future__ import annotations
 
@@ -762,7 +763,10 @@ def stack_bench(torch, awq_b200, dev, world, rank, comm, args):
     calls stand where the reference has two kernels: the q/k/v bias in the product
     (model/qwen2.py:108-109) and SiLU-mul with the gate+up product (:181-194).  Attention
     itself is not part of the linear stack: o reads the rank's query columns of q/k/v in
-    its place."""
+    its place.  With ``--attention`` it is: rotary positions, a paged 4-bit cache with its
+    page bookkeeping (one call per step) and attention over it
+    (``AttentionLinearsTP.attend``), and the residual adds move into the epilogues of o and
+    down."""
     from awq_b200 import tp
     gen = torch.Generator(device=dev).manual_seed(4321)     # the same full weights everywhere
     eps = 1e-6
@@ -791,8 +795,37 @@ def stack_bench(torch, awq_b200, dev, world, rank, comm, args):
             h = h + mlp(rms(h, n2))
         return h
 
+    if args.attention:
+        page = 64
+        blocks = -(-(args.prefill + args.decode + 8) // page)
+        g0, g1 = layers[0][0].shard.kv_heads
+        caches = [awq_b200.KV4Cache.allocate(blocks, g1 - g0, 128, page, device=dev) for _ in layers]
+        i32 = dict(dtype=torch.int32, device=dev)
+        table = torch.full((1, blocks), -1, **i32)
+        held, kv_lens = torch.zeros(1, **i32), torch.zeros(1, **i32)
+        free, count = torch.arange(blocks, **i32), torch.full((1,), blocks, **i32)
+        inv_freq = (1e6 ** (-torch.arange(64, dtype=torch.float64, device=dev) / 64)).float()
+
+        def forward(h):                                     # noqa: F811
+            T = h.shape[0]
+            slots, pos, cu, lens, _ = awq_b200.kv4_pages_step(
+                table, held, free, count, kv_lens, torch.full((1,), T, **i32), page, T)
+            for (attn, mlp, n1, n2), cache in zip(layers, caches):
+                h = attn.attend(rms(h, n1), cache, slots, table, lens, pos, inv_freq, (64,),
+                                cu_q=cu if T > 1 else None, max_q=T, residual=h)
+                h = mlp(rms(h, n2), residual=h)
+            kv_lens.copy_(lens)
+            return h
+
     x = (torch.randn((args.prefill, HIDDEN), device=dev, generator=gen) * 0.1).half()
-    prefill_ms = _dev_time_ms(torch, dev, world, lambda: forward(x), 1, False)
+    if args.attention:                                      # each timed prefill starts empty
+        def prefill():
+            kv_lens.zero_()
+            return forward(x)
+    else:
+        def prefill():
+            return forward(x)
+    prefill_ms = _dev_time_ms(torch, dev, world, prefill, 1, False)
     tok = (torch.randn((1, HIDDEN), device=dev, generator=gen) * 0.1).half()
     s = torch.cuda.Stream(device=dev)
     s.wait_stream(torch.cuda.current_stream(dev))
@@ -826,7 +859,10 @@ def stack_bench(torch, awq_b200, dev, world, rank, comm, args):
             "decode_steps": args.decode, "decode_ms_per_token": round(decode_ms, 4),
             "decode_tokens_per_s": round(1e3 / decode_ms, 1),
             "decode_weight_TBps": round(w_bytes / (decode_ms * 1e-3) / 1e12, 4),
-            "between_layers": "torch RMSNorm and residual adds; q/k/v bias and SiLU-mul fused",
+            "between_layers": "torch RMSNorm; q/k/v bias, SiLU-mul and residual adds fused; rotary "
+                              "positions, 4-bit paged cache and attention over it"
+                              if args.attention else
+                              "torch RMSNorm and residual adds; q/k/v bias and SiLU-mul fused",
             "device_status": st, "data": "synthetic (random int4 AWQ weights, no checkpoint)"}
 
 
@@ -868,6 +904,8 @@ def main():
     ap.add_argument("--cpu-seconds", type=float, default=12.0)
     ap.add_argument("--stack", action="store_true",
                     help="config 5: prefill + decode through the 28-layer linear stack (1 GPU)")
+    ap.add_argument("--attention", action="store_true",
+                    help="with --stack: attention over a paged 4-bit key/value cache in every layer")
     ap.add_argument("--prefill", type=int, default=1024)
     ap.add_argument("--decode", type=int, default=512)
     args = ap.parse_args()

@@ -16,7 +16,8 @@ AWQ drop-in, in the packed layout the reference registers (model/qwen2.py:34-36)
 * attention by whole heads (``AttentionLinearsTP``): the fused q/k/v columns of the
   rank's query heads and of the key/value heads they read under grouped-query attention
   (model/qwen2.py:131-138), and o's rows of the same query heads, so attention itself
-  runs per rank with no exchange until o's all-reduce.
+  runs per rank with no exchange until o's all-reduce.  ``attend`` is the whole block over
+  a paged 4-bit cache of the rank's heads (awq_b200.layer).
 
 The product runs through ``kernels.awq_gemm.awq_gemm_forward`` (the sm_100a
 library); ``gemm=`` lets host-logic tests substitute a CPU function under ``gloo``.
@@ -42,6 +43,12 @@ def _default_gemm_bias():
     """The library product with the bias added in its epilogue (one kernel)."""
     from kernels.awq_gemm import awq_gemm_bias_forward
     return awq_gemm_bias_forward
+
+
+def _default_epilogue():
+    """The library's product with bias and residual added in its epilogue."""
+    from kernels.awq_gemm import awq_gemm_epilogue_forward
+    return awq_gemm_epilogue_forward
 
 
 def _default_silu_mul():
@@ -190,6 +197,8 @@ class RowParallelAWQ:
             dist.all_gather_object(ks, self.k1 - self.k0, group=group)
             self.k_all = [int(k) for k in ks]
         self._fused_ok: dict = {}
+        # on one GPU the library adds the residual (and the bias) in the product's epilogue
+        self.epilogue = _default_epilogue() if gemm is None and world == 1 else None
 
     def fused_for(self, M: int) -> bool:
         """Whether a call with M activation rows runs the library's all-reduce (the same
@@ -227,8 +236,17 @@ class RowParallelAWQ:
         out = out.view(*x_local.shape[:-1], N)
         return out + self.bias if self.bias is not None else out
 
-    def __call__(self, x_local: torch.Tensor) -> torch.Tensor:
-        """x_local holds this rank's K columns [k0, k1) of the activation."""
+    def __call__(self, x_local: torch.Tensor,
+                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x_local holds this rank's K columns [k0, k1) of the activation.  ``residual`` (the
+        full output's shape, the same on every rank) is added to the sum: in the product's
+        epilogue on one GPU, after the all-reduce on several."""
+        if residual is not None:
+            if self.epilogue is not None and self.k1 > self.k0:
+                w = self.w
+                return self.epilogue(x_local, w.qweight, w.qzeros, w.scales, w.group_size,
+                                     bias=w.bias, residual=residual)
+            return self(x_local) + residual
         fused = self._fused(x_local)
         if fused is not None:
             return fused
@@ -313,7 +331,8 @@ class AttentionLinearsTP:
     (the reference runs them on one GPU, model/qwen2.py:81-113,156): the fused q/k/v
     projection column-parallel over the rank's query heads plus the key/value heads they
     use, and o row-parallel over the same query heads' rows, followed by the all-reduce.
-    Attention itself (RoPE, cache, softmax) runs on the rank's heads in between."""
+    Attention itself (RoPE, cache, softmax) runs on the rank's heads in between; ``attend``
+    is the whole block with the library's own operators."""
 
     def __init__(self, qkv: AWQWeights, o: AWQWeights, num_heads: int, num_kv_heads: int,
                  head_dim: int, world: int, rank: int, group: Optional[object] = None,
@@ -322,6 +341,7 @@ class AttentionLinearsTP:
             raise ValueError("o must have K == num_heads * head_dim")
         self.shard = shard_qkv_by_heads(qkv, num_heads, num_kv_heads, head_dim, world, rank)
         h0, h1 = self.shard.q_heads
+        self.head_group = num_heads // num_kv_heads
         self.gemm = gemm or _default_gemm()
         self.gemm_bias = _default_gemm_bias() if gemm is None else None
         self.o = RowParallelAWQ(o, world, rank, group=group, gemm=gemm, comm=comm,
@@ -336,6 +356,35 @@ class AttentionLinearsTP:
     def project_o(self, attn_local: torch.Tensor) -> torch.Tensor:
         """o of the rank's heads' attention output [..., q_size], summed over the ranks."""
         return self.o(attn_local)
+
+    def attend(self, x: torch.Tensor, cache, slots: torch.Tensor, block_table: torch.Tensor,
+               kv_lens: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections,
+               cu_q: Optional[torch.Tensor] = None, max_q: int = 1, interleaved: bool = False,
+               residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The attention block of one layer for the step's new tokens x [T, hidden]: q/k/v
+        product, rotary positions (in place on its output), keys and values quantized into
+        ``cache`` (an ``awq_b200.KV4Cache`` of this rank's kv heads), attention over it, o
+        product, plus ``residual`` [T, hidden].  slots, positions, cu_q and kv_lens are
+        ``awq_b200.kv4_pages_step``'s (new_lens); without cu_q every request has one token.
+        Tokens behind cu_q's last one have slot -1 and give ``residual`` plus o's bias."""
+        import awq_b200
+        s = self.shard
+        (h0, h1), (g0, g1) = s.q_heads, s.kv_heads
+        if h1 - h0 != (g1 - g0) * self.head_group:
+            raise ValueError(f"this rank's query heads [{h0}, {h1}) are not whole groups of "
+                             f"{self.head_group}: attention needs a world size that divides the "
+                             "kv heads")
+        if cache.kv_heads != g1 - g0 or cache.head_dim != s.head_dim:
+            raise ValueError(f"the cache holds {cache.kv_heads} heads of {cache.head_dim}, this "
+                             f"rank has {g1 - g0} of {s.head_dim}")
+        if x.dim() != 2:
+            raise ValueError(f"x must be [tokens, hidden], got {tuple(x.shape)}")
+        T = x.shape[0]
+        q, k, v = (t.unflatten(-1, (-1, s.head_dim)) for t in self.project_qkv(x))
+        awq_b200.rope_axes(q, k, positions, inv_freq, sections, interleaved, out_q=q, out_k=k)
+        awq_b200.kv4_append(k, v, slots, cache)
+        attn = awq_b200.kv4_attention(q, cache, block_table, kv_lens, cu_q, max_q)
+        return self.o(attn.view(T, -1), residual)
 
 
 class TensorParallelMLP:
@@ -365,12 +414,13 @@ class TensorParallelMLP:
         # (host-logic tests) goes through the slices below
         self.silu_mul = _default_silu_mul() if gemm is None and gate_up.bias is None else None
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The block's output, plus ``residual`` when given (see RowParallelAWQ)."""
         if self.silu_mul is not None and self.inter_local > 0:
             w = self.gate_up.w
             h = self.silu_mul(x, w.qweight, w.qzeros, w.scales, w.group_size)
-            return self.down(h)
+            return self.down(h, residual)
         gu = self.gate_up(x)
         gate, up = gu[..., :self.inter_local], gu[..., self.inter_local:]
         h = (F.silu(gate.float()) * up.float()).to(torch.float16)
-        return self.down(h)
+        return self.down(h, residual)
