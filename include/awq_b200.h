@@ -239,7 +239,8 @@ AWQ_API int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64
  * gives zeros.  Rows of out behind cu_q[requests] are left as they are.  max_q: most query
  * rows of a request (a hint for the choice of kernel).  Tokens in a page outside
  * 0 .. num_pages - 1 are not seen, kv_lens is clipped to the table, a request whose cu_q is
- * not ascending within 0 .. tokens is left out; each sets status bit 2.  The workspace
+ * not ascending within 0 .. tokens is left out, and where requests claim the same rows so often
+ * that the list of work passes 2^31 nothing is computed; each sets status bit 2.  The workspace
  * (awq_kv4_attention_workspace_bytes with max_rows = min(max_q, tokens) * q_heads / kv_heads,
  * 16-byte aligned) needs no initialisation; calls that may overlap on the GPU need different
  * ones.

@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include "awq_common.cuh"
+
 namespace awq {
 namespace kv4 {
 
@@ -29,6 +31,51 @@ struct AttnArgs {
   int R, width, page_shift, kv_heads, G;
   int min_rows;       // requests with this many query rows per kv head are the prefill kernel's
 };
+
+// Requests of one entry of the prefix sums: 1 << shift.
+__device__ __forceinline__ int prefix_shift(const AttnArgs& a) {
+  int shift = 0;
+  while ((a.R >> shift) + 1 > kPrefixEntries) ++shift;
+  return shift;
+}
+// Prefix sums pre[] of the requests' units of work (units(r), below 2^31), and their total.
+// All THREADS threads call it.
+template <int THREADS, class F>
+__device__ __forceinline__ int scan_units(const AttnArgs& a, int* pre, F units) {
+  constexpr int WARPS = THREADS / 32;
+  static_assert(kPrefixEntries <= 1 << 10, "entries below 2^21 units do not overflow");
+  __shared__ int wsum[WARPS];
+  __shared__ int s_total, s_high;                        // high: entries of 2^21 and more, / 2^16
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
+  const int shift = prefix_shift(a), entries = (a.R + (1 << shift) - 1) >> shift;
+  if (tid == 0) s_total = s_high = 0;
+  for (int e0 = 0; e0 < entries; e0 += THREADS) {
+    const int e = e0 + tid;
+    uint32_t v = 0;
+    if (e < entries)
+      for (int r = e << shift; r < min(a.R, (e + 1) << shift); ++r)
+        v = min(v + (uint32_t)units(r), 0x7fffffffu);
+    int inc = (int)v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int nb = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += nb;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    if (__syncthreads_or(v >= 1u << 21)) atomicAdd(&s_high, (int)(v >> 16));
+    const int part = lane < WARPS ? wsum[lane] : 0;
+    const int before = s_total + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
+    if (e < entries) pre[e] = before + inc - (int)v;
+    const int all = __reduce_add_sync(0xffffffffu, part);
+    __syncthreads();
+    if (tid == 0) s_total += all;
+    __syncthreads();
+  }
+  // a list of 2^31 or more (requests that claim the same query rows): nothing is computed
+  if (s_high <= 32767 && s_total >= 0) return s_total;
+  if (tid == 0) atomicOr(a.status, kDevErrShape);
+  return 0;
+}
 
 }  // namespace kv4
 }  // namespace awq

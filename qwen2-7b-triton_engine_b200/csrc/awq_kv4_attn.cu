@@ -18,13 +18,13 @@
 // rows of a kv head its 8 columns), as are the outputs (channels x query rows), so seven
 // query heads of a group waste one column in eight instead of nine rows in sixteen.
 //
-// Work split (kv4_attn_kernel): the (request, kv head, 8 NT query rows) items are cut into
-// tiles of 64 tokens, and the linear list of all tiles is dealt evenly to all warps of one
-// CTA per SM; ragged batches balance to within a tile.  Every item has one empty tile more,
-// which stands for its fixed cost.  A warp reads its tiles from a ring of its own; one more
-// warp fills all rings with bulk copies, each of its lanes one (no CTA barrier in the loop).  Items that cross warps are
-// joined in the CTA at its end; items that cross CTAs by kv4_merge_kernel, in CTA order, so
-// results do not depend on timing.
+// Work split (kv4_attn_kernel): the (request, kv head, 8 query rows) items are cut into tiles
+// of 64 tokens, and the linear list of all tiles is dealt evenly to all warps of one CTA per
+// SM; ragged batches balance to within a tile.  Every item has one empty tile more, which
+// stands for its fixed cost.  A warp reads its tiles from a ring of its own; one more warp
+// fills all rings with bulk copies, each of its lanes one (no CTA barrier in the loop).  Items
+// that cross warps are joined in the CTA at its end; items that cross CTAs by
+// kv4_merge_kernel, in CTA order, so results do not depend on timing.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -97,12 +97,14 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-template <int D_, int GROUP_, int NT_, int TB_, int WARPS_>
+constexpr int kRows = 8;                               // query rows of an item
+
+template <int D_, int GROUP_, int TB_, int WARPS_>
 struct Geo {
   static constexpr int TB = TB_, TOKENS = 16 * TB_;    // blocks and tokens of a tile
-  static constexpr int D = D_, GROUP = GROUP_, NT = NT_, WARPS = WARPS_;
+  static constexpr int D = D_, GROUP = GROUP_, WARPS = WARPS_;
   static constexpr int THREADS = (WARPS + 1) * 32;     // and the producer warp
-  static constexpr int NG = D / GROUP, W = D / 32, ROWS = 8 * NT;
+  static constexpr int NG = D / GROUP, W = D / 32, ROWS = kRows;
   static constexpr int BLK = kv4::block_bytes(D, GROUP), TILE = TB * BLK;
   static constexpr int BUDGET = 227 * 1024 - (kPrefixEntries + 8) * 4 - 5120;
   static constexpr int FIT = BUDGET / (WARPS * TILE);
@@ -161,8 +163,9 @@ struct Cursor {
     vis = max(0, x.L - x.n + last + 1);
   }
   template <class G_>
-  __device__ void locate(const AttnArgs& a, const int* pre, int entries, int shift, int u) {
-    int lo = 0, hi = entries;
+  __device__ void locate(const AttnArgs& a, const int* pre, int u) {
+    const int shift = kv4::prefix_shift(a);
+    int lo = 0, hi = (a.R + (1 << shift) - 1) >> shift;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pre[mid] <= u) lo = mid; else hi = mid;
@@ -209,7 +212,7 @@ static_assert(sizeof(Entry) == 40, "entry size");
 
 template <class G_>
 __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs a) {
-  constexpr int D = G_::D, NG = G_::NG, W = G_::W, NT = G_::NT, ROWS = G_::ROWS;
+  constexpr int D = G_::D, NG = G_::NG, W = G_::W, ROWS = G_::ROWS;
   constexpr int TB = G_::TB, TOKENS = G_::TOKENS, THREADS = G_::THREADS;
   constexpr int WARPS = G_::WARPS, STAGES = G_::STAGES, BLK = G_::BLK, TILE = G_::TILE;
   constexpr int GW = W / NG;                           // words (32 channels) per group
@@ -220,8 +223,6 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
   int* meta = reinterpret_cast<int*>(smem + G_::OFF_META);     // [warp][stage] blocks that arrive
   Entry* ent = reinterpret_cast<Entry*>(smem + G_::OFF_ENT);
   const uint32_t bars = sbase + G_::OFF_BAR;           // [warp][stage] full, empty
-  __shared__ int wsum[WARPS + 1];
-  __shared__ int s_total;
   __shared__ volatile int s_abort;                     // a wait ran out: everyone stops
 
   if (tid < WARPS * STAGES) {
@@ -231,36 +232,11 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
   }
   if (tid < 2 * WARPS) ent[tid].ptr = nullptr;
 
-  // ---- prefix sums of the requests' tiles (1 << shift requests per entry) ---------------
-  int shift = 0;
-  while ((a.R >> shift) + 1 > kPrefixEntries) ++shift;
-  const int entries = (a.R + (1 << shift) - 1) >> shift;
-  if (tid == 0) s_total = 0, s_abort = 0;
-  for (int e0 = 0; e0 < entries; e0 += THREADS) {
-    const int e = e0 + tid;
-    int v = 0;
-    if (e < entries)
-      for (int r = e << shift; r < min(a.R, (e + 1) << shift); ++r) {
-        const Req x = request<G_>(a, r);
-        v += a.kv_heads * x.nrt * x.tiles;
-      }
-    int inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int nb = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += nb;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    const int part = lane <= WARPS ? wsum[lane] : 0;
-    const int before = s_total + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
-    const int all = __reduce_add_sync(0xffffffffu, part);
-    if (e < entries) pre[e] = before + inc - v;
-    __syncthreads();
-    if (tid == 0) s_total += all;
-    __syncthreads();
-  }
-  const int U = s_total;
+  if (tid == 0) s_abort = 0;
+  const int U = kv4::scan_units<THREADS>(a, pre, [&](int r) {
+    const Req x = request<G_>(a, r);
+    return a.kv_heads * x.nrt * x.tiles;
+  });
   const int ctas = min((int)gridDim.x, (U + WARPS - 1) / WARPS);
   const int cta = blockIdx.x;
   if (cta >= ctas) {
@@ -288,7 +264,7 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
         }
         if (next < u1) pid = a.table[lc.r * a.table_rs + ((lc.tile * TB) >> bpp_shift)];
       };
-      if (next < u1) lc.locate<G_>(a, pre, entries, shift, next);
+      if (next < u1) lc.locate<G_>(a, pre, next);
       settle();
       uint64_t t0 = sm100::globaltimer_ns();
       while (next < u1 && !s_abort) {
@@ -334,56 +310,50 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
     const uint8_t* stage0 = smem + warp * STAGES * TILE;
     const uint32_t bar0 = bars + warp * STAGES * 16;
     Cursor cc = {};
-    cc.locate<G_>(a, pre, entries, shift, u0);
+    cc.locate<G_>(a, pre, u0);
     bool dead = false;
     int u = u0, use = 0, phase = 0;                     // use: the stage to read next
     while (u < u1) {
       // ---- one item, or this warp's part of it ----------------------------------------
       const int rows = cc.x.n * a.G, row0 = cc.rt * ROWS;
       const int ib = u - cc.tile, ie = ib + cc.x.tiles, ue = min(u1, ie);
-      uint32_t qa[NT][W][2], qb[NT][W][2];              // B operands: even / odd nibbles
-      float qs[NT][NG][2];                              // scale * sum of q over the group
-      int lim[NT][2];                                   // last visible token of the columns
-      uint4 qv[NT][W];
+      uint32_t qa[W][2], qb[W][2];              // B operands: even / odd nibbles
+      float qs[NG][2];                              // scale * sum of q over the group
+      int lim[2];                                   // last visible token of the columns
+      uint4 qv[W];
       float big = 0.f;
+      const int row = row0 + g;
+      const bool in = row < rows;
+      const __half* qp = a.q + (in ? (int64_t)(cc.x.q0 + row / a.G) * a.q_ts +
+                                         (int64_t)(cc.h * a.G + row % a.G) * a.q_hs
+                                   : 0);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int row = row0 + nt * 8 + g;
-        const bool in = row < rows;
-        const __half* qp = a.q + (in ? (int64_t)(cc.x.q0 + row / a.G) * a.q_ts +
-                                           (int64_t)(cc.h * a.G + row % a.G) * a.q_hs
-                                     : 0);
+      for (int j = 0; j < W; ++j) {
+        qv[j] = make_uint4(0, 0, 0, 0);
+        if (in) qv[j] = *reinterpret_cast<const uint4*>(qp + 8 * (4 * j + t));
+      }
+      float sum[NG] = {};
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          qv[nt][j] = make_uint4(0, 0, 0, 0);
-          if (in) qv[nt][j] = *reinterpret_cast<const uint4*>(qp + 8 * (4 * j + t));
+      for (int j = 0; j < W; ++j) {
+        const uint32_t w4[4] = {qv[j].x, qv[j].y, qv[j].z, qv[j].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = __half22float2(u32_as_h2(w4[k]));
+          sum[j / GW] += f.x + f.y;
+          big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float sum[NG] = {};
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t w4[4] = {qv[nt][j].x, qv[nt][j].y, qv[nt][j].z, qv[nt][j].w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 f = __half22float2(u32_as_h2(w4[k]));
-            sum[j / GW] += f.x + f.y;
-            big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < NG; ++k) {
-          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
-          sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
-          sum[k] *= a.scale_log2;
-          qs[nt][k][0] = __shfl_sync(0xffffffffu, sum[k], 8 * t);
-          qs[nt][k][1] = __shfl_sync(0xffffffffu, sum[k], 8 * t + 4);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          lim[nt][c] = cc.x.L - cc.x.n + (row0 + nt * 8 + 2 * t + c) / a.G;
+      for (int k = 0; k < NG; ++k) {
+        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+        sum[k] *= a.scale_log2;
+        qs[k][0] = __shfl_sync(0xffffffffu, sum[k], 8 * t);
+        qs[k][1] = __shfl_sync(0xffffffffu, sum[k], 8 * t + 4);
       }
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        lim[c] = cc.x.L - cc.x.n + (row0 + 2 * t + c) / a.G;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
       // 2^(15 - e) for the largest |q| in [2^e, 2^(e + 1)); 1 for zeros and infinities
@@ -391,31 +361,27 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
       const int up2 = big > 0.f && e_big <= 15 ? 15 - e_big : 0;
       const float qmul = __uint_as_float((uint32_t)(127 + up2) << 23);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int j = 0; j < W; ++j) {
+        const uint4 v = qv[j];
+        const uint32_t even[2] = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410)};
+        const uint32_t odd[2] = {__byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x7632)};
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint4 v = qv[nt][j];
-          const uint32_t even[2] = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410)};
-          const uint32_t odd[2] = {__byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x7632)};
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {                  // channels (0, 4), (2, 6); (1, 5), (3, 7)
-            const float2 e = __half22float2(u32_as_h2(even[k])), o = __half22float2(u32_as_h2(odd[k]));
-            qa[nt][j][k] = h2_as_u32(__floats2half2_rn(e.x * qmul, e.y * qmul));
-            qb[nt][j][k] = h2_as_u32(__floats2half2_rn(o.x * (qmul * 0.0625f), o.y * (qmul * 0.0625f)));
-          }
+        for (int k = 0; k < 2; ++k) {                    // channels (0, 4), (2, 6); (1, 5), (3, 7)
+          const float2 e = __half22float2(u32_as_h2(even[k])), o = __half22float2(u32_as_h2(odd[k]));
+          qa[j][k] = h2_as_u32(__floats2half2_rn(e.x * qmul, e.y * qmul));
+          qb[j][k] = h2_as_u32(__floats2half2_rn(o.x * (qmul * 0.0625f), o.y * (qmul * 0.0625f)));
         }
+      }
       const int lim_all = cc.x.L - cc.x.n + row0 / a.G;  // every row sees tokens up to here
       // codes enter the MMA times 2^-24, queries times qmul
       const float ksc = a.scale_log2 * 16777216.0f * __uint_as_float((uint32_t)(127 - up2) << 23);
-      float O[NT][2 * W][4] = {}, M[NT][2], l[NT][2] = {}, pm[NT][NG][2] = {};
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) M[nt][0] = M[nt][1] = -CUDART_INF_F;
+      float O[2 * W][4] = {}, M[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {}, pm[NG][2] = {};
 
       // One tile; EDGE: some of its tokens may be unseen (past a row's limit, or in a page the
       // table does not name).
       auto tile = [&](auto edge, const uint8_t* st, int tok0, int ok) {
         constexpr bool EDGE = decltype(edge)::value;
-        float x[NT][TB][4];                     // [block][token g / g + 8, column]
+        float x[TB][4];                         // [block][token g / g + 8, column]
         float ls[TB][2];                        // log2 of a token's largest value scale
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
@@ -429,37 +395,32 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
           for (int k = 0; k < NG; ++k) {
             const float2 f0 = __half22float2(u32_as_h2(p0[k])), f1 = __half22float2(u32_as_h2(p1[k]));
             const float s0 = f0.x * ksc, s1 = f1.x * ksc;
+            float acc[4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float acc[4];
+            for (int j = k * GW; j < (k + 1) * GW; ++j) {
+              // x >> 8 as the high half of x 2^24: the multiplier has room, the logic pipe not
+              const uint32_t h0 = __umulhi(k0[j], 1u << 24), h1 = __umulhi(k1[j], 1u << 24);
+              if (j == k * GW)
+                mma16816_first(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
+                               qa[j][0], qa[j][1]);
+              else
+                mma16816(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
+                         qa[j][0], qa[j][1]);
+              mma16816(acc, k0[j] & kHiMask, k1[j] & kHiMask, h0 & kHiMask, h1 & kHiMask,
+                       qb[j][0], qb[j][1]);
+            }
 #pragma unroll
-              for (int j = k * GW; j < (k + 1) * GW; ++j) {
-                // x >> 8 as the high half of x 2^24: the multiplier has room, the logic pipe not
-                const uint32_t h0 = __umulhi(k0[j], 1u << 24), h1 = __umulhi(k1[j], 1u << 24);
-                if (j == k * GW)
-                  mma16816_first(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
-                                 qa[nt][j][0], qa[nt][j][1]);
-                else
-                  mma16816(acc, k0[j] & kLoMask, k1[j] & kLoMask, h0 & kLoMask, h1 & kLoMask,
-                           qa[nt][j][0], qa[nt][j][1]);
-                mma16816(acc, k0[j] & kHiMask, k1[j] & kHiMask, h0 & kHiMask, h1 & kHiMask,
-                         qb[nt][j][0], qb[nt][j][1]);
-              }
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float m = i < 2 ? f0.y : f1.y, q1 = qs[nt][k][i & 1];
-                const float base = k == 0 ? m * q1 : fmaf(m, q1, x[nt][b][i]);
-                x[nt][b][i] = fmaf(acc[i], i < 2 ? s0 : s1, base);
-              }
+            for (int i = 0; i < 4; ++i) {
+              const float m = i < 2 ? f0.y : f1.y, q1 = qs[k][i & 1];
+              const float base = k == 0 ? m * q1 : fmaf(m, q1, x[b][i]);
+              x[b][i] = fmaf(acc[i], i < 2 ? s0 : s1, base);
             }
           }
           if constexpr (EDGE) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (tok0 + b * 16 + g + (i / 2) * 8 > lim[nt][i & 1] || !((ok >> b) & 1))
-                  x[nt][b][i] = -CUDART_INF_F;
+            for (int i = 0; i < 4; ++i)
+              if (tok0 + b * 16 + g + (i / 2) * 8 > lim[i & 1] || !((ok >> b) & 1))
+                x[b][i] = -CUDART_INF_F;
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -474,70 +435,62 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
         // the softmax reference moves only when it is more than 2^8 behind (the fp16 weights
         // then reach 2^8 at most); -inf + 8 = -inf, so the first visible token sets it
         bool up = false;
-        float nm[NT][2];
+        float nm[2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int c = 0; c < 2; ++c) {
+          float m = fmaxf(x[0][c] + ls[0][0], x[0][2 + c] + ls[0][1]);
+#pragma unroll
+          for (int b = 1; b < TB; ++b)
+            m = fmaxf(m, fmaxf(x[b][c] + ls[b][0], x[b][2 + c] + ls[b][1]));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          nm[c] = m;
+          up |= m > M[c] + 8.0f;
+        }
+        if (__any_sync(0xffffffffu, up)) {
+          float f[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float m = fmaxf(x[nt][0][c] + ls[0][0], x[nt][0][2 + c] + ls[0][1]);
+            const float m = fmaxf(M[c], nm[c]);
+            f[c] = M[c] == m ? 1.0f : ex2(M[c] - m);
+            M[c] = m;
+            l[c] *= f[c];
 #pragma unroll
-            for (int b = 1; b < TB; ++b)
-              m = fmaxf(m, fmaxf(x[nt][b][c] + ls[b][0], x[nt][b][2 + c] + ls[b][1]));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            nm[nt][c] = m;
-            up |= m > M[nt][c] + 8.0f;
+            for (int k = 0; k < NG; ++k) pm[k][c] *= f[c];
           }
-        if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float f[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float m = fmaxf(M[nt][c], nm[nt][c]);
-              f[c] = M[nt][c] == m ? 1.0f : ex2(M[nt][c] - m);
-              M[nt][c] = m;
-              l[nt][c] *= f[c];
-#pragma unroll
-              for (int k = 0; k < NG; ++k) pm[nt][k][c] *= f[c];
-            }
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) {
-              O[nt][i][0] *= f[0], O[nt][i][1] *= f[1];
-              O[nt][i][2] *= f[0], O[nt][i][3] *= f[1];
-            }
+          for (int i = 0; i < 2 * W; ++i) {
+            O[i][0] *= f[0], O[i][1] *= f[1];
+            O[i][2] *= f[0], O[i][3] *= f[1];
           }
         }
 #pragma unroll
         for (int b = 0; b < TB; ++b) {
           const uint8_t* blk = st + b * BLK;
-          uint32_t wb[NT][NG][2];                        // B operands: weights p s per group
+          uint32_t wb[NG][2];                            // B operands: weights p s per group
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t pv[NG];
             load_words<NG>(blk + kv4::off_vp(D, G_::GROUP) + (g + 8 * e) * (4 * NG), pv);
+            float p[2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float p[2];
+            for (int c = 0; c < 2; ++c) {
+              p[c] = ex2(x[b][2 * e + c] - (EDGE && M[c] == -CUDART_INF_F ? 0.f : M[c]));
+              l[c] += p[c];
+            }
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+              const float2 f = __half22float2(u32_as_h2(pv[k]));
+              float w[2];
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                p[c] = ex2(x[nt][b][2 * e + c] - (EDGE && M[nt][c] == -CUDART_INF_F ? 0.f : M[nt][c]));
-                l[nt][c] += p[c];
+                // an unseen token's scale and minimum may be anything: no 0 * NaN
+                const bool seen = !EDGE || p[c] != 0.f;
+                w[c] = seen ? p[c] * f.x : 0.f;
+                pm[k][c] = seen ? fmaf(p[c], f.y, pm[k][c]) : pm[k][c];
               }
-#pragma unroll
-              for (int k = 0; k < NG; ++k) {
-                const float2 f = __half22float2(u32_as_h2(pv[k]));
-                float w[2];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  // an unseen token's scale and minimum may be anything: no 0 * NaN
-                  const bool seen = !EDGE || p[c] != 0.f;
-                  w[c] = seen ? p[c] * f.x : 0.f;
-                  pm[nt][k][c] = seen ? fmaf(p[c], f.y, pm[nt][k][c]) : pm[nt][k][c];
-                }
-                wb[nt][k][e] = movmatrix(h2_as_u32(__floats2half2_rn(w[0], w[1])));
-              }
+              wb[k][e] = movmatrix(h2_as_u32(__floats2half2_rn(w[0], w[1])));
             }
           }
           uint32_t v0[W], v1[W];
@@ -548,12 +501,9 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
             // bytes: code p in the low nibble, code p + 1 in the high one
             const uint32_t a0 = __byte_perm(v0[i], 0, 0x4240), a1 = __byte_perm(v0[i], 0, 0x4341);
             const uint32_t a2 = __byte_perm(v1[i], 0, 0x4240), a3 = __byte_perm(v1[i], 0, 0x4341);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(O[nt][2 * i], a0 & kLoMask, a1 & kLoMask, a2 & kLoMask, a3 & kLoMask,
-                       wb[nt][i / GW][0], wb[nt][i / GW][1]);
-              mma16816(O[nt][2 * i + 1], a0, a1, a2, a3, wb[nt][i / GW][0], wb[nt][i / GW][1]);
-            }
+            mma16816(O[2 * i], a0 & kLoMask, a1 & kLoMask, a2 & kLoMask, a3 & kLoMask,
+                     wb[i / GW][0], wb[i / GW][1]);
+            mma16816(O[2 * i + 1], a0, a1, a2, a3, wb[i / GW][0], wb[i / GW][1]);
           }
         }
       };
@@ -579,16 +529,14 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
 
       // ---- the item's (part's) result ---------------------------------------------------
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int o = 4; o < 32; o <<= 1) {
+          l[c] += __shfl_xor_sync(0xffffffffu, l[c], o);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) {
-            l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
-#pragma unroll
-            for (int k = 0; k < NG; ++k) pm[nt][k][c] += __shfl_xor_sync(0xffffffffu, pm[nt][k][c], o);
-          }
+          for (int k = 0; k < NG; ++k) pm[k][c] += __shfl_xor_sync(0xffffffffu, pm[k][c], o);
         }
+      }
       const bool whole = ib >= u0 && ie <= u1;
       float* slot = nullptr;
       if (!whole) {
@@ -602,36 +550,34 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
         }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int c = 0; c < 2; ++c) {
+        const int col = 2 * t + c, row = row0 + col;
+        const float inv = l[c] == 0.f ? 0.f : 1.0f / l[c];
+        __half* op = nullptr;
+        if (whole && row < rows)
+          op = a.out + (int64_t)(cc.x.q0 + row / a.G) * a.o_ts + (int64_t)(cc.h * a.G + row % a.G) * a.o_hs;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int col = nt * 8 + 2 * t + c, row = row0 + col;
-          const float inv = l[nt][c] == 0.f ? 0.f : 1.0f / l[nt][c];
-          __half* op = nullptr;
-          if (whole && row < rows)
-            op = a.out + (int64_t)(cc.x.q0 + row / a.G) * a.o_ts + (int64_t)(cc.h * a.G + row % a.G) * a.o_hs;
-#pragma unroll
-          for (int i = 0; i < W; ++i) {
-            const float m = pm[nt][i / GW][c];
-            // 2 i: even codes; 2 i + 1: even + 16 odd
-            const float e0 = O[nt][2 * i][c], e1 = O[nt][2 * i][2 + c];
-            const float4 v = make_float4(fmaf(e0, 16777216.f, m),
-                                         fmaf(O[nt][2 * i + 1][c] - e0, 1048576.f, m),
-                                         fmaf(e1, 16777216.f, m),
-                                         fmaf(O[nt][2 * i + 1][2 + c] - e1, 1048576.f, m));
-            if (slot) {
-              *reinterpret_cast<float4*>(slot + col * D + 32 * i + 4 * g) = v;
-            } else if (op) {
-              *reinterpret_cast<uint2*>(op + 32 * i + 4 * g) =
-                  make_uint2(h2_as_u32(__floats2half2_rn(v.x * inv, v.y * inv)),
-                             h2_as_u32(__floats2half2_rn(v.z * inv, v.w * inv)));
-            }
-          }
-          if (slot && g == 0) {
-            slot[ROWS * D + col] = M[nt][c];
-            slot[ROWS * D + ROWS + col] = l[nt][c];
+        for (int i = 0; i < W; ++i) {
+          const float m = pm[i / GW][c];
+          // 2 i: even codes; 2 i + 1: even + 16 odd
+          const float e0 = O[2 * i][c], e1 = O[2 * i][2 + c];
+          const float4 v = make_float4(fmaf(e0, 16777216.f, m),
+                                       fmaf(O[2 * i + 1][c] - e0, 1048576.f, m),
+                                       fmaf(e1, 16777216.f, m),
+                                       fmaf(O[2 * i + 1][2 + c] - e1, 1048576.f, m));
+          if (slot) {
+            *reinterpret_cast<float4*>(slot + col * D + 32 * i + 4 * g) = v;
+          } else if (op) {
+            *reinterpret_cast<uint2*>(op + 32 * i + 4 * g) =
+                make_uint2(h2_as_u32(__floats2half2_rn(v.x * inv, v.y * inv)),
+                           h2_as_u32(__floats2half2_rn(v.z * inv, v.w * inv)));
           }
         }
+        if (slot && g == 0) {
+          slot[ROWS * D + col] = M[c];
+          slot[ROWS * D + ROWS + col] = l[c];
+        }
+      }
       if (u < u1) cc.next_item<G_>(a);
     }
   }
@@ -713,7 +659,7 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
 // Joins an item that crosses CTAs: block (c, col) sums column col of the item that starts in
 // CTA c, over the slots of CTAs c .. c + span - 1, in four (eight) interleaved groups.
 template <int D>
-__global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const int rows_per_item) {
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a) {
   constexpr int LANES = D / 4, GROUPS = 128 / LANES;
   __shared__ float s_m[4], s_l[GROUPS];
   __shared__ float4 s_o[GROUPS][LANES];
@@ -724,11 +670,11 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const 
   if (span == 0) return;
   const int row = d[2] + col;
   if (row >= d[3]) return;
-  const size_t slot = (size_t)rows_per_item * (D + 2);
+  const size_t slot = (size_t)kRows * (D + 2);
   // CTA c's item is in its slot 1, the following CTAs' parts of it in their slots 0
   auto part = [&](int k) { return a.part + (size_t)((cta + k) * 2 + (k == 0)) * slot; };
   float m = -CUDART_INF_F;
-  for (int k = tid; k < span; k += 128) m = fmaxf(m, part(k)[rows_per_item * D + col]);
+  for (int k = tid; k < span; k += 128) m = fmaxf(m, part(k)[kRows * D + col]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) s_m[tid / 32] = m;
@@ -740,9 +686,9 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const 
 #pragma unroll 4
   for (int k = grp; k < span; k += GROUPS) {
     const float* p = part(k);
-    const float mk = p[rows_per_item * D + col], f = mk == m ? 1.0f : ex2(mk - m);
+    const float mk = p[kRows * D + col], f = mk == m ? 1.0f : ex2(mk - m);
     const float4 v = *reinterpret_cast<const float4*>(p + col * D + 4 * ch);
-    l = fmaf(f, p[rows_per_item * D + rows_per_item + col], l);
+    l = fmaf(f, p[kRows * D + kRows + col], l);
     o.x = fmaf(f, v.x, o.x), o.y = fmaf(f, v.y, o.y), o.z = fmaf(f, v.z, o.z), o.w = fmaf(f, v.w, o.w);
   }
   s_o[grp][ch] = o;
@@ -762,13 +708,13 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a, const 
                                                       h2_as_u32(__floats2half2_rn(o.z * inv, o.w * inv)));
 }
 
-// Consumer warps of a CTA.  With the producer 12 (8) warps: 168 (255) registers a thread, what
-// a 64-token tile of 8 (16) query rows takes without spilling.  Measured on B200, 48 requests
-// of 1 to 16384 tokens, 28 / 4 heads: 11 warps x 64 tokens 47.4 us, 15 warps x 32 tokens
-// 53.5 us (more instructions per token: the logic pipe, which unpacks the codes, binds).
-constexpr int kWarps1 = 11, kWarps2 = 7;
-// warp slots of either kernel, in rows
-constexpr int kSlotRows = kWarps1 * 8 > kWarps2 * 16 ? kWarps1 * 8 : kWarps2 * 16;
+// Consumer warps of a CTA.  With the producer 12: 168 registers a thread, what a 64-token tile
+// of 8 query rows takes without spilling.  Measured on B200, 48 requests of 1 to 16384 tokens,
+// 28 / 4 heads: 11 warps x 64 tokens 47.4 us, 15 warps x 32 tokens 53.5 us (more instructions
+// per token: the logic pipe, which unpacks the codes, binds).  Items of 16 rows halve the
+// unpacking but fit 7 warps only: 8 requests of 4096 tokens with 4 query tokens take 27.2 us
+// (8 rows: 26.8), with 24 tokens 76 (78), with one token 30 (21).
+constexpr int kWarps = 11;
 
 template <class G_>
 cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
@@ -790,23 +736,21 @@ cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<G_::D>, a, (int)G_::ROWS);
+  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<G_::D>, a);
 }
 
 template <int D, int GROUP>
-cudaError_t launch_rows(const AttnArgs& a, int64_t max_rows, int num_sms, cudaStream_t stream) {
+cudaError_t launch_form(const AttnArgs& a, int num_sms, cudaStream_t stream) {
   // two stages must fit shared memory: 32-token tiles where a 64-token one takes 10 KB
-  constexpr int tb = D / GROUP == 4 ? 2 : 4;
-  if (max_rows <= 8) return launch_geo<Geo<D, GROUP, 1, tb, kWarps1>>(a, num_sms, stream);
-  return launch_geo<Geo<D, GROUP, 2, 4, kWarps2>>(a, num_sms, stream);
+  return launch_geo<Geo<D, GROUP, D / GROUP == 4 ? 2 : 4, kWarps>>(a, num_sms, stream);
 }
 
 }  // namespace
 
 size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms) {
-  // descriptors, 2 slots per CTA (up to 16 rows) and one per warp; or the prefill kernel's 2
-  // slots of 256 rows per CTA (the two kernels of a call run one after the other)
-  const int rows = max_rows >= kKv4PrefillMinRows ? 2 * kKv4PrefillRows : 2 * 16 + kSlotRows;
+  // descriptors, 2 slots per CTA and one per warp; or the prefill kernel's 2 slots of 256 rows
+  // per CTA (the two kernels of a call run one after the other)
+  const int rows = max_rows >= kKv4PrefillMinRows ? 2 * kKv4PrefillRows : (2 + kWarps) * kRows;
   return (size_t)num_sms * (kDescInts * 4 + (size_t)rows * (head_dim + 2) * 4);
 }
 
@@ -825,21 +769,19 @@ cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_sta
   a.R = c.rows, a.width = c.width, a.kv_heads = c.cache.heads, a.G = c.q_heads / c.cache.heads;
   a.page_shift = 0;
   while ((1 << a.page_shift) < c.cache.page) ++a.page_shift;
-  int64_t max_rows = (int64_t)c.max_q * a.G;
   const int D = c.cache.dim, g = c.cache.group;
   a.min_rows = 0x7fffffff;
-  if (max_rows >= kKv4PrefillMinRows) {
+  if ((int64_t)c.max_q * a.G >= kKv4PrefillMinRows) {
     // requests with many query rows, then those with few, which share no output row
     a.min_rows = kKv4PrefillMinRows;
     const cudaError_t e = launch_kv4_prefill(a, D, g, num_sms, stream);
     if (e != cudaSuccess) return e;
-    max_rows = a.G;                                      // decode rows are the ones to be fast
   }
-  if (D == 64 && g == 32) return launch_rows<64, 32>(a, max_rows, num_sms, stream);
-  if (D == 64 && g == 64) return launch_rows<64, 64>(a, max_rows, num_sms, stream);
-  if (D == 128 && g == 32) return launch_rows<128, 32>(a, max_rows, num_sms, stream);
-  if (D == 128 && g == 64) return launch_rows<128, 64>(a, max_rows, num_sms, stream);
-  if (D == 128 && g == 128) return launch_rows<128, 128>(a, max_rows, num_sms, stream);
+  if (D == 64 && g == 32) return launch_form<64, 32>(a, num_sms, stream);
+  if (D == 64 && g == 64) return launch_form<64, 64>(a, num_sms, stream);
+  if (D == 128 && g == 32) return launch_form<128, 32>(a, num_sms, stream);
+  if (D == 128 && g == 64) return launch_form<128, 64>(a, num_sms, stream);
+  if (D == 128 && g == 128) return launch_form<128, 128>(a, num_sms, stream);
   return cudaErrorInvalidValue;
 }
 

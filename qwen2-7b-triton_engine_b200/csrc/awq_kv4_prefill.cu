@@ -203,15 +203,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
   const int tid = threadIdx.x, lane = tid & 31, warp = tid / 32;
   int* pre = reinterpret_cast<int*>(smem + G_::OFF_PRE);
   const uint32_t bars = sbase + G_::OFF_BAR;
-  __shared__ int wsum[kThreads / 32];
-  __shared__ int s_total;
   __shared__ volatile int s_abort;
   __shared__ uint32_t s_tmem;
   __shared__ Item s_first;
   __shared__ int raw_ok[kRawStages], par_ok[kParStages];   // blocks of the step that are there
 
   if (tid == 0) {
-    s_total = 0, s_abort = 0;
+    s_abort = 0;
     for (int i = 0; i < NBARS; ++i) {
       int count = 1;                                     // bulk copies, MMA commits
       if (i >= RAW_EMPTY && i < RAW_EMPTY + 2) count = 128;
@@ -224,37 +222,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     }
     sm100::fence_mbar_init();
   }
-  // ---- prefix sums of the requests' steps -------------------------------------------------
-  int shift = 0;
-  while ((a.R >> shift) + 1 > kPrefixEntries) ++shift;
-  const int entries = (a.R + (1 << shift) - 1) >> shift;
-  for (int e0 = 0; e0 < entries; e0 += kThreads) {
-    const int e = e0 + tid;
-    int v = 0;
-    if (e < entries)
-      for (int r = e << shift; r < min(a.R, (e + 1) << shift); ++r) {
-        Item it;
-        it.r = r;
-        it.request<G_>(a);
-        v += a.kv_heads * it.units<G_>(a);
-      }
-    int inc = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int nb = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += nb;
-    }
-    if (lane == 31) wsum[warp] = inc;
-    __syncthreads();
-    const int part = lane < kThreads / 32 ? wsum[lane] : 0;
-    const int before = s_total + __reduce_add_sync(0xffffffffu, lane < warp ? part : 0);
-    const int all = __reduce_add_sync(0xffffffffu, part);
-    if (e < entries) pre[e] = before + inc - v;
-    __syncthreads();
-    if (tid == 0) s_total += all;
-    __syncthreads();
-  }
-  const int U = s_total;
+  const int U = kv4::scan_units<kThreads>(a, pre, [&](int r) {
+    Item it;
+    it.r = r;
+    it.request<G_>(a);
+    return a.kv_heads * it.units<G_>(a);
+  });
   const int cta = blockIdx.x, ctas = min((int)gridDim.x, U);
   if (cta >= ctas) {
     if (tid == 0) a.desc[cta * kDescInts] = 0;
@@ -268,7 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     sm100::tmem_relinquish();
   }
   if (tid == 32) {
-    int lo = 0, hi = entries;
+    const int shift = kv4::prefix_shift(a);
+    int lo = 0, hi = (a.R + (1 << shift) - 1) >> shift;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (pre[mid] <= u0) lo = mid; else hi = mid;

@@ -168,7 +168,8 @@ int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   // the list of (request, kv head, row tile, 32-token tile) is counted in 32 bits
   const double tiles = (double)max_blocks * (double)page_size / 32 + 1;
   const double rows = (double)tokens * (double)(q_heads / kv_heads) / 8 + (double)requests;
-  if (tiles * rows * (double)kv_heads > 2147000000.0 || (double)max_blocks * page_size > 2147000000.0)
+  if (tiles * rows * (double)kv_heads > 2147000000.0 || (double)max_blocks * page_size > 2147000000.0 ||
+      tokens * (q_heads / kv_heads) > 2147000000)
     return fail(AWQ_ERR_UNSUPPORTED, "tokens x max_blocks x page_size is too large for one call");
   int sms = 0, *status = nullptr;
   if ((rc = awq::device_context(&sms, &status))) return rc;

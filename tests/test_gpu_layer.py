@@ -417,6 +417,56 @@ def test_attention_prompt_chunks(cuda, D, group, H, Hk, lens, qs, page):
     check_attention(np.random.default_rng(sum(lens)), lens, qs, H, Hk, D, group, page, pad=2)
 
 
+@pytest.mark.parametrize("D,group,H,Hk", [(128, 128, 7, 1), (128, 32, 4, 4), (64, 64, 16, 2),
+                                          (64, 32, 1, 1)])
+@pytest.mark.parametrize("rows", [255, 256, 257, 512, 513])
+def test_attention_prompt_row_tiles(cuda, D, group, H, Hk, rows):
+    """Chunks whose query rows end at, before and behind an item of 256 rows, beside a chunk
+    and a token that take the other kernel."""
+    G = H // Hk
+    n = -(-rows // G)
+    check_attention(np.random.default_rng(rows), [n + 45, 40, 9], [n, 3, 1], H, Hk, D, group, 32, pad=1)
+
+
+@pytest.mark.parametrize("D,group", CACHES)
+def test_attention_prompt_nan_and_lost_page(cuda, D, group):
+    """300 query rows of a request: a page the table does not name, and a NaN key and value."""
+    rng = np.random.default_rng(24)
+    cache, table, KV, _, kv = make_cache(rng, [200], 1, D, group, 16)
+    q = rng.standard_normal((150, 2, D)).astype(np.float16)
+    lens, cu = dev(np.array([200])).int(), dev(np.array([0, 150])).int()
+    page1 = int(table[0, 1])
+    table[0, 1] = -1
+    got = awq_b200.kv4_attention(dev(q), cache, table, lens, cu, 150).double().cpu().numpy()
+    assert awq_b200.device_status() == 2
+    keep = [*range(16), *range(32, 200)]
+    K, V = (x[keep] for x in KV[0])
+    # row i sees the tokens up to 50 + i
+    ref = np.stack([L.attention(q[i:i + 1], K[:35 + i], V[:35 + i], D ** -0.5)[0] for i in range(150)])
+    assert np.abs(got - ref).max() <= 2e-3 * np.abs(V).max()
+    table[0, 1] = page1
+    k = torch.full((1, 1, D), float("nan"), dtype=torch.float16, device="cuda")
+    awq_b200.kv4_append(k, k, dev(kv[0][2][150:151]), cache)
+    got = awq_b200.kv4_attention(dev(q), cache, table, lens, cu, 150)
+    bad = torch.isnan(got).flatten(1)
+    assert bad[100:].all() and not bad[:100].any()
+
+
+def test_attention_requests_that_share_rows(cuda):
+    """cu_q that goes back and forth lists more work than the call admits: the kernels count
+    it, compute nothing and say so.  R requests of n rows and 2^19 tokens each."""
+    R, n, width, page = 8192, 800, 512, 1024
+    cache = awq_b200.KV4Cache.allocate(1, 1, 64, page, 64)
+    table = torch.full((1, width), -1, dtype=torch.int32, device="cuda").expand(R, width)
+    lens = torch.full((R,), width * page, dtype=torch.int32, device="cuda")
+    cu = (torch.arange(R + 1, device="cuda") % 2 * n).int()
+    q = torch.zeros((n, 1, 64), dtype=torch.float16, device="cuda")
+    out = torch.full_like(q, 7.0)
+    awq_b200.kv4_attention(q, cache, table.contiguous(), lens, cu, 4, out=out)
+    assert awq_b200.device_status() == 2
+    assert (out == 7.0).all()
+
+
 def test_attention_prompt_scale_and_small_values(cuda):
     rng = np.random.default_rng(21)
     for kw in (dict(small=True), dict(scale=2.0), dict(scale=-0.3), dict(scale=0.0)):
