@@ -207,6 +207,7 @@ struct AttnArgs;
 }
 cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, int head_dim, int group, int num_sms,
                                cudaStream_t stream);
+cudaError_t launch_kv4_prefill_merge(const kv4::AttnArgs& a, int head_dim, int num_sms, cudaStream_t stream);
 struct Kv4AttnCall {
   Kv4Shape cache;
   const void* data;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "awq_common.cuh"
@@ -23,6 +24,7 @@ struct AttnArgs {
   int64_t q_ts, q_hs, o_ts, o_hs, table_rs;
   int64_t num_pages;
   int64_t tokens;
+  // each kernel's own, as the two may overlap:
   float* part;        // [ctas][2] slots of items that cross CTAs
   float* warp_part;   // [ctas][warps] slots of items that cross warps, not a warp's last
   int* desc;          // [ctas][kDescInts]
@@ -31,6 +33,24 @@ struct AttnArgs {
   int R, width, page_shift, kv_heads, G;
   int min_rows;       // requests with this many query rows per kv head are the prefill kernel's
 };
+
+// Launch of a kernel that may start while the one before it in the stream still runs, and
+// waits for it (grid_dependency_wait) where it needs its results.
+template <class K>
+cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                              const AttnArgs& a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
 
 // Requests of one entry of the prefix sums: 1 << shift.
 __device__ __forceinline__ int prefix_shift(const AttnArgs& a) {

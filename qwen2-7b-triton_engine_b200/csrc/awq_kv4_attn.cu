@@ -241,6 +241,7 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
   const int cta = blockIdx.x;
   if (cta >= ctas) {
     if (tid == 0) a.desc[cta * kDescInts] = 0;
+    sm100::grid_dependency_wait();
     return;
   }
   // unit ranges: warp w of all Wt starts at floor(U w / Wt)
@@ -654,6 +655,9 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
     int* d = a.desc + cta * kDescInts;
     d[0] = span, d[1] = head.q0, d[2] = head.row0, d[3] = head.rows, d[4] = head.h;
   }
+  // The tcgen05 kernel may still run: this one has not ended before it, so that whoever waits
+  // for this one has waited for both.
+  sm100::grid_dependency_wait();
 }
 
 // Joins an item that crosses CTAs: block (c, col) sums column col of the item that starts in
@@ -663,6 +667,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a) {
   constexpr int LANES = D / 4, GROUPS = 128 / LANES;
   __shared__ float s_m[4], s_l[GROUPS];
   __shared__ float4 s_o[GROUPS][LANES];
+  sm100::grid_launch_dependents();
   sm100::grid_dependency_wait();
   const int cta = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, lane = tid & 31;
   const int* d = a.desc + cta * kDescInts;
@@ -715,6 +720,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a) {
 // unpacking but fit 7 warps only: 8 requests of 4096 tokens with 4 query tokens take 27.2 us
 // (8 rows: 26.8), with 24 tokens 76 (78), with one token 30 (21).
 constexpr int kWarps = 11;
+constexpr int kNoPrefill = 0x7fffffff;                 // min_rows where only this kernel runs
 
 template <class G_>
 cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
@@ -724,19 +730,15 @@ cudaError_t launch_geo(AttnArgs a, int num_sms, cudaStream_t stream) {
   });
   if (attr != cudaSuccess) return attr;
   a.warp_part = a.part + (size_t)num_sms * 2 * G_::SLOT;
-  kv4_attn_kernel<G_><<<num_sms, G_::THREADS, G_::SMEM, stream>>>(a);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (a.min_rows == kNoPrefill) {
+    kv4_attn_kernel<G_><<<num_sms, G_::THREADS, G_::SMEM, stream>>>(a);
+    e = cudaGetLastError();
+  } else {                                               // beside the end of the tcgen05 kernel
+    e = kv4::launch_overlapped(kv4_attn_kernel<G_>, dim3(num_sms), G_::THREADS, G_::SMEM, stream, a);
+  }
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms, G_::ROWS, 1);
-  cfg.blockDim = dim3(128, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_merge_kernel<G_::D>, a);
+  return kv4::launch_overlapped(kv4_merge_kernel<G_::D>, dim3(num_sms, kRows), 128, 0, stream, a);
 }
 
 template <int D, int GROUP>
@@ -745,13 +747,24 @@ cudaError_t launch_form(const AttnArgs& a, int num_sms, cudaStream_t stream) {
   return launch_geo<Geo<D, GROUP, D / GROUP == 4 ? 2 : 4, kWarps>>(a, num_sms, stream);
 }
 
+cudaError_t launch_decode(const AttnArgs& a, int D, int g, int num_sms, cudaStream_t stream) {
+  if (D == 64 && g == 32) return launch_form<64, 32>(a, num_sms, stream);
+  if (D == 64 && g == 64) return launch_form<64, 64>(a, num_sms, stream);
+  if (D == 128 && g == 32) return launch_form<128, 32>(a, num_sms, stream);
+  if (D == 128 && g == 64) return launch_form<128, 64>(a, num_sms, stream);
+  if (D == 128 && g == 128) return launch_form<128, 128>(a, num_sms, stream);
+  return cudaErrorInvalidValue;
+}
+
 }  // namespace
 
 size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms) {
-  // descriptors, 2 slots per CTA and one per warp; or the prefill kernel's 2 slots of 256 rows
-  // per CTA (the two kernels of a call run one after the other)
-  const int rows = max_rows >= kKv4PrefillMinRows ? 2 * kKv4PrefillRows : (2 + kWarps) * kRows;
-  return (size_t)num_sms * (kDescInts * 4 + (size_t)rows * (head_dim + 2) * 4);
+  // per CTA a descriptor, 2 slots and one per warp; and for the prefill kernel, which the other
+  // may overlap, a descriptor and 2 slots of 256 rows
+  const size_t row = (size_t)(head_dim + 2) * 4;
+  size_t bytes = kDescInts * 4 + (2 + kWarps) * kRows * row;
+  if (max_rows >= kKv4PrefillMinRows) bytes += kDescInts * 4 + 2 * kKv4PrefillRows * row;
+  return num_sms * bytes;
 }
 
 cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
@@ -770,19 +783,19 @@ cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_sta
   a.page_shift = 0;
   while ((1 << a.page_shift) < c.cache.page) ++a.page_shift;
   const int D = c.cache.dim, g = c.cache.group;
-  a.min_rows = 0x7fffffff;
-  if ((int64_t)c.max_q * a.G >= kKv4PrefillMinRows) {
-    // requests with many query rows, then those with few, which share no output row
-    a.min_rows = kKv4PrefillMinRows;
-    const cudaError_t e = launch_kv4_prefill(a, D, g, num_sms, stream);
-    if (e != cudaSuccess) return e;
+  if ((int64_t)c.max_q * a.G < kKv4PrefillMinRows) {
+    a.min_rows = kNoPrefill;
+    return launch_decode(a, D, g, num_sms, stream);
   }
-  if (D == 64 && g == 32) return launch_form<64, 32>(a, num_sms, stream);
-  if (D == 64 && g == 64) return launch_form<64, 64>(a, num_sms, stream);
-  if (D == 128 && g == 32) return launch_form<128, 32>(a, num_sms, stream);
-  if (D == 128 && g == 64) return launch_form<128, 64>(a, num_sms, stream);
-  if (D == 128 && g == 128) return launch_form<128, 128>(a, num_sms, stream);
-  return cudaErrorInvalidValue;
+  // requests with many query rows beside those with few; they share no output row
+  a.min_rows = kKv4PrefillMinRows;
+  AttnArgs p = a;
+  p.desc = reinterpret_cast<int*>(a.part + (size_t)num_sms * (2 + kWarps) * kRows * (D + 2));
+  p.part = reinterpret_cast<float*>(p.desc + num_sms * kDescInts);
+  cudaError_t e = launch_kv4_prefill(p, D, g, num_sms, stream);
+  if (e == cudaSuccess) e = launch_decode(a, D, g, num_sms, stream);
+  if (e == cudaSuccess) e = launch_kv4_prefill_merge(p, D, num_sms, stream);
+  return e;
 }
 
 }  // namespace awq

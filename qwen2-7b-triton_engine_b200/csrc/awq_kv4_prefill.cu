@@ -44,6 +44,10 @@ using kv4::kPrefixEntries;
 constexpr int kThreads = 512;
 constexpr int kRows = kKv4PrefillRows;   // 256: query rows of an item, two tiles of 128
 constexpr int kKvSlots = 3, kRawStages = 2, kParStages = 2;
+// Empty steps of an item, for its fixed cost (queries, first and last step, result).  Four
+// requests of 1024 query and up to 8192 cached tokens, 28 / 4 heads: 1 375 us, 2 368 us, 4 360 us
+// with a result that took 6 us; with today's 2 345 us, 3 344 us.
+constexpr int kItemSteps = 3;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D_, int GROUP_>
@@ -71,7 +75,7 @@ enum Bar { RAW_FULL = 0, RAW_EMPTY = 2, KV_FULL = 4, KV_EMPTY = 7, PAR_FULL = 10
            Q_READY = 14, S_FULL = 16, P_READY = 18, O_FULL = 20, DRAIN = 22, NBARS = 23 };
 
 // A request's items: nrt row tiles of 256 per kv head, each with its causal number of steps
-// and one empty step that stands for its fixed cost.
+// and kItemSteps empty ones that stand for its fixed cost.
 struct Item {
   int L, n, q0, nrt;
   int r, h, rt, step;
@@ -95,12 +99,19 @@ struct Item {
   __device__ int steps_of(const AttnArgs& a, int tile, int* seen) const {
     const int last = min(n - 1, (int)(((long long)(tile + 1) * kRows - 1) / a.G));
     *seen = max(0, L - n + last + 1);
-    return (*seen + G_::NTOK - 1) / G_::NTOK + 1;
+    return (*seen + G_::NTOK - 1) / G_::NTOK + kItemSteps;
   }
   template <class G_>
   __device__ int units(const AttnArgs& a) const {       // of one kv head
-    int s = 0, v;
-    for (int i = 0; i < nrt; ++i) s += steps_of<G_>(a, i, &v);
+    // steps_of of every tile, its last row's token counted up instead of divided out
+    const int dq = kRows / a.G, dr = kRows - dq * a.G;
+    int s = 0, last = -1, rem = a.G - 1;                 // row -1: token -1, its last row
+    for (int i = 0; i < nrt; ++i) {
+      last += dq, rem += dr;
+      if (rem >= a.G) rem -= a.G, ++last;
+      const int seen = max(0, L - n + min(n - 1, last) + 1);
+      s += (seen + G_::NTOK - 1) / G_::NTOK + kItemSteps;
+    }
     return s;
   }
   template <class G_>
@@ -126,11 +137,11 @@ struct Segment {
   bool skip, whole, starts;
   bool two;             // the second row tile has rows
   __device__ Segment(const Item& it, const AttnArgs& a, int u, int u0, int u1) {
-    const int ib = u - it.step, real = it.steps - 1;
+    const int ib = u - it.step, real = it.steps - kItemSteps;
     k0 = it.step;
     count = max(0, min(real, k0 + u1 - u) - k0);
-    skip = real > 0 && count == 0;                       // only the empty step is left
     starts = ib >= u0;
+    skip = count == 0 && (real > 0 || !starts);                       // only empty steps are left
     whole = starts && ib + max(1, real) <= u1;
     two = (long long)it.n * a.G > (long long)it.rt * kRows + 128;
   }
@@ -228,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     it.request<G_>(a);
     return a.kv_heads * it.units<G_>(a);
   });
+  sm100::grid_launch_dependents();                       // the other kernel fills SMs as they end
   const int cta = blockIdx.x, ctas = min((int)gridDim.x, U);
   if (cta >= ctas) {
     if (tid == 0) a.desc[cta * kDescInts] = 0;
@@ -515,7 +527,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
       __half* op = a.out + (in ? (int64_t)tokq * a.o_ts + (int64_t)head * a.o_hs : 0);
       float* slot = a.part + (size_t)(cta * 2 + (sg.starts ? 1 : 0)) * (kRows * (D + 2));
       const int srow = T * 128 + rloc;
-#pragma unroll
+      // 32 channels at a time through the warp's rows of the Q tile, whose products are done,
+      // so that eight lanes store a row's 128 (64) bytes
+      const uint32_t mine_smem = qs_base + (warp & 3) * 4096;
+      const uint32_t out_rows = __ballot_sync(0xffffffffu, in);
+#pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
 #pragma unroll
@@ -524,23 +540,35 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
           sm100::tmem_ld_32x32b_x32(tO + 32 * c, o);
           sm100::tmem_ld_wait();
         }
-        float f[32];
-        const float m = pm[c * 32 / GROUP];
+        float m = pm[0];
 #pragma unroll
-        for (int j = 0; j < 32; ++j)                     // odd channels' codes entered times 2^-20
-          f[j] = fmaf(__uint_as_float(o[j]), (j & 1) ? 1048576.f : 16777216.f, m);
-        if (!sg.whole) {
+        for (int g = 1; g < NG; ++g) m = c * 32 / GROUP == g ? pm[g] : m;
+        const float mul = sg.whole ? inv : 1.f;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(slot + (size_t)srow * D + 32 * c + j) =
-                make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
-        } else if (in) {
+        for (int j = 0; j < 32; j += 4) {                // odd channels' codes entered times 2^-20
+          float f[4];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint2*>(op + 32 * c + j) =
-                make_uint2(h2_as_u32(__floats2half2_rn(f[j] * inv, f[j + 1] * inv)),
-                           h2_as_u32(__floats2half2_rn(f[j + 2] * inv, f[j + 3] * inv)));
+          for (int e = 0; e < 4; ++e)
+            f[e] = fmaf(__uint_as_float(o[j + e]), (e & 1) ? 1048576.f : 16777216.f, m) * mul;
+          sm100::st_shared_v4(mine_smem + swz(lane, j / 4), __float_as_uint(f[0]), __float_as_uint(f[1]),
+                              __float_as_uint(f[2]), __float_as_uint(f[3]));
         }
+        __syncwarp();
+        const int ch = 32 * c + 4 * (lane & 7);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = 4 * i + lane / 8;
+          const uint4 v = sm100::ld_shared_v4(mine_smem + swz(r, lane & 7));
+          const __half* rp = reinterpret_cast<const __half*>(__shfl_sync(0xffffffffu, (unsigned long long)op, r));
+          if (!sg.whole)
+            *reinterpret_cast<uint4*>(slot + (size_t)(T * 128 + (warp & 3) * 32 + r) * D + ch) =
+                v;
+          else if ((out_rows >> r) & 1)
+            *reinterpret_cast<uint2*>(const_cast<__half*>(rp) + ch) =
+                make_uint2(h2_as_u32(__floats2half2_rn(__uint_as_float(v.x), __uint_as_float(v.y))),
+                           h2_as_u32(__floats2half2_rn(__uint_as_float(v.z), __uint_as_float(v.w))));
+        }
+        __syncwarp();
       }
       if (!sg.whole) {
         slot[kRows * D + srow] = M;
@@ -759,7 +787,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
-  sm100::grid_launch_dependents();
   if (tid == 0) {
     // the item that starts here and goes on in the next CTAs, if there is one
     int* d = a.desc + cta * kDescInts;
@@ -768,7 +795,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     for (int u = u0; u < u1; u += x.steps - x.step, x.next<G_>(a)) {
       const Segment sg(x, a, u, u0, u1);
       if (!sg.whole && sg.starts) {
-        const int end = u - x.step + max(1, x.steps - 1);     // past the last step with tokens
+        const int end = u - x.step + max(1, x.steps - kItemSteps);     // past the last step with tokens
         span = (int)(((double)end * ctas - 1.0) / U) - cta + 1;
         d[1] = x.q0, d[2] = x.rt * kRows, d[3] = x.n * a.G, d[4] = x.h;
       }
@@ -779,31 +806,47 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
 }
 
 // Joins an item that crosses CTAs: block (c, y) takes rows [8 y, 8 y + 8) of the item that
-// starts in CTA c, over the slots of CTAs c .. c + span - 1 in order, 32 lanes a row.
+// starts in CTA c, over the slots of CTAs c .. c + span - 1, a warp a row.  Lanes read 32
+// parts' statistics at once and then their channels of one part after the other; the loads of
+// eight parts are under way together (latency is all this kernel costs).
 template <int D>
 __global__ void __launch_bounds__(256) kv4_prefill_merge(const AttnArgs a) {
   sm100::grid_dependency_wait();
-  const int cta = blockIdx.x, tid = threadIdx.x;
+  const int cta = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
   const int* d = a.desc + cta * kDescInts;
   const int span = d[0];
   if (span == 0) return;
-  const int r = blockIdx.y * 8 + tid / 32, ch = (tid & 31) * (D / 32), row = d[2] + r;
+  const int r = blockIdx.y * 8 + tid / 32, ch = lane * (D / 32), row = d[2] + r;
   if (row >= d[3]) return;
   constexpr size_t kSlot = (size_t)kRows * (D + 2);
   auto part = [&](int k) { return a.part + (size_t)((cta + k) * 2 + (k == 0)) * kSlot; };
   float m = -CUDART_INF_F;
-  for (int k = 0; k < span; ++k) m = fmaxf(m, part(k)[kRows * D + r]);
-  float o[D / 32] = {}, l = 0.f;
-  for (int k = 0; k < span; ++k) {
-    const float* p = part(k);
-    const float mk = p[kRows * D + r], f = mk == m ? 1.0f : ex2(mk - m);
-    l = fmaf(f, p[kRows * D + kRows + r], l);
+  for (int k = lane; k < span; k += 32) m = fmaxf(m, part(k)[kRows * D + r]);
 #pragma unroll
-    for (int j = 0; j < D / 32; j += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(p + (size_t)r * D + ch + j);
-      o[j] = fmaf(f, v.x, o[j]), o[j + 1] = fmaf(f, v.y, o[j + 1]);
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float o[D / 32] = {}, l = 0.f;
+  for (int k0 = 0; k0 < span; k0 += 32) {
+    float f = 0.f;
+    if (k0 + lane < span) {
+      const float* p = part(k0 + lane);
+      const float mk = p[kRows * D + r];
+      f = mk == m ? 1.0f : ex2(mk - m);
+      l = fmaf(f, p[kRows * D + kRows + r], l);
+    }
+    const int n = min(32, span - k0);
+#pragma unroll 8
+    for (int k = 0; k < n; ++k) {
+      const float* p = part(k0 + k) + (size_t)r * D + ch;
+      const float fk = __shfl_sync(0xffffffffu, f, k);
+#pragma unroll
+      for (int j = 0; j < D / 32; j += 2) {
+        const float2 v = *reinterpret_cast<const float2*>(p + j);
+        o[j] = fmaf(fk, v.x, o[j]), o[j + 1] = fmaf(fk, v.y, o[j + 1]);
+      }
     }
   }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   __half* op = a.out + (int64_t)(d[1] + row / a.G) * a.o_ts + (int64_t)(d[4] * a.G + row % a.G) * a.o_hs + ch;
 #pragma unroll
@@ -820,18 +863,7 @@ cudaError_t launch_geo(const AttnArgs& a, int num_sms, cudaStream_t stream) {
   });
   if (attr != cudaSuccess) return attr;
   kv4_prefill_kernel<G_><<<num_sms, kThreads, G_::SMEM, stream>>>(a);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(num_sms, kRows / 8, 1);
-  cfg.blockDim = dim3(256, 1, 1);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_prefill_merge<D>, a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -844,6 +876,11 @@ cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, int head_dim, int group, 
   if (head_dim == 128 && group == 64) return launch_geo<128, 64>(a, num_sms, stream);
   if (head_dim == 128 && group == 128) return launch_geo<128, 128>(a, num_sms, stream);
   return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_kv4_prefill_merge(const kv4::AttnArgs& a, int head_dim, int num_sms, cudaStream_t stream) {
+  return kv4::launch_overlapped(head_dim == 64 ? kv4_prefill_merge<64> : kv4_prefill_merge<128>,
+                                dim3(num_sms, kRows / 8), 256, 0, stream, a);
 }
 
 }  // namespace awq
