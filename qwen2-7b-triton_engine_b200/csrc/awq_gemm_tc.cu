@@ -130,7 +130,8 @@ struct TcArgs {
 };
 
 // A call of its own, its array in local memory: inlined, the activations' temporaries made
-// the kernel spill in its main loop (down at M = 2048: 307 us against 207 for the product).
+// the kernel spill in its main loop (K = 18944, N = 3584, M = 2048: 307 us, against 219
+// for the product alone).
 __device__ __noinline__ void activate32(float* v, int act) {
 #pragma unroll 1
   for (int j = 0; j < 32; ++j) v[j] = activate(v[j], act);

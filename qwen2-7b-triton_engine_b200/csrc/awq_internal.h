@@ -225,12 +225,13 @@ struct Kv4AttnCall {
   void* workspace;
 };
 // Query rows per kv head (tokens x heads of a group) from which a request runs on the tcgen05
-// kernel, and the rows of one of that kernel's items: a request that fills an item.  Measured
-// on B200 (us, mma.sync kernel / tcgen05 kernel): 8 requests of 4096 tokens, 28 / 4 heads, 168
-// rows 75 / 85, 224 rows 89 / 87, 448 rows 159 / 152; of 512 tokens, 224 rows 41 / 43, 448 rows
-// 70 / 58; one request of 4096 tokens, 224 rows 25 / 44, 896 rows 55 / 60; 8 requests of 4096
-// tokens, 8 / 8 heads, 64 rows 68 / 148, 128 rows 113 / 153.
-constexpr int kKv4PrefillMinRows = 256, kKv4PrefillRows = 256;
+// kernel, and the rows of one of that kernel's items.  Measured on B200 (us, mma.sync kernel /
+// tcgen05 kernel), 28 / 4 heads: 8 requests of 4096 tokens, 112 rows 57 / 56, 168 rows 78 / 62,
+// 224 rows 99 / 64, 448 rows 177 / 95; of 512 tokens, 168 rows 29 / 37, 224 rows 33 / 38, 448
+// rows 52 / 45; one request of 4096 tokens, 224 rows 26 / 47, 448 rows 36 / 45, 896 rows 57 / 48.
+// The kernels cross between 112 rows, where the SMs are full, and 500, where they are not; the
+// cached lengths that tell the two apart are on the device.
+constexpr int kKv4PrefillMinRows = 192, kKv4PrefillRows = 256;
 size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms);
 cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,
                                  cudaStream_t stream);

@@ -9,7 +9,9 @@
 // subnormals, one AND per two codes), and scales and minima are applied per token in fp32.
 // The odd codes of a word sit four bits higher, times 2^-20; the queries they meet are scaled
 // by 1/16 for it, after an item's queries are scaled up together by a power of two so that
-// the largest lies just below fp16's limit and nothing that matters becomes subnormal.
+// the largest lies just below fp16's limit and nothing that matters becomes subnormal.  Of the
+// values' codes one product takes the even ones and one whole bytes, even + 16 odd; the odd sum
+// is their difference over 16, exact to fp32's rounding.
 // The softmax reference M runs over log2(p s) rather than log2(p), so that the fp16 weights
 // stay below 2^8 and near the top of the range whatever the size of the value scales; sums,
 // statistics and accumulators are fp32.
@@ -25,6 +27,12 @@
 // fills all rings with bulk copies, each of its lanes one (no CTA barrier in the loop).  Items
 // that cross warps are joined in the CTA at its end; items that cross CTAs by
 // kv4_merge_kernel, in CTA order, so results do not depend on timing.
+//
+// Bound: for large batches the logic pipe (unpacking: two ANDs, a shift and two permutations per
+// eight codes, at half rate) and then the cache's bytes, for few tokens latency.  Measured on
+// B200, 48 requests of 1 to 16384 tokens, 28 / 4 heads of 128 channels in groups of 64: 49 us
+// (176 MB, 3.6 TB/s, 55 % of a copy's rate); 64-token tiles start within 4 us and the joins take
+// 6.  One request of 1000 tokens: 12.5 us.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -661,7 +669,8 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
 }
 
 // Joins an item that crosses CTAs: block (c, col) sums column col of the item that starts in
-// CTA c, over the slots of CTAs c .. c + span - 1, in four (eight) interleaved groups.
+// CTA c, over the slots of CTAs c .. c + span - 1, in four (eight) interleaved groups.  Latency
+// is its cost: 2 us behind the attention kernel's end, whose tail hides the launch.
 template <int D>
 __global__ void __launch_bounds__(128) kv4_merge_kernel(const AttnArgs a) {
   constexpr int LANES = D / 4, GROUPS = 128 / LANES;

@@ -7,8 +7,11 @@
 // lose nothing: |pos * inv_freq / 2 pi| keeps 53 bits before the whole turns go, and the
 // fp32 remainder is exact to 2^-25 of a turn.
 //
-// Bound: HBM.  One block per token: `half` threads make the token's sines and cosines once
-// for all heads, then every thread turns pairs in 16-byte pieces.
+// Bound: HBM.  One block for four neighbouring tokens: it makes their sines and cosines once
+// for all heads, then every thread turns pairs in 16-byte pieces, with its first loads under way
+// while the angles are made.  8191 tokens, 28 + 4 heads of 128 channels: 26 us on B200 (134 MB,
+// 5.2 TB/s, 79 % of a copy's rate); with the loads behind the angles 31 us.  Eight tokens: 4.3
+// us, a launch and the reduction of the angles.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
