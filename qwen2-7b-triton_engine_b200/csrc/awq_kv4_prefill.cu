@@ -7,7 +7,7 @@
 //   S_g [128 x NTOK] = Q_g [128 x group] . C_g^T      codes as fp16 integers (subnormals)
 //   x = scale sum_g (s_tg S_g + m_tg sum q_g)          fp32, one thread per query row
 //   P_g = fp16(2^(x - M) v_tg)                         value scales, reference M as there
-//   O_g [128 x group] += P_g . C'_g
+//   O_g [128 x group] += P_g . (C'_g - 8)
 // so keys and values are never rounded: scales and minima are applied in fp32.  One group
 // (NG = 1) is a plain flash step of 128 tokens; more groups trade tokens for accumulators, so
 // that S always takes 128 columns of tensor memory, P 64 of them (over S, once it is read)
@@ -23,7 +23,7 @@
 // cross CTAs are joined by kv4_prefill_merge in CTA order.
 //
 // Bound: the softmax warps' latency.  Measured on B200, four requests of 1 to 1024 query tokens
-// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 344 us, 0.52 PFLOP/s; a step of 256
+// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 338 us, 0.53 PFLOP/s; a step of 256
 // rows x 128 tokens takes 3.4 us, of which the MMAs need 1.1, the exponentials 1.1 and the
 // operand traffic in shared memory 1.4; no pipe is busier than 38 %.  A tile waits a third of
 // the time for its S, which shares tensor memory with its P: 512 columns hold two tiles of S
@@ -53,10 +53,12 @@ using kv4::kPrefixEntries;
 
 constexpr int kThreads = 512;
 constexpr int kRows = kKv4PrefillRows;   // 256: query rows of an item, two tiles of 128
-constexpr int kKvSlots = 3, kRawStages = 2, kParStages = 2;
+// One stage of raw blocks is enough, as the unpacking warps hold a step's in registers; the
+// room is better spent on a fourth operand slot (338 us; two stages and three slots 361 us).
+constexpr int kKvSlots = 4, kRawStages = 1, kParStages = 2;
 // Empty steps of an item, for its fixed cost (queries, first and last step, result).  Four
 // requests of 1024 query and up to 8192 cached tokens, 28 / 4 heads: 1 375 us, 2 368 us, 4 360 us
-// with a result that took 6 us; with today's 2 345 us, 3 344 us.
+// with a result that took 6 us; with today's 2 345 us, 3 344 us (three operand slots).
 constexpr int kItemSteps = 3;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
@@ -81,8 +83,21 @@ struct Geo {
   static_assert(SMEM <= 227 * 1024 && QTILE % 1024 == 0 && SLOT % 1024 == 0 && RAW % 16 == 0 &&
                     PAR % 16 == 0, "shared memory");
 };
-enum Bar { RAW_FULL = 0, RAW_EMPTY = 2, KV_FULL = 4, KV_EMPTY = 7, PAR_FULL = 10, PAR_EMPTY = 12,
-           Q_READY = 14, S_FULL = 16, P_READY = 18, O_FULL = 20, DRAIN = 22, NBARS = 23 };
+enum Bar {
+  RAW_FULL = 0,
+  RAW_EMPTY = RAW_FULL + kRawStages,
+  KV_FULL = RAW_EMPTY + kRawStages,
+  KV_EMPTY = KV_FULL + kKvSlots,
+  PAR_FULL = KV_EMPTY + kKvSlots,
+  PAR_EMPTY = PAR_FULL + kParStages,
+  Q_READY = PAR_EMPTY + kParStages,
+  S_FULL = Q_READY + 2,
+  P_READY = S_FULL + 2,
+  O_FULL = P_READY + 2,
+  DRAIN = O_FULL + 2,
+  NBARS = DRAIN + 1
+};
+static_assert(NBARS * 8 <= 256, "barriers");
 
 // A request's items: nrt row tiles of 256 per kv head, each with its causal number of steps
 // and kItemSteps empty ones that stand for its fixed cost.
@@ -233,10 +248,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     s_abort = 0;
     for (int i = 0; i < NBARS; ++i) {
       int count = 1;                                     // bulk copies, MMA commits
-      if (i >= RAW_EMPTY && i < RAW_EMPTY + 2) count = 128;
-      if (i >= KV_FULL && i < KV_FULL + 3) count = 128;
-      if (i >= PAR_FULL && i < PAR_FULL + 2) count = 128;
-      if (i >= PAR_EMPTY && i < PAR_EMPTY + 2) count = 256;
+      if (i >= RAW_EMPTY && i < RAW_EMPTY + kRawStages) count = 128;
+      if (i >= KV_FULL && i < KV_FULL + kKvSlots) count = 128;
+      if (i >= PAR_FULL && i < PAR_FULL + kParStages) count = 128;
+      if (i >= PAR_EMPTY && i < PAR_EMPTY + kParStages) count = 256;
       if (i >= Q_READY && i < Q_READY + 2) count = 128;
       if (i >= P_READY && i < P_READY + 2) count = 128;
       sm100::mbar_init(bars + 8 * i, count);
@@ -623,11 +638,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         const float2 kp = __half22float2(reinterpret_cast<const __half2*>(pblk + kv4::off_kp(D))[(ptok % 16) * NG + pg]);
         const float2 vp = __half22float2(reinterpret_cast<const __half2*>(pblk + kv4::off_vp(D, GROUP))[(ptok % 16) * NG + pg]);
         const int ok = raw_ok[rs];
+        sm100::mbar_arrive(bar(RAW_EMPTY + rs));         // all that is needed is in registers
         if (n >= kParStages && !(live = wait(PAR_EMPTY + ps, (n / kParStages - 1) & 1))) break;
         {
           float* par = reinterpret_cast<float*>(smem + G_::OFF_PAR + ps * PAR);
           par[pg * NTOK + ptok] = kp.x, par[128 + pg * NTOK + ptok] = kp.y;
-          par[256 + pg * NTOK + ptok] = vp.x, par[384 + pg * NTOK + ptok] = vp.y;
+          par[256 + pg * NTOK + ptok] = vp.x, par[384 + pg * NTOK + ptok] = fmaf(8.f, vp.x, vp.y);
           float big = fmaxf(vp.x, 5.9604645e-8f);        // 2^-24, fp16's least scale
 #pragma unroll
           for (int o = 1; o < NG; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
@@ -657,7 +673,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         sm100::fence_proxy_async_smem();
         sm100::mbar_arrive(bar(KV_FULL + slot));
         ++kv;
-        // V: rows of channels
+        // V: rows of channels, codes less 8 (the odd ones times 16)
+        auto lo = [](uint32_t w) { return hsub2_u32(w & kLoMask, 0x00080008u); };
+        auto hi = [](uint32_t w) { return hsub2_u32(w & kHiMask, 0x00800080u); };
         slot = kv % kKvSlots;
         if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
         dst = sbase + G_::OFF_KV + slot * G_::SLOT + (run / 8) * (D * 128);
@@ -666,14 +684,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
           for (int j = 0; j < D / 32; ++j) {
             const int ch = 4 * (8 * j + h8);             // first of the quad's channels
             const uint32_t a0 = vw[0][j], a1 = vw[1][j], a2 = vw[2][j], a3 = vw[3][j];
-            sm100::st_shared_v4(dst + swz(ch, run & 7), a0 & kLoMask, a1 & kLoMask, a2 & kLoMask, a3 & kLoMask);
-            sm100::st_shared_v4(dst + swz(ch + 1, run & 7), a0 & kHiMask, a1 & kHiMask, a2 & kHiMask, a3 & kHiMask);
+            sm100::st_shared_v4(dst + swz(ch, run & 7), lo(a0), lo(a1), lo(a2), lo(a3));
+            sm100::st_shared_v4(dst + swz(ch + 1, run & 7), hi(a0), hi(a1), hi(a2), hi(a3));
             const uint32_t b0 = a0 >> 8, b1 = a1 >> 8, b2 = a2 >> 8, b3 = a3 >> 8;
-            sm100::st_shared_v4(dst + swz(ch + 2, run & 7), b0 & kLoMask, b1 & kLoMask, b2 & kLoMask, b3 & kLoMask);
-            sm100::st_shared_v4(dst + swz(ch + 3, run & 7), b0 & kHiMask, b1 & kHiMask, b2 & kHiMask, b3 & kHiMask);
+            sm100::st_shared_v4(dst + swz(ch + 2, run & 7), lo(b0), lo(b1), lo(b2), lo(b3));
+            sm100::st_shared_v4(dst + swz(ch + 3, run & 7), hi(b0), hi(b1), hi(b2), hi(b3));
           }
         }
-        sm100::mbar_arrive(bar(RAW_EMPTY + rs));
         sm100::fence_proxy_async_smem();
         sm100::mbar_arrive(bar(KV_FULL + slot));
         ++kv;

@@ -12,8 +12,10 @@ Tolerances.  u16 = 2^-11 is half a step of fp16, u32 = 2^-24 of fp32.
   A, plus the hardware exponential's 2 ulp (2^-22).  A softmax weight p_t is then off by
   d_t = e_t + sum_t p_t e_t (its own error and the sum's), relative.  The weights p s are
   rounded to fp16: u16 relative, or, below fp16's normal range, half a subnormal step 2^-25
-  of the softmax reference, which is at most the largest p s.  Hence
-  |err| <= sum_t (p_t ((u16 + d_t) s c + d_t |m|) + 2^-25 max(p s) 15) + u16 |o| + 2^-25.
+  of the softmax reference, which is at most the largest p s.  The weights meet c - 8, and
+  p meets m + 8 s, in fp32 (rounded once, u32).  Hence
+  |err| <= sum_t (p_t ((u16 + d_t) s |c - 8| + (d_t + u32) |m + 8 s|) + 2^-25 max(p s) 15)
+           + u16 |o| + 2^-25.
 """
 from __future__ import annotations
 
@@ -269,10 +271,11 @@ def bound(q, K, V, ref, scale, data, slots, D, page, group):
             e = (D + 8) * U32 * size + 2.0 ** -22
             d = e + (p @ e)                             # of a weight, and of the sum
             sc = vs[:seen, hk]
-            c15 = np.abs(V[:seen, hk] - vm[:seen, hk])  # s c
+            mid = vm[:seen, hk] + 8 * sc
+            c8 = np.abs(V[:seen, hk] - mid)             # s |c - 8|
             w = p[:, None] * sc
             sub = (2.0 ** -25) * w.max() * np.where(sc > 0, 15.0, 0).max(-1, keepdims=True)
-            out[i, h] = (p[:, None] * ((U16 + d[:, None]) * c15 + d[:, None] * np.abs(vm[:seen, hk]))
+            out[i, h] = (p[:, None] * ((U16 + d[:, None]) * c8 + (d[:, None] + U32) * np.abs(mid))
                          + sub).sum(0)
     return out + U16 * np.abs(ref) + TINY
 
