@@ -237,7 +237,8 @@ AWQ_API int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64
  * block_table, and the query rows cu_q[r] .. cu_q[r + 1] (cu_q null: row r alone), which are
  * its last tokens: row i of n sees tokens 0 .. kv_lens[r] - n + i.  A row that sees no token
  * gives zeros.  Rows of out behind cu_q[requests] are left as they are.  max_q: most query
- * rows of a request (a hint for the choice of kernel).  Tokens in a page outside
+ * rows of a request (a hint for the choice of kernel: a wrong one costs time and
+ * may move roundings).  Tokens in a page outside
  * 0 .. num_pages - 1 are not seen, kv_lens is clipped to the table, a request whose cu_q is
  * not ascending within 0 .. tokens is left out, and where requests claim the same rows so often
  * that the list of work passes 2^31 nothing is computed; each sets status bit 2.  The workspace

@@ -306,8 +306,8 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
     block_table int32 [R, max_blocks], kv_lens int32 [R]: the tokens of each request in the
     cache, its new ones included.  Without cu_q, T = R and row r is request r's last token.
     With cu_q (int32 [R + 1]) request r has the rows cu_q[r] to cu_q[r + 1], its last tokens;
-    max_q says how many rows a request has at most (it chooses the kernel, no result depends
-    on it).  Query head h reads kv head h // (q_heads / kv_heads).  scale defaults to
+    max_q says how many rows a request has at most (it chooses the kernel; a wrong one costs
+    time and may move roundings).  Query head h reads kv head h // (q_heads / kv_heads).  scale defaults to
     head_dim ** -0.5.  Rows that see no token are zeros.  Rows behind cu_q[R] are left as they
     are in ``out`` and are zeros in a new tensor."""
     ext = _ext()

@@ -226,9 +226,9 @@ struct Kv4AttnCall {
 };
 // Query rows per kv head (tokens x heads of a group) from which a request runs on the tcgen05
 // kernel, and the rows of one of that kernel's items.  Measured on B200 (us, mma.sync kernel /
-// tcgen05 kernel), 28 / 4 heads: 8 requests of 4096 tokens, 112 rows 57 / 56, 168 rows 78 / 62,
-// 224 rows 99 / 64, 448 rows 177 / 95; of 512 tokens, 168 rows 29 / 37, 224 rows 33 / 38, 448
-// rows 52 / 45; one request of 4096 tokens, 224 rows 26 / 47, 448 rows 36 / 45, 896 rows 57 / 48.
+// tcgen05 kernel), 28 / 4 heads: 8 requests of 4096 tokens, 112 rows 61 / 56, 168 rows 83 / 62,
+// 224 rows 106 / 63, 448 rows 193 / 94; of 512 tokens, 168 rows 33 / 37, 224 rows 37 / 39, 448
+// rows 62 / 45; one request of 4096 tokens, 224 rows 27 / 45, 448 rows 38 / 46, 896 rows 60 / 48.
 // The kernels cross between 112 rows, where the SMs are full, and 500, where they are not; the
 // cached lengths that tell the two apart are on the device.
 constexpr int kKv4PrefillMinRows = 192, kKv4PrefillRows = 256;
