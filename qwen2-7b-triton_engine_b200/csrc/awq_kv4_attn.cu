@@ -32,8 +32,9 @@
 // that cross warps are joined in the CTA at its end; items that cross CTAs by
 // kv4_merge_kernel, in CTA order, so results do not depend on timing.
 //
-// Bound: for large batches the logic pipe (unpacking: two ANDs, a shift and two permutations per
-// eight codes, at half rate) and then the cache's bytes, for few tokens latency.  Measured on
+// Bound: for large batches the instructions of the 11 warps an SM's registers hold (45 % of the
+// issue slots, start and joins included; unpacking goes through the half-rate logic pipe, 31 %)
+// and then the cache's bytes, for few tokens latency.  Measured on
 // B200, 48 requests of 1 to 16384 tokens, 28 / 4 heads of 128 channels in groups of 64: 51 us
 // (176 MB, 3.5 TB/s, 53 % of a copy's rate; 47.6 us before the values' codes were centred); 64-token tiles start within 4 us and the joins take
 // 6.  One request of 1000 tokens: 12.5 us.
