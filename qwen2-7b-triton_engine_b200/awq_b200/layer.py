@@ -307,9 +307,9 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
     cache, its new ones included.  Without cu_q, T = R and row r is request r's last token.
     With cu_q (int32 [R + 1]) request r has the rows cu_q[r] to cu_q[r + 1], its last tokens;
     max_q says how many rows a request has at most (it chooses the kernel; a wrong one costs
-    time and may move roundings).  Query head h reads kv head h // (q_heads / kv_heads).  scale defaults to
-    head_dim ** -0.5.  Rows that see no token are zeros.  Rows behind cu_q[R] are left as they
-    are in ``out`` and are zeros in a new tensor."""
+    time and may move roundings).  Query head h reads kv head h // (q_heads / kv_heads).
+    scale defaults to head_dim ** -0.5.  Rows that see no token are zeros.  Rows behind cu_q[R]
+    are left as they are in ``out`` and are zeros in a new tensor."""
     ext = _ext()
     if ext is not None and _tensors(q, block_table, kv_lens, cu_q, out):
         return ext.kv4_attention(q, cache.data, cache.head_dim, cache.page_size, cache.group_size,
