@@ -23,7 +23,7 @@
 // cross CTAs are joined by kv4_prefill_merge in CTA order.
 //
 // Bound: the softmax warps' latency.  Measured on B200, four requests of 1 to 1024 query tokens
-// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 338 us, 0.53 PFLOP/s; a step of 256
+// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 344 us, 0.52 PFLOP/s; a step of 256
 // rows x 128 tokens takes 3.4 us, of which the MMAs need 1.1, the exponentials 1.1 and the
 // operand traffic in shared memory 1.4; no pipe is busier than 44 % (shared memory).  A tile waits a third of
 // the time for its S, which shares tensor memory with its P: 512 columns hold two tiles of S
@@ -54,7 +54,7 @@ using kv4::kPrefixEntries;
 constexpr int kThreads = 512;
 constexpr int kRows = kKv4PrefillRows;   // 256: query rows of an item, two tiles of 128
 // One stage of raw blocks is enough, as the unpacking warps hold a step's in registers; the
-// room is better spent on a fourth operand slot (338 us; two stages and three slots 361 us).
+// room is better spent on a fourth operand slot (the header's case: 6 % less time).
 constexpr int kKvSlots = 4, kRawStages = 1, kParStages = 2;
 // Empty steps of an item, for its fixed cost (queries, first and last step, result).  Four
 // requests of 1024 query and up to 8192 cached tokens, 28 / 4 heads: 1 375 us, 2 368 us, 4 360 us
@@ -309,7 +309,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
   sm100::tc_fence_after();
   const uint32_t tmem = s_tmem;
   auto bar = [&](int i) { return bars + 8 * i; };
-  // Waits end the CTA's work when they run out or when another role's has.
+  // A wait that runs out ends every later wait of the CTA at once.  The roles of one lane or
+  // warp stop there; the softmax and unpacking warps, whose lanes vote and shuffle, run through
+  // their remaining steps together, on whatever they find (the status says that the output is
+  // wrong).  A vote behind every wait instead costs 2 %: 351 us for 344 in the header's case.
   auto wait = [&](int b, uint32_t parity) {
     if (s_abort) return false;
     if (sm100::mbar_wait_bounded(bar(b), parity, a.status, kWaitNs)) return true;
@@ -326,8 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     const uint32_t tS = tmem + lanes + T * 128, tO = tmem + lanes + 256 + T * 128;
     const uint32_t qs_base = sbase + G_::OFF_Q + T * G_::QTILE;
     int np = 0, ns = 0, nq = 0;                          // steps, this tile's steps, segments
-    bool live = true;
-    for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+    for (int u = u0; u < u1; u += it.steps - it.step, it.next<G_>(a)) {
       const Segment sg(it, a, u, u0, u1);
       if (sg.skip) continue;
       const int row = it.rt * kRows + T * 128 + rloc;
@@ -388,12 +390,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
       const int lim_lo = it.L - it.n + (it.rt * kRows + T * 128) / a.G;   // all rows see these
       for (int k = 0; k < sg.count; ++k, ++np) {
         const int ps = np % kParStages;
-        if (!(live = wait(PAR_FULL + ps, (np / kParStages) & 1))) break;
+        wait(PAR_FULL + ps, (np / kParStages) & 1);
         if (!mine) {
           sm100::mbar_arrive(bar(PAR_EMPTY + ps));
           continue;
         }
-        if (!(live = wait(S_FULL + T, ns & 1))) break;
+        wait(S_FULL + T, ns & 1);
         ++ns;
         sm100::tc_fence_after();
         const int tok0 = (sg.k0 + k) * NTOK;
@@ -532,11 +534,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         sm100::tc_fence_before();
         sm100::mbar_arrive(bar(P_READY + T));
       }
-      if (!live) break;
       if (!mine) continue;
       // ---- the rows' result ------------------------------------------------------------------
       if (sg.count > 0) {
-        if (!(live = wait(O_FULL + T, nq & 1))) break;
+        wait(O_FULL + T, nq & 1);
         ++nq;
         sm100::tc_fence_after();
       }
@@ -606,12 +607,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
     sm100::setmaxnreg_dec<88>();
     const int i = tid - 256;
     int n = 0, kv = 0;                                   // steps, operand slots filled
-    bool live = true;
-    for (int u = u0; live && u < u1; u += it.steps - it.step, it.next<G_>(a)) {
+    for (int u = u0; u < u1; u += it.steps - it.step, it.next<G_>(a)) {
       const Segment sg(it, a, u, u0, u1);
       for (int k = 0; k < sg.count; ++k, ++n) {
         const int rs = n % kRawStages, ps = n % kParStages;
-        if (!(live = wait(RAW_FULL + rs, (n / kRawStages) & 1))) break;
+        wait(RAW_FULL + rs, (n / kRawStages) & 1);
         const uint8_t* raw = smem + G_::OFF_RAW + rs * G_::RAW;
         // every load of the step's raw blocks first: K rows by quads of lanes (a phase of eight
         // lanes has rows r and r ^ 5, which meet neither in banks nor in swizzled chunks), V
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         const float2 vp = __half22float2(reinterpret_cast<const __half2*>(pblk + kv4::off_vp(D, GROUP))[(ptok % 16) * NG + pg]);
         const int ok = raw_ok[rs];
         sm100::mbar_arrive(bar(RAW_EMPTY + rs));         // all that is needed is in registers
-        if (n >= kParStages && !(live = wait(PAR_EMPTY + ps, (n / kParStages - 1) & 1))) break;
+        if (n >= kParStages) wait(PAR_EMPTY + ps, (n / kParStages - 1) & 1);
         {
           float* par = reinterpret_cast<float*>(smem + G_::OFF_PAR + ps * PAR);
           par[pg * NTOK + ptok] = kp.x, par[128 + pg * NTOK + ptok] = kp.y;
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         }
         sm100::mbar_arrive(bar(PAR_FULL + ps));
         int slot = kv % kKvSlots;
-        if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
+        if (kv >= kKvSlots) wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1);
         uint32_t dst = sbase + G_::OFF_KV + slot * G_::SLOT;
         // K: rows of tokens
 #pragma unroll
@@ -677,7 +677,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         auto lo = [](uint32_t w) { return hsub2_u32(w & kLoMask, 0x00080008u); };
         auto hi = [](uint32_t w) { return hsub2_u32(w & kHiMask, 0x00800080u); };
         slot = kv % kKvSlots;
-        if (kv >= kKvSlots && !(live = wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1))) break;
+        if (kv >= kKvSlots) wait(KV_EMPTY + slot, (kv / kKvSlots - 1) & 1);
         dst = sbase + G_::OFF_KV + slot * G_::SLOT + (run / 8) * (D * 128);
         if (i < NTOK) {
 #pragma unroll
