@@ -194,7 +194,8 @@ AWQ_API int awq_rope_axes(const void* q, int64_t q_token_stride, int64_t q_head_
  * awq_kv4_append quantizes k and v ([tokens][kv_heads][head_dim], last dimension dense) into
  * their slots.  A negative slot is skipped; one past the cache is skipped and sets status
  * bit 2 (awq_device_status).  The slots of one call must differ.  awq_kv4_gather reads slots
- * back as dense fp16 [tokens][kv_heads][head_dim] (a negative or bad slot as zeros).
+ * back as dense fp16 [tokens][kv_heads][head_dim] (a negative or bad slot as zeros); out_k
+ * and out_v must be 16-byte aligned.
  */
 AWQ_API size_t awq_kv4_page_bytes(int64_t kv_heads, int64_t head_dim, int64_t group_size,
                                   int64_t page_size);

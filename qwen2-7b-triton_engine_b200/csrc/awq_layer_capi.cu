@@ -88,8 +88,8 @@ int awq_kv4_gather(const void* cache, int64_t num_pages, int64_t kv_heads, int64
   if (tokens < 0 || tokens > (int64_t)1 << 31) return fail(AWQ_ERR_INVALID_ARG, "tokens=%lld out of range", (long long)tokens);
   if (tokens == 0) return AWQ_OK;
   if (!cache || !slots || !out_k || !out_v) return fail(AWQ_ERR_INVALID_ARG, "null cache, slots or output");
-  if (!aligned(cache, 16) || !aligned(slots, 8) || !aligned(out_k, 8) || !aligned(out_v, 8))
-    return fail(AWQ_ERR_INVALID_ARG, "cache must be 16-byte, slots and the outputs 8-byte aligned");
+  if (!aligned(cache, 16) || !aligned(slots, 8) || !aligned(out_k, 16) || !aligned(out_v, 16))
+    return fail(AWQ_ERR_INVALID_ARG, "cache, out_k and out_v must be 16-byte, slots 8-byte aligned");
   int sms = 0, *status = nullptr;
   if ((rc = awq::device_context(&sms, &status))) return rc;
   const cudaError_t e = awq::launch_kv4_gather(c, cache, slots, tokens, out_k, out_v, sms, status,

@@ -87,6 +87,13 @@ def test_gather_entry_refusals():
     assert _gather(k=P + 4) == INV and _gather(v=None) == INV and _gather(T=0, k=None, v=None) == 0
 
 
+def test_gather_entry_refuses_outputs_its_stores_do_not_fit():
+    """The kernel stores 16 bytes at a time."""
+    for off in (2, 8):
+        assert _gather(k=P + off) == INV and _gather(v=P + off) == INV
+    assert "16-byte" in (_gather(k=P + 8), _lib.load().awq_last_error().decode())[1]
+
+
 def _attention(q=P, q_ts=128, T=4, H=4, cache=P, Hk=2, D=64, table=P, stride=8, width=8, lens=P,
                cu=None, R=4, max_q=1, scale=0.1, out=P, o_ts=256, ws=P, nb=1 << 40, page=16):
     return _lib.load().awq_kv4_attention(q, q_ts, 64, T, H, cache, 4, Hk, D, 64, page, table, stride,
