@@ -408,7 +408,7 @@ cudaError_t launch_gemv(const GemvPlan& plan, const void* x, int64_t ldx, const 
                         const void* bias, const EpiArgs* epi) {
   GemvArgs a;
   a.bias = static_cast<const __half*>(bias);
-  a.residual = epi ? static_cast<const __half*>(epi->residual) : nullptr;
+  const __half* residual = epi ? static_cast<const __half*>(epi->residual) : nullptr;
   a.ldr = epi ? epi->ldr : 0;
   a.act = epi ? epi->act : kActNone;
   a.ldx = ldx;
@@ -426,6 +426,7 @@ cudaError_t launch_gemv(const GemvPlan& plan, const void* x, int64_t ldx, const 
     const int64_t mrows = (M - m0 < rows_per_launch) ? (M - m0) : rows_per_launch;
     a.x = static_cast<const __half*>(x) + m0 * ldx;
     a.out = static_cast<__half*>(out) + m0 * ldo;
+    a.residual = residual ? residual + m0 * a.ldr : nullptr;
     a.M = (int)mrows;
     const int z = (int)((mrows + 15) / 16);
     switch (plan.toksets) {

@@ -155,3 +155,28 @@ def test_graphs_replay_at_the_same_time(cuda):
     torch.cuda.synchronize()
     for _, out in graphs:
         assert torch.equal(out, want)
+
+
+def test_residual_where_the_generic_kernel_takes_several_launches(cuda):
+    """N % 32 != 0 and more 16-token chunks than one launch has counters for: 148 column strips,
+    so 110 chunks a launch, and the last 40 rows in a second one."""
+    M, K, N, gs = 1800, 64, 37880, 64
+    first = 16384 // -(-N // 256) * 16
+    assert first == 1760
+    x, qw, qz, s, bias, _ = make(M, K, N, gs, seed=8)
+    rd = (2 * torch.randn((M, N), device="cuda", generator=torch.Generator("cuda").manual_seed(9))).half()
+    xd, qwd, qzd, sd, bd = dev(x, qw, qz, s, bias)
+    rows = [*range(8), *range(first - 8, M)]
+    y, S = product(x[rows], qw, qz, s, gs)
+    res = rd[rows].cpu().numpy()
+    out = awq_b200.gemm_epilogue(xd, qwd, qzd, sd, gs, bias=bd, activation="relu", residual=rd)
+    check(out[rows], y, S, M, K, bias, "relu", res)
+    # a residual of wider rows, and the residual stream in place
+    want = awq_b200.gemm_epilogue(xd, qwd, qzd, sd, gs, residual=rd)
+    check(want[rows], y, S, M, K, None, "none", res)
+    wide = torch.zeros((M, N + 8), dtype=torch.float16, device="cuda")
+    wide[:, :N] = rd
+    assert torch.equal(awq_b200.gemm_epilogue(xd, qwd, qzd, sd, gs, residual=wide[:, :N]), want)
+    awq_b200.gemm_epilogue(xd, qwd, qzd, sd, gs, residual=rd, out=rd)
+    assert torch.equal(rd, want)
+    assert awq_b200.device_status() == 0
