@@ -16,9 +16,10 @@
 // the largest lies just below fp16's limit and nothing that matters becomes subnormal.  Of the
 // values' codes one product takes the even ones and one whole bytes, even + 16 odd (each less
 // 8); the odd sum is their difference over 16, exact to fp32's rounding.
-// The softmax reference M runs over log2(p s) rather than log2(p), so that the fp16 weights
-// stay below 2^8 and near the top of the range whatever the size of the value scales; sums,
-// statistics and accumulators are fp32.
+// The softmax reference M runs over log2(p s) rather than log2(p), and lies 2^7 below the
+// largest, so that the fp16 weights stay below 2^15 and near the top of the range whatever the
+// size of the value scales (s is a token's largest: groups with scales up to 2^21 below it keep
+// all bits of their weights); sums, statistics and accumulators are fp32.
 //
 // Operand order: scores are computed transposed (tokens are the MMA's 16 rows, the query
 // rows of a kv head its 8 columns), as are the outputs (channels x query rows), so seven
@@ -446,8 +447,8 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
             ls[b][e] = lg2(top);
           }
         }
-        // the softmax reference moves only when it is more than 2^8 behind (the fp16 weights
-        // then reach 2^8 at most); -inf + 8 = -inf, so the first visible token sets it
+        // the softmax reference moves only when it is more than 2^8 behind (kBelowTop);
+        // -inf + 8 = -inf, so the first visible token sets it
         bool up = false;
         float nm[2];
 #pragma unroll
@@ -459,8 +460,8 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
           m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-          nm[c] = m;
-          up |= m > M[c] + 8.0f;
+          nm[c] = m - kv4::kBelowTop;
+          up |= nm[c] > M[c] + kv4::kMoveAt;
         }
         if (__any_sync(0xffffffffu, up)) {
           float f[2];

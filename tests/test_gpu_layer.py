@@ -518,3 +518,81 @@ def test_attention_prompt_graph_with_other_lengths(cuda):
         torch.cuda.synchronize()
         assert torch.equal(out[:new_cu[-1]], want[:new_cu[-1]])
     assert awq_b200.device_status() == 0
+
+
+# ---- attention: value scales close together and far apart, and tokens of little weight -------
+class Tokens:
+    """One request's keys and values as the cache holds them, in float64, from its definition."""
+
+    def __init__(self, k, v, group):
+        self.group = group
+        (kc, ks, km), (vc, vs, vm) = L.quantize(k, group), L.quantize(v, group)
+        self.K, self.V = L.values(kc, ks, km), L.values(vc, vs, vm)
+        rep = lambda x: np.repeat(x.astype(np.float64), group, -1)
+        self.ks, self.km, self.vs, self.vm = rep(ks), rep(km), rep(vs), rep(vm)
+        self.top = vs.astype(np.float64).max(-1).T      # [kv heads][tokens] largest value scale
+
+    def cached(self, k, v, rng, page):
+        """A cache with these tokens in shuffled pages, and its table."""
+        n, Hk, D = k.shape
+        need = -(-n // page)
+        cache = awq_b200.KV4Cache.allocate(need + 1, Hk, D, page, self.group)
+        table = rng.permutation(need + 1)[:need]
+        slots = table[np.arange(n) // page] * page + np.arange(n) % page
+        awq_b200.kv4_append(dev(k), dev(v), dev(slots), cache)
+        return cache, dev(table[None]).int()
+
+    def check(self, q, got, seen, lost, scale):
+        """A token's rows q, got [H, D] that see `seen` tokens, against the docstring's bound,
+        `lost` (of the largest p s) in the place of 2^-25."""
+        H, D = q.shape
+        q = q.astype(np.float64)
+        ref = L.attention(q[None], self.K[:seen], self.V[:seen], scale)[0]
+        for h in range(H):
+            hk = h // (H // self.K.shape[1])
+            K, ks, km, vs, vm = (x[:seen, hk] for x in (self.K, self.ks, self.km, self.vs, self.vm))
+            s = scale * (K @ q[h])
+            p = np.exp(s - s.max())
+            p /= p.sum()
+            e = (D + 8) * U32 * abs(scale) * ((15 * ks + np.abs(km)) @ np.abs(q[h])) + 2.0 ** -22
+            d = (e + p @ e)[:, None]
+            mid = vm + 8 * vs
+            sub = lost * (p[:, None] * vs).max() * np.where(vs > 0, 15.0, 0).max(-1, keepdims=True)
+            tol = (p[:, None] * ((U16 + d) * np.abs(self.V[:seen, hk] - mid) + (d + U32) * np.abs(mid))
+                   + sub).sum(0) + U16 * np.abs(ref[h]) + TINY
+            err = np.abs(got[h] - ref[h])
+            assert (err <= tol).all(), (seen, h, float((err / tol).max()))
+
+
+def ladder(rng, n, Hk, D, group, q0, drop, sizes):
+    """Keys whose scores against q = q0 in channel 0 fall below token 0's by `drop` [n] bits, and
+    values with codes 0 (a group's first channel) and 15, at the scales `sizes` [n]."""
+    bits = D ** -0.5 * np.log2(np.e) * q0
+    k, v = np.zeros((n, Hk, D)), np.zeros((n, Hk, D))
+    k[:, :, 0] = ((drop.max() + 1 - drop) / bits)[:, None]
+    v[:] = 15 * sizes[:, None, None]
+    v[:, :, ::group] = 0
+    return k.astype(np.float16), v.astype(np.float16)
+
+
+@pytest.mark.parametrize("D,group", [(64, 32), (128, 64), (128, 32)])
+@pytest.mark.parametrize("n,H", [(1, 1), (3, 4)])
+def test_attention_groups_of_unequal_scale(cuda, D, group, n, H):
+    """The first group's value scales are 2^22 times the others', and every eighth token weighs
+    2^0.55 times the rest, so that a weight rounded to the fourth of itself would show.  Where
+    all tokens have one scale the softmax reference lies 2^7 below the largest p s: a weight is
+    off by 2^-32 of that at most."""
+    rng = np.random.default_rng(D + n)
+    Lk = 300
+    drop = np.where(np.arange(Lk) % 8 == 0, 0, 0.55)
+    k, v = ladder(rng, Lk, 1, D, group, 8.0, drop, np.full(Lk, 2.0 ** -12))
+    v[:, :, :group] = (v[:, :, :group].astype(np.float64) * 2.0 ** 22).astype(np.float16)
+    tok = Tokens(k, v, group)
+    assert (tok.vs[:, 0, :group] == 2.0 ** 10).all() and (tok.vs[:, 0, group:] == 2.0 ** -12).all()
+    cache, table = tok.cached(k, v, rng, 64)
+    q = np.zeros((n, H, D), np.float16)
+    q[:, :, 0] = 8
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev([Lk]).int(), dev([0, n]).int(), n)
+    got = got.double().cpu().numpy()
+    for i in {0, n - 1}:
+        tok.check(q[i], got[i], Lk - n + i + 1, 2.0 ** -32, D ** -0.5)
