@@ -60,6 +60,7 @@ constexpr int kKvSlots = 4, kRawStages = 1, kParStages = 2;
 // requests of 1024 query and up to 8192 cached tokens, 28 / 4 heads: 1 375 us, 2 368 us, 4 360 us
 // with a result that took 6 us; with today's 2 345 us, 3 344 us (three operand slots).
 constexpr int kItemSteps = 3;
+constexpr float kMaxSpread = 128.f;      // 2^kBelowTop
 constexpr uint64_t kWaitNs = 2000000000ull;
 
 template <int D_, int GROUP_>
@@ -403,8 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
         const float* par = reinterpret_cast<const float*>(smem + G_::OFF_PAR + ps * PAR);
         const float* ls = par + 512;
         // One step.  SLOW: some of its tokens may be unseen (past a row's limit, or in a page
-        // the table does not name), or their value scales differ by more than 2^8, so that
-        // the reference has to look at every token's scale instead of the step's largest.
+        // the table does not name), or their value scales differ by more than 2^kBelowTop, so
+        // that the reference has to look at every token's scale: with the step's largest in
+        // their place it lies up to their spread too high, and never above the largest p s.
         const float4 hi4 = *reinterpret_cast<const float4*>(ls + NTOK);
         const float4 lo4 = *reinterpret_cast<const float4*>(ls + NTOK + 4);
         const float v_hi = fmaxf(fmaxf(hi4.x, hi4.y), fmaxf(hi4.z, hi4.w));
@@ -462,8 +464,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
           }
         }
         if constexpr (!SLOW) top = fmaf(top, ksc, lg2(v_hi));
+        top -= kv4::kBelowTop;
         // the reference moves when it is more than 2^8 behind
-        if (__any_sync(0xffffffffu, top > M + 8.0f)) {
+        if (__any_sync(0xffffffffu, top > M + kv4::kMoveAt)) {
           const float m = fmaxf(M, top), f = M == m ? 1.0f : ex2(M - m);
           M = m;
           const F2 f2 = pack2(f, f);
@@ -525,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const AttnArgs
           for (int g = 0; g < NG; ++g) sm100::tmem_st_32x32b<PT / 2>(tS + g * NTOK + c * (PT / 2), w[g]);
         }
         };
-        if (tok0 + NTOK - 1 > lim_lo || ok != (1 << NBLK) - 1 || !(v_hi <= 256.f * v_lo))
+        if (tok0 + NTOK - 1 > lim_lo || ok != (1 << NBLK) - 1 || !(v_hi <= kMaxSpread * v_lo))
           softmax_step(std::true_type{});
         else
           softmax_step(std::false_type{});

@@ -564,6 +564,31 @@ class Tokens:
             assert (err <= tol).all(), (seen, h, float((err / tol).max()))
 
 
+@pytest.mark.parametrize("D,group,H,Hk", [(128, 128, 7, 1), (128, 64, 8, 2), (128, 32, 4, 4),
+                                          (64, 64, 14, 2), (64, 32, 2, 1)])
+@pytest.mark.parametrize("spread", [0, 4])
+def test_attention_prompt_values_of_one_size(cuda, D, group, H, Hk, spread):
+    """Values whose scales lie within 2^7 of one another in every step of 128 / groups tokens,
+    over 3000 cached tokens, so that most steps are all seen and take the tcgen05 kernel's
+    shorter form."""
+    rng = np.random.default_rng(D + group + spread)
+    n = -(-300 * Hk // H)
+    Lk = 3000 + n
+    k = (rng.standard_normal((Lk, Hk, D)) + 4 * (rng.random((1, Hk, D)) < 0.05)).astype(np.float16)
+    v = (rng.standard_normal((Lk, Hk, D)) * np.exp2(rng.uniform(0, spread, (Lk, Hk, 1)))).astype(np.float16)
+    tok = Tokens(k, v, group)
+    step = 128 * group // D
+    steps = tok.top[:, :Lk // step * step].reshape(Hk, -1, step)
+    assert (steps.max(-1) <= 128 * steps.min(-1)).all()
+    cache, table = tok.cached(k, v, rng, 64)
+    q = rng.standard_normal((n, H, D)).astype(np.float16)
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev([Lk]).int(), dev([0, n]).int(), n)
+    assert awq_b200.device_status() == 0
+    got = got.double().cpu().numpy()
+    for i in (0, n // 2, n - 1):
+        tok.check(q[i], got[i], Lk - n + i + 1, 2.0 ** -25, D ** -0.5)
+
+
 def ladder(rng, n, Hk, D, group, q0, drop, sizes):
     """Keys whose scores against q = q0 in channel 0 fall below token 0's by `drop` [n] bits, and
     values with codes 0 (a group's first channel) and 15, at the scales `sizes` [n]."""
@@ -575,8 +600,34 @@ def ladder(rng, n, Hk, D, group, q0, drop, sizes):
     return k.astype(np.float16), v.astype(np.float16)
 
 
+@pytest.mark.parametrize("D,group,H", [(128, 128, 7), (128, 32, 4), (64, 64, 8)])
+@pytest.mark.parametrize("ratio", [100, 250])
+def test_attention_prompt_one_token_weighs_most(cuda, D, group, H, ratio):
+    """One token that takes nearly all the weight, one beside it without weight whose value
+    scale is `ratio` times as large, and 4000 tokens 17 to 18 bits below the first: their sum
+    counts 0.1 of its scale, and none may be lost against the large scale.  160 requests over
+    the same pages, so that one CTA works through all tokens of the first."""
+    rng = np.random.default_rng(ratio + D)
+    R, n, Lk = 160, -(-256 // H), 4100
+    drop = rng.uniform(17.2, 18.2, Lk)
+    drop[0] = 0
+    sizes = np.full(Lk, 2.0 ** -6)
+    sizes[5] *= ratio
+    k, v = ladder(rng, Lk, 1, D, group, 8.0, drop, sizes)
+    tok = Tokens(k, v, group)
+    assert tok.top[0].max() == ratio * tok.top[0].min()
+    cache, table = tok.cached(k, v, rng, 64)
+    q = np.zeros((R * n, H, D), np.float16)
+    q[:, :, 0] = 8
+    got = awq_b200.kv4_attention(dev(q), cache, table.expand(R, -1).contiguous(), dev([Lk] * R).int(),
+                                 dev(n * np.arange(R + 1)).int(), n)
+    got = got.double().cpu().numpy()
+    for r, i in ((0, 0), (0, n - 1), (R - 1, n // 2)):
+        tok.check(q[0], got[r * n + i], Lk - n + i + 1, 2.0 ** -25, D ** -0.5)
+
+
 @pytest.mark.parametrize("D,group", [(64, 32), (128, 64), (128, 32)])
-@pytest.mark.parametrize("n,H", [(1, 1), (3, 4)])
+@pytest.mark.parametrize("n,H", [(1, 1), (3, 4), (37, 7)])
 def test_attention_groups_of_unequal_scale(cuda, D, group, n, H):
     """The first group's value scales are 2^22 times the others', and every eighth token weighs
     2^0.55 times the rest, so that a weight rounded to the fourth of itself would show.  Where
