@@ -396,6 +396,9 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
       // table does not name).
       auto tile = [&](auto edge, const uint8_t* st, int tok0, int ok) {
         constexpr bool EDGE = decltype(edge)::value;
+        auto unseen = [&](int b, int e, int c) {  // token g + 8 e of block b, column c
+          return tok0 + b * 16 + g + e * 8 > lim[c] || !((ok >> b) & 1);
+        };
         float x[TB][4];                         // [block][token g / g + 8, column]
         float ls[TB][2];                        // log2 of a token's largest value scale
 #pragma unroll
@@ -434,8 +437,7 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
           if constexpr (EDGE) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-              if (tok0 + b * 16 + g + (i / 2) * 8 > lim[i & 1] || !((ok >> b) & 1))
-                x[b][i] = -CUDART_INF_F;
+              if (unseen(b, i / 2, i & 1)) x[b][i] = -CUDART_INF_F;
           }
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -501,8 +503,9 @@ __global__ void __launch_bounds__(G_::THREADS, 1) kv4_attn_kernel(const AttnArgs
               float w[2];
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                // an unseen token's scale and minimum may be anything: no 0 * NaN
-                const bool seen = !EDGE || p[c] != 0.f;
+                // an unseen token's scale and minimum may be anything: no 0 * NaN (a seen
+                // one's weight may be 0 as well, and its NaN counts)
+                const bool seen = !EDGE || !unseen(b, e, c);
                 w[c] = seen ? p[c] * f.x : 0.f;
                 pm[k][c] = seen ? fmaf(p[c], mid, pm[k][c]) : pm[k][c];
               }

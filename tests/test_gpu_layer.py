@@ -647,3 +647,24 @@ def test_attention_groups_of_unequal_scale(cuda, D, group, n, H):
     got = got.double().cpu().numpy()
     for i in {0, n - 1}:
         tok.check(q[i], got[i], Lk - n + i + 1, 2.0 ** -32, D ** -0.5)
+
+
+@pytest.mark.parametrize("n", [1, 3, 200])
+@pytest.mark.parametrize("at", [3, 290])
+def test_attention_nan_value_of_no_weight(cuda, n, at):
+    """A seen token whose value is NaN makes its group NaN even where its weight is below
+    fp32's range (0 * NaN), in full tiles and in the last one."""
+    rng = np.random.default_rng(at)
+    Lk, D, group = 300 + n, 128, 64
+    k = np.zeros((Lk, 1, D), np.float16)
+    k[:, :, 0] = 8
+    k[at, :, 0] = -8                                     # 64 x 16 x 128^-0.5 = 90 nats: 130 bits
+    v = rng.standard_normal((Lk, 1, D)).astype(np.float16)
+    v[at, 0, 5] = np.nan
+    tok = Tokens(k, v, group)
+    cache, table = tok.cached(k, v, rng, 64)
+    q = np.zeros((n, 1, D), np.float16)
+    q[:, :, 0] = 64
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev([Lk]).int(), dev([0, n]).int(), n)
+    got = torch.isnan(got).cpu().numpy()
+    assert got[:, 0, :64].all() and not got[:, 0, 64:].any()
