@@ -220,9 +220,10 @@ AWQ_API int awq_kv4_gather(const void* cache, int64_t num_pages, int64_t kv_head
  * first one is taken first, and entries at or above *free_count are -1.  Output: slots
  * [max_tokens] and positions [max_tokens] of the new tokens, request after request (-1 and 0
  * behind the last), cu_q [requests + 1] (first token of each request), new_lens [requests].
- * *step_status: 0; n > 0 when the stack is n pages short; -1 when a length, held or count is
- * out of range (negative, more than max_blocks pages, more than max_tokens tokens).  A
- * refused step changes no state and gives slots -1, cu_q 0 and new_lens = kv_lens.
+ * *step_status: 0; n > 0 when the stack is n pages short (at most 2^31 - 1 is reported); -1
+ * when a length, held or count is out of range (negative, more than max_blocks pages, more
+ * than max_tokens tokens).  A refused step changes no state and gives slots -1, cu_q 0 and
+ * new_lens = kv_lens.
  */
 AWQ_API int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64_t max_blocks,
                                int32_t* held, int32_t* free_pages, int64_t free_capacity,

@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(THREADS) kv4_pages_kernel(const PagesArgs a) {
   const long long gone = total[0], need = total[1], tokens = total[2];
   int status = 0;
   if (s_bad || count < 0 || count + gone > a.capacity || tokens > a.max_tokens) status = -1;
-  else if (need > count + gone) status = (int)(need - count - gone);
+  else if (need > count + gone) status = (int)min(need - count - gone, 0x7fffffffLL);
   const bool ok = status == 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {

@@ -668,3 +668,20 @@ def test_attention_nan_value_of_no_weight(cuda, n, at):
     got = awq_b200.kv4_attention(dev(q), cache, table, dev([Lk]).int(), dev([0, n]).int(), n)
     got = torch.isnan(got).cpu().numpy()
     assert got[:, 0, :64].all() and not got[:, 0, 64:].any()
+
+
+@pytest.mark.parametrize("width,pages,want", [(1 << 18, 7, (1 << 31) - 7), (1 << 18, 0, (1 << 31) - 1),
+                                              ((1 << 18) + 1, 7, (1 << 31) - 1), (1 << 19, 0, (1 << 31) - 1)])
+def test_pages_step_shortage_beyond_32_bits(cuda, width, pages, want):
+    """8192 requests that need 2^18 pages or more each, which the table has room for: the
+    shortage is reported as 2^31 - 1 at most, 2^32 of it included."""
+    R = 8192
+    table = torch.empty((R, width), dtype=torch.int32, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    held, new = torch.zeros(R, **i32), torch.zeros(R, **i32)
+    lens = torch.full((R,), width, **i32)
+    free, count = torch.arange(7, **i32), torch.full((1,), pages, **i32)
+    slots, pos, cu, new_lens, status = awq_b200.kv4_pages_step(table, held, free, count, lens, new, 1, 4)
+    assert int(status) == want
+    assert int(count) == pages and (held == 0).all() and torch.equal(free, torch.arange(7, **i32))
+    assert (slots == -1).all() and (cu == 0).all() and torch.equal(new_lens, lens)
