@@ -163,7 +163,8 @@ AWQ_API int awq_gemm_f16_silu_mul(const void* x, int64_t ldx, const int32_t* qwe
  * No counterpart in the reference as such: it keeps an fp16 cache (inference/kv_cache.py),
  * rotates with one position per token (kernels/rope.py) and attends over fp16 keys and
  * values (kernels/flash_attention.py).  All entry points enqueue kernels on `stream`,
- * allocate nothing and do not synchronize; fp16 data, int32 lengths and pages.
+ * allocate nothing and do not synchronize; fp16 data, int32 lengths and pages; every pointer
+ * is aligned to its element type at least.
  *
  * awq_rope_axes: positions int64 or int32 [axes][tokens] (row stride axis_stride), inv_freq
  * fp32 [half], half = sum of sections[axes] (host array; 1 to 4 axes).  Frequency i turns

@@ -114,6 +114,12 @@ int awq_kv4_pages_step(int32_t* block_table, int64_t table_stride, int64_t max_b
       (requests && (!block_table || !held || !kv_lens || !new_tokens || !new_lens)) ||
       (max_tokens && (!slots || !positions)) || (free_capacity && !free_pages))
     return fail(AWQ_ERR_INVALID_ARG, "null pointer");
+  for (const void* p : {(const void*)block_table, (const void*)held, (const void*)free_pages,
+                        (const void*)free_count, (const void*)kv_lens, (const void*)new_tokens,
+                        (const void*)positions, (const void*)cu_q, (const void*)new_lens,
+                        (const void*)step_status})
+    if (!aligned(p, 4)) return fail(AWQ_ERR_INVALID_ARG, "an int32 pointer is not 4-byte aligned");
+  if (!aligned(slots, 8)) return fail(AWQ_ERR_INVALID_ARG, "slots must be 8-byte aligned");
   awq::Kv4PagesCall c = {};
   c.table = block_table, c.table_rs = table_stride, c.held = held;
   c.free_pages = free_pages, c.free_count = free_count;
@@ -165,6 +171,8 @@ int awq_kv4_attention(const void* q, int64_t q_token_stride, int64_t q_head_stri
   if (!aligned(out, 8) || out_token_stride % 4 || out_head_stride % 4)
     return fail(AWQ_ERR_INVALID_ARG, "out must be 8-byte aligned with strides that are multiples of 4 elements");
   if (!aligned(cache, 16)) return fail(AWQ_ERR_INVALID_ARG, "cache must be 16-byte aligned");
+  if (!aligned(block_table, 4) || !aligned(kv_lens, 4) || !aligned(cu_q, 4))
+    return fail(AWQ_ERR_INVALID_ARG, "block_table, kv_lens and cu_q must be 4-byte aligned");
   // the list of (request, kv head, row tile, 32-token tile) is counted in 32 bits
   const double tiles = (double)max_blocks * (double)page_size / 32 + 1;
   const double rows = (double)tokens * (double)(q_heads / kv_heads) / 8 + (double)requests;

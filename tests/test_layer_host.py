@@ -127,6 +127,15 @@ def test_pages_entry_refusals():
         assert _pages(**{name: None}) == INV, name
 
 
+def test_pages_and_attention_entries_refuse_misaligned_integers():
+    for name in ("table", "held", "free", "count", "lens", "new", "pos", "cu", "nl", "st"):
+        assert _pages(**{name: P + 2}) == INV, name
+    assert _pages(slots=P + 4) == INV
+    assert _attention(table=P + 2) == INV and _attention(lens=P + 1) == INV
+    assert _attention(cu=P + 2) == INV
+    assert "4-byte" in _lib.load().awq_last_error().decode()
+
+
 def _rope(q=P, H=2, k=P, Hk=1, T=3, D=64, pos=P, is64=1, inv=P, sections=(32,), out_q=P, out_k=P):
     import ctypes
     sec = (ctypes.c_int32 * max(1, len(sections)))(*sections)
