@@ -171,8 +171,8 @@ AWQ_API int awq_gemm_f16_silu_mul(const void* x, int64_t ldx, const int32_t* qwe
  * the channels (i, i + half) of every head of token t by positions[axis(i)][t] *
  * inv_freq[i].  axis(i): the section that holds i; with `interleaved`, a = i % axes while
  * i / axes < sections[a], else axis 0.  Channels from 2 half up are copied.  q or k may have
- * no heads.  out may be q or k itself with the same strides (in place); it must not overlap
- * the inputs in any other way.
+ * no heads.  out may be q or k itself with the same strides (in place); the outputs must not
+ * overlap the inputs in any other way, nor each other.
  */
 AWQ_API int awq_rope_axes(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                           int64_t q_heads, const void* k, int64_t k_token_stride,

@@ -173,6 +173,8 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
                     raise ValueError(f"{name} overlaps an input other than as that input itself")
         outs.append(o)
     oq, ok = outs
+    if _core()._overlap(oq, ok) and not _apart(oq, ok):
+        raise ValueError("out_q overlaps out_k")
     if T == 0:
         return oq, ok
     lib = _lib.load()

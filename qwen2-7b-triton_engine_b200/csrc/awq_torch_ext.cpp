@@ -364,6 +364,7 @@ std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Ten
                         " overlaps an input other than as that input itself");
     outs[i] = o;
   }
+  TORCH_CHECK_VALUE(!overlap(outs[0], outs[1]) || apart(outs[0], outs[1]), "out_q overlaps out_k");
   if (T == 0) return {outs[0], outs[1]};
   const c10::cuda::CUDAGuard guard(dev);
   check(awq_rope_axes(q.data_ptr(), q.stride(0), q.stride(1), q.size(1), k.data_ptr(), k.stride(0), k.stride(1),

@@ -36,6 +36,15 @@ def _status(cuda):
     yield
 
 
+@pytest.fixture(params=["extension", "ctypes"])
+def glue(request, monkeypatch):
+    """The C++ host glue, and the Python path that stands in for it where it is not built."""
+    if request.param == "ctypes":
+        monkeypatch.setattr(awq_b200, "_ext", None)
+    else:
+        assert awq_b200._ext is not None
+
+
 def dev(x, dtype=None):
     t = torch.as_tensor(np.asarray(x), device="cuda")
     return t if dtype is None else t.to(dtype)
@@ -86,6 +95,22 @@ def test_rope_unaligned_and_transposed(cuda):
     for q in (odd, heads):
         got = awq_b200.rope_axes(q, q[:, :2], pos[0], inv, (32,))
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_rope_refuses_outputs_that_share_memory(cuda, glue):
+    """out_q and out_k may be columns of the same rows, and nothing else in common."""
+    x = torch.randn((6, 5, 64), device="cuda").half()
+    q, k = x[:, :4], x[:, 4:]
+    pos, inv = torch.arange(6, device="cuda"), torch.ones(32, device="cuda")
+    buf = torch.zeros((7, 5, 64), dtype=torch.float16, device="cuda")
+    want = awq_b200.rope_axes(q, k, pos, inv, (32,))
+    got = awq_b200.rope_axes(q, k, pos, inv, (32,), out_q=buf[:6, :4], out_k=buf[:6, 4:])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = awq_b200.rope_axes(q, k, pos, inv, (32,), out_q=buf[:6, 1:], out_k=buf[:6, :1])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for oq, ok in ((buf[:6, :4], buf[:6, 3:4]), (buf[:6, :4], buf[1:, :1]), (buf[:6, 1:], buf[:6, 1:2])):
+        with pytest.raises(ValueError, match="out_q overlaps out_k"):
+            awq_b200.rope_axes(q, k, pos, inv, (32,), out_q=oq, out_k=ok)
 
 
 # ---- append and gather --------------------------------------------------------------------

@@ -151,6 +151,16 @@ def test_rope_entry_refusals():
     assert _rope(T=0) == 0 and _rope(H=0, Hk=0, q=None, k=None) == 0
 
 
+def test_rows_of_one_tensor_apart():
+    """What rope_axes asks of two views: their ranges meet, but they are different columns."""
+    from awq_b200 import layer
+    buf = torch.zeros((7, 5, 64), dtype=torch.float16)
+    for a, b, apart in ((buf[:6, :4], buf[:6, 4:], True), (buf[:6, 4:], buf[:6, :4], True),
+                        (buf[:6, :4], buf[1:, 4:], True), (buf[:6, :4], buf[:6, 3:4], False),
+                        (buf[:6, :4], buf[1:, :1], False), (buf[:6, 1:], buf[:6, 1:2], False)):
+        assert awq_b200._overlap(a, b) and layer._apart(a, b) is apart
+
+
 def _epilogue(act=0, res=P, ldr=64, bias=P, out=P, N=64):
     return _lib.load().awq_gemm_f16_epilogue(P, 64, P, P, P, bias, act, res, ldr, out, N, 2, N, 64, 64,
                                              None, 0, None)
