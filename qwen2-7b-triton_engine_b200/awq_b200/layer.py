@@ -165,8 +165,9 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
             o = torch.empty(x.shape, dtype=torch.float16, device=dev)
         else:
             _need(o, name, torch.float16, 3, dev)
-            if o.shape != x.shape or (D > 1 and o.stride(2) != 1):
-                raise ValueError(f"{name} must be {tuple(x.shape)} with a dense last dimension")
+            if o.shape != x.shape or (D > 1 and o.stride(2) != 1) or not _distinct(o):
+                raise ValueError(f"{name} must be {tuple(x.shape)} with a dense last dimension "
+                                 "and rows that share no element")
             same = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
             for y in (q, k):
                 if _core()._overlap(o, y) and not (same and y is x) and not _apart(o, y):
@@ -187,6 +188,14 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
             oq.data_ptr(), oq.stride(0), oq.stride(1), ok.data_ptr(), ok.stride(0), ok.stride(1),
             _core()._stream_handle(dev)))
     return oq, ok
+
+
+def _distinct(t: torch.Tensor) -> bool:
+    """Whether no two rows of t [T, H, D] (last dimension dense) share an element: heads within
+    tokens or tokens within heads, not expanded ones."""
+    (T, H, D), (ts, hs) = t.shape, t.stride()[:2]
+    return t.numel() == 0 or (H == 1 or hs >= D) and (T == 1 or ts >= (H - 1) * hs + D) \
+        or (T == 1 or ts >= D) and (H == 1 or hs >= (T - 1) * ts + D)
 
 
 def _apart(o: torch.Tensor, y: torch.Tensor) -> bool:
@@ -347,9 +356,9 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, block_table: torch.Tensor,
     else:
         _need(out, "out", torch.float16, 3, dev)
         if tuple(out.shape) != (T, H, D) or out.stride(2) != 1 or out.data_ptr() % 8 \
-                or out.stride(0) % 4 or out.stride(1) % 4:
+                or out.stride(0) % 4 or out.stride(1) % 4 or not _distinct(out):
             raise ValueError(f"out must be {(T, H, D)} with a dense last dimension, 8-byte "
-                             "aligned rows")
+                             "aligned rows that share no element")
         if _core()._overlap(out, q):
             raise ValueError("out overlaps q")
     if T == 0 or R == 0:

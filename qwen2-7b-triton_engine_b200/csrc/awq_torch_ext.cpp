@@ -230,6 +230,14 @@ bool apart(const at::Tensor& o, const at::Tensor& y) {
   return cols(o) <= d && d + cols(y) <= row;
 }
 
+// Whether no two rows of t [T, H, D] (last dimension dense) share an element: heads within tokens
+// or tokens within heads, not expanded ones.
+bool distinct(const at::Tensor& t) {
+  const int64_t T = t.size(0), H = t.size(1), D = t.size(2), ts = t.stride(0), hs = t.stride(1);
+  return t.numel() == 0 || ((H == 1 || hs >= D) && (T == 1 || ts >= (H - 1) * hs + D)) ||
+         ((T == 1 || ts >= D) && (H == 1 || hs >= (T - 1) * ts + D));
+}
+
 uintptr_t address(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()); }
 
 void check(int rc) {
@@ -356,8 +364,8 @@ std::tuple<at::Tensor, at::Tensor> rope_axes(at::Tensor q, at::Tensor k, at::Ten
     const char* name = i ? "out_k" : "out_q";
     const at::Tensor& o = **asked[i];
     need(o, name, at::kHalf, 3, &dev);
-    TORCH_CHECK_VALUE(o.sizes() == ins[i].sizes() && (D == 1 || o.stride(2) == 1), name, " must be ",
-                      ins[i].sizes(), " with a dense last dimension");
+    TORCH_CHECK_VALUE(o.sizes() == ins[i].sizes() && (D == 1 || o.stride(2) == 1) && distinct(o), name,
+                      " must be ", ins[i].sizes(), " with a dense last dimension and rows that share no element");
     const bool same = o.data_ptr() == ins[i].data_ptr() && o.strides() == ins[i].strides();
     for (int j = 0; j < 2; ++j)
       TORCH_CHECK_VALUE(!overlap(o, ins[j]) || (same && i == j) || apart(o, ins[j]), name,
@@ -479,8 +487,9 @@ at::Tensor kv4_attention(at::Tensor q, const at::Tensor& data, int64_t D, int64_
     out = *out_opt;
     need(out, "out", at::kHalf, 3, &dev);
     TORCH_CHECK_VALUE(out.sizes() == q.sizes() && out.stride(2) == 1 && address(out) % 8 == 0 &&
-                          out.stride(0) % 4 == 0 && out.stride(1) % 4 == 0,
-                      "out must be ", q.sizes(), " with a dense last dimension, 8-byte aligned rows");
+                          out.stride(0) % 4 == 0 && out.stride(1) % 4 == 0 && distinct(out),
+                      "out must be ", q.sizes(),
+                      " with a dense last dimension, 8-byte aligned rows that share no element");
     TORCH_CHECK_VALUE(!overlap(out, q), "out overlaps q");
   } else {
     out = ragged ? at::zeros(q.sizes(), q.options()) : at::empty(q.sizes(), q.options());

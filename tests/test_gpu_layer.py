@@ -113,6 +113,26 @@ def test_rope_refuses_outputs_that_share_memory(cuda, glue):
             awq_b200.rope_axes(q, k, pos, inv, (32,), out_q=oq, out_k=ok)
 
 
+def test_outputs_whose_rows_share_memory_are_refused(cuda, glue):
+    """An expanded output has one row for many; any order of tokens and heads is fine."""
+    x = torch.randn((6, 4, 64), device="cuda").half()
+    pos, inv = torch.arange(6, device="cuda"), torch.ones(32, device="cuda")
+    want = awq_b200.rope_axes(x, x, pos, inv, (32,))[0]
+    heads = torch.zeros((4, 6, 64), dtype=torch.float16, device="cuda").transpose(0, 1)
+    assert torch.equal(awq_b200.rope_axes(x, x, pos, inv, (32,), out_k=heads)[1], want)
+    cache = awq_b200.KV4Cache.allocate(6, 2, 64, 16)
+    awq_b200.kv4_append(x[:, :2], x[:, 2:], torch.arange(6, device="cuda") * 16, cache)
+    table = torch.arange(6, dtype=torch.int32, device="cuda")[:, None]
+    lens = torch.ones(6, dtype=torch.int32, device="cuda")
+    want = awq_b200.kv4_attention(x, cache, table, lens)
+    assert torch.equal(awq_b200.kv4_attention(x, cache, table, lens, out=heads), want)
+    for o in (heads[:1].expand(6, 4, 64), heads[:, :1].expand(6, 4, 64)):
+        with pytest.raises(ValueError, match="share no element"):
+            awq_b200.rope_axes(x, x, pos, inv, (32,), out_q=o)
+        with pytest.raises(ValueError, match="share no element"):
+            awq_b200.kv4_attention(x, cache, table, lens, out=o)
+
+
 # ---- append and gather --------------------------------------------------------------------
 def sample(rng, T, H, D):
     """Rows with wide, narrow, constant, subnormal and large groups."""

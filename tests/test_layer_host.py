@@ -161,6 +161,18 @@ def test_rows_of_one_tensor_apart():
         assert awq_b200._overlap(a, b) and layer._apart(a, b) is apart
 
 
+def test_rows_that_share_no_element():
+    """What rope_axes and kv4_attention ask of a given output."""
+    from awq_b200 import layer
+    buf = torch.zeros((6, 4, 64), dtype=torch.float16)
+    for t in (buf, buf[:, 1:3], buf[::2], buf[:, ::2], buf[..., :32], buf[:1], buf[:, :1], buf[:0],
+              buf.view(4, 6, 64).transpose(0, 1), buf[:1].expand(1, 4, 64)):
+        assert layer._distinct(t), t.stride()
+    for t in (buf[:1].expand(6, 4, 64), buf[:, :1].expand(6, 4, 64),
+              buf.as_strided((6, 4, 64), (128, 64, 1)), buf.as_strided((6, 4, 64), (256, 32, 1))):
+        assert not layer._distinct(t), t.stride()
+
+
 def _epilogue(act=0, res=P, ldr=64, bias=P, out=P, N=64):
     return _lib.load().awq_gemm_f16_epilogue(P, 64, P, P, P, bias, act, res, ldr, out, N, 2, N, 64, 64,
                                              None, 0, None)
