@@ -379,12 +379,11 @@ class AttentionLinearsTP:
                              f"rank has {g1 - g0} of {s.head_dim}")
         if x.dim() != 2:
             raise ValueError(f"x must be [tokens, hidden], got {tuple(x.shape)}")
-        T = x.shape[0]
         q, k, v = (t.unflatten(-1, (-1, s.head_dim)) for t in self.project_qkv(x))
         awq_b200.rope_axes(q, k, positions, inv_freq, sections, interleaved, out_q=q, out_k=k)
         awq_b200.kv4_append(k, v, slots, cache)
         attn = awq_b200.kv4_attention(q, cache, block_table, kv_lens, cu_q, max_q)
-        return self.o(attn.view(T, -1), residual)
+        return self.o(attn.flatten(1), residual)
 
 
 class TensorParallelMLP:

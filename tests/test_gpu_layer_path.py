@@ -164,3 +164,15 @@ def test_attend_refusals(cuda, layer):
     odd = tp.AttentionLinearsTP(weights(HID, (H + 2 * HK) * D, 1), weights(H * D, HID, 2), H, HK, D, 3, 1)
     with pytest.raises(ValueError, match="whole groups"):
         odd.attend(x, st.cache, slots, st.table, lens, pos, layer[2], (D // 2,))
+
+
+def test_step_without_tokens(cuda, layer):
+    """A step of requests that all pause: no rows, no pages, no change."""
+    st = State(2, 4, 4)
+    before = st.cache.data.clone()
+    y, z, slots, pos, cu, lens, status = run(layer, st, torch.zeros((0, HID), dtype=torch.float16,
+                                                                    device="cuda"), 0, 1)
+    assert y.shape == z.shape == (0, HID) and slots.shape == pos.shape == (0,)
+    assert int(status) == 0 and cu.tolist() == [0, 0, 0] and lens.tolist() == [0, 0]
+    assert torch.equal(st.cache.data, before) and int(st.count) == 4
+    assert awq_b200.device_status() == 0
