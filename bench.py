@@ -804,12 +804,14 @@ def stack_bench(torch, awq_b200, dev, world, rank, comm, args):
         table = torch.full((1, blocks), -1, **i32)
         held, kv_lens = torch.zeros(1, **i32), torch.zeros(1, **i32)
         free, count = torch.arange(blocks, **i32), torch.full((1,), blocks, **i32)
+        refused = torch.zeros(1, **i32)                     # steps that got no pages
         inv_freq = (1e6 ** (-torch.arange(64, dtype=torch.float64, device=dev) / 64)).float()
 
         def forward(h):                                     # noqa: F811
             T = h.shape[0]
-            slots, pos, cu, lens, _ = awq_b200.kv4_pages_step(
+            slots, pos, cu, lens, status = awq_b200.kv4_pages_step(
                 table, held, free, count, kv_lens, torch.full((1,), T, **i32), page, T)
+            refused.add_(status != 0)
             for (attn, mlp, n1, n2), cache in zip(layers, caches):
                 h = attn.attend(rms(h, n1), cache, slots, table, lens, pos, inv_freq, (64,),
                                 cu_q=cu if T > 1 else None, max_q=T, residual=h)
@@ -849,6 +851,9 @@ def stack_bench(torch, awq_b200, dev, world, rank, comm, args):
         torch.cuda.synchronize(dev)
     decode_ms = _max_over_ranks(torch, dev, world, e0.elapsed_time(e1) / args.decode)
     st = awq_b200.device_status()
+    if args.attention and int(refused):
+        raise RuntimeError(f"{int(refused)} steps of the stack were refused by kv4_pages_step: not a "
+                           "measurement")
     del g
     layers.clear()
     torch.cuda.empty_cache()
