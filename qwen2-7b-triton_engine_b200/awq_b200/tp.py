@@ -238,10 +238,15 @@ class RowParallelAWQ:
 
     def __call__(self, x_local: torch.Tensor,
                  residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x_local holds this rank's K columns [k0, k1) of the activation.  ``residual`` (the
-        full output's shape, the same on every rank) is added to the sum: in the product's
+        """x_local holds this rank's K columns [k0, k1) of the activation.  ``residual`` (fp16,
+        the full output's shape, the same on every rank) is added to the sum: in the product's
         epilogue on one GPU, after the all-reduce on several."""
         if residual is not None:
+            shape = (*x_local.shape[:-1], self.w.scales.shape[1])
+            if residual.dtype != torch.float16:
+                raise TypeError(f"residual must be float16, got {residual.dtype}")
+            if tuple(residual.shape) != shape:
+                raise ValueError(f"residual must be {shape}, got {tuple(residual.shape)}")
             if self.epilogue is not None and self.k1 > self.k0:
                 w = self.w
                 return self.epilogue(x_local, w.qweight, w.qzeros, w.scales, w.group_size,

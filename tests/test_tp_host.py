@@ -311,3 +311,54 @@ def test_row_parallel_fused_choice_agrees_across_ranks(world, K, want, want64):
     if not want:
         # at least one rank would have chosen the fused kernel on its own K alone
         assert any(g[2] for g in got) or any(g[1] == 0 for g in got)
+
+
+# ---- residual= over several ranks: added once, behind the sum ----
+def _residual_worker(rank, world, port, seed, q):
+    os.environ["MASTER_ADDR"] = "127.0.0.1"
+    os.environ["MASTER_PORT"] = str(port)
+    import datetime
+    dist.init_process_group("gloo", rank=rank, world_size=world,
+                            timeout=datetime.timedelta(seconds=30))
+    try:
+        from awq_b200 import tp
+        hidden, inter = 384, 512
+        bias = torch.from_numpy(O.make_x(1, hidden, seed=seed + 5))[0]
+        ro = tp.RowParallelAWQ(tp.AWQWeights(*_layer(hidden, hidden, seed), 128, bias), world, rank,
+                               gemm=_cpu_gemm)
+        mlp = tp.TensorParallelMLP(tp.AWQWeights(*_layer(hidden, 2 * inter, seed + 1)),
+                                   tp.AWQWeights(*_layer(inter, hidden, seed + 2)), inter, world, rank,
+                                   gemm=_cpu_gemm)
+        x = torch.from_numpy(O.make_x(6, hidden, seed=seed + 3)).view(2, 3, hidden)
+        res = torch.from_numpy(O.make_x(6, hidden, seed=seed + 4)).view(2, 3, hidden)
+        xl = x[..., ro.k0:ro.k1].contiguous()
+        refused = 0
+        for bad in (res[:1], res[:, :1], res[0, 0], res.float()):
+            for f, a in ((ro, xl), (mlp, x)):
+                try:
+                    f(a, bad)
+                except (TypeError, ValueError):
+                    refused += 1
+        q.put((rank, refused, ro(xl).numpy(), ro(xl, res).numpy(), ro(xl, residual=res).numpy(),
+               mlp(x).numpy(), mlp(x, res).numpy(), res.numpy()))
+    finally:
+        dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("world", [1, 2, 4])          # 4: the last rank holds no rows of o
+def test_residual_gloo(world):
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    port = _free_port()
+    procs = [ctx.Process(target=_residual_worker, args=(r, world, port, 71, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    got = [q.get(timeout=120) for _ in range(world)]
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    import numpy as np
+    for rank, refused, y, yr, yk, m, mr, res in got:
+        assert refused == 8, rank
+        assert np.array_equal(yr, y + res) and np.array_equal(yk, yr) and np.array_equal(mr, m + res)
+        assert np.array_equal(yr, got[0][3]) and np.array_equal(mr, got[0][6])
