@@ -180,3 +180,21 @@ def test_residual_where_the_generic_kernel_takes_several_launches(cuda):
     awq_b200.gemm_epilogue(xd, qwd, qzd, sd, gs, residual=rd, out=rd)
     assert torch.equal(rd, want)
     assert awq_b200.device_status() == 0
+
+
+def test_activation_of_infinite_sums(cuda):
+    """+-inf through every activation as its formula gives them: y / (1 + exp(-y)) and the gelu
+    forms are inf at inf and -inf / inf or -inf * 0 = NaN at -inf."""
+    inf, nan = np.inf, np.nan
+    want = {"none": (inf, -inf), "relu": (inf, 0.0), "silu": (inf, nan), "gelu": (inf, nan),
+            "gelu_tanh": (inf, nan)}
+    for M, K, N in ((1, 64, 64), (12, 64, 64), (100, 64, 64), (300, 64, 512), (20, 64, 40)):
+        qw, qz, s = O.make_awq_layer(K, N, 64, seed=4)
+        x = np.zeros((M, K), np.float16)
+        bias = np.resize(np.array([inf, -inf, 1.0], np.float16), N)
+        xd, qwd, qzd, sd, bd = dev(x, qw, qz, s, bias)
+        for act, (plus, minus) in want.items():
+            got = awq_b200.gemm_epilogue(xd, qwd, qzd, sd, 64, bias=bd, activation=act).float().cpu().numpy()
+            for at, ref in ((bias == inf, plus), (bias == -inf, minus)):
+                assert np.array_equal(got[:, at], np.full((M, at.sum()), ref, np.float32), equal_nan=True), act
+            assert np.isfinite(got[:, bias == 1]).all()

@@ -730,3 +730,21 @@ def test_pages_step_shortage_beyond_32_bits(cuda, width, pages, want):
     assert int(status) == want
     assert int(count) == pages and (held == 0).all() and torch.equal(free, torch.arange(7, **i32))
     assert (slots == -1).all() and (cu == 0).all() and torch.equal(new_lens, lens)
+
+
+@pytest.mark.parametrize("D,group,H,Hk", [(128, 128, 7, 1), (128, 32, 7, 1), (64, 64, 2, 1)])
+@pytest.mark.parametrize("n", [1, 5, 150])
+def test_attention_long_context(cuda, D, group, H, Hk, n):
+    """20000 cached tokens, values of one size: sums of many small weights, on both kernels."""
+    rng = np.random.default_rng(n + D)
+    Lk = 20000
+    k = (rng.standard_normal((Lk, Hk, D)) + 4 * (rng.random((1, Hk, D)) < 0.05)).astype(np.float16)
+    v = (0.7 * rng.standard_normal((Lk, Hk, D))).astype(np.float16)
+    tok = Tokens(k, v, group)
+    cache, table = tok.cached(k, v, rng, 64)
+    q = rng.standard_normal((n, H, D)).astype(np.float16)
+    got = awq_b200.kv4_attention(dev(q), cache, table, dev([Lk]).int(), dev([0, n]).int(), n)
+    assert awq_b200.device_status() == 0
+    got = got.double().cpu().numpy()
+    for i in {0, n - 1}:
+        tok.check(q[i], got[i], Lk - n + i + 1, 2.0 ** -25, D ** -0.5)
