@@ -748,3 +748,29 @@ def test_attention_long_context(cuda, D, group, H, Hk, n):
     got = got.double().cpu().numpy()
     for i in {0, n - 1}:
         tok.check(q[i], got[i], Lk - n + i + 1, 2.0 ** -25, D ** -0.5)
+
+
+@pytest.mark.parametrize("n", [2, 60])
+def test_cache_beyond_32_bits(cuda, n):
+    """A cache of 9.7 GB whose requests lie on both sides of 2^32 bytes and at its end."""
+    rng = np.random.default_rng(n)
+    D, group, Hk, H, page, Lk = 128, 128, 2, 8, 64, 130
+    pages = 9_700_000_000 // (Hk * page * (D + 8))
+    cache = awq_b200.KV4Cache.allocate(pages, Hk, D, page, group)
+    cache.data.fill_(0xFF)
+    half = 2 ** 32 // (Hk * page * (D + 8))
+    table = np.array([[half - 1, half, half + 1], [pages - 1, 0, pages - 2]])
+    k, v = (rng.standard_normal((2, Lk, Hk, D)).astype(np.float16) for _ in range(2))
+    slots = table[:, np.arange(Lk) // page] * page + np.arange(Lk) % page
+    awq_b200.kv4_append(dev(k).flatten(0, 1), dev(v).flatten(0, 1), dev(slots).flatten(), cache)
+    q = rng.standard_normal((2 * n, H, D)).astype(np.float16)
+    got = awq_b200.kv4_attention(dev(q), cache, dev(table).int(), dev([Lk, Lk]).int(),
+                                 dev([0, n, 2 * n]).int(), n).double().cpu().numpy()
+    gk, gv = (x.double().cpu().numpy() for x in awq_b200.kv4_gather(cache, dev(slots[1])))
+    for r in range(2):
+        tok = Tokens(k[r], v[r], group)
+        for i in {0, n - 1}:
+            tok.check(q[r * n + i], got[r * n + i], Lk - n + i + 1, 2.0 ** -25, D ** -0.5)
+    for a, ref in ((gk, tok.K), (gv, tok.V)):
+        assert (np.abs(a - ref) <= (U16 + U32) * np.abs(ref) + TINY).all()
+    assert awq_b200.device_status() == 0
