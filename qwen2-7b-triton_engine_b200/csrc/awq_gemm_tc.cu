@@ -131,7 +131,9 @@ struct TcArgs {
 
 // A call of its own, its array in local memory: inlined, the activations' temporaries made
 // the kernel spill in its main loop (K = 18944, N = 3584, M = 2048: 307 us, against 219
-// for the product alone).
+// for the product alone).  It is not cheap: M = 2048 with a residual, none / relu / gelu_tanh,
+// takes 215 / 248 / 274 us at K = 18944, N = 3584 and 225 / 423 / 440 at K = 3584, N = 18944,
+// more than a kernel over the product's output would add there.
 __device__ __noinline__ void activate32(float* v, int act) {
 #pragma unroll 1
   for (int j = 0; j < 32; ++j) v[j] = activate(v[j], act);

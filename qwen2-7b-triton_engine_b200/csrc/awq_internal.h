@@ -48,8 +48,10 @@ constexpr int kMaxCounters = 16384;
 constexpr size_t kCounterRegionBytes = kMaxCounters * sizeof(int);
 
 // Epilogue behind the bias: out = fp16(act(sum + bias) + residual), in fp32 up to the one
-// rounding.  residual fp16 [M, N] with row stride ldr (may be out itself: every kernel reads
-// an element's residual in the thread that then writes it), or null.
+// rounding.  residual fp16 [M, N] with row stride ldr, or null.  It may be out itself: an
+// element's residual is read by the thread that then writes it, and in the prefill kernel,
+// which stages its rows in shared memory, by the warp that then writes it (all reads of a
+// staged chunk come before its stores, with a warp barrier between).
 enum Activation : int { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActGeluTanh = 4 };
 struct EpiArgs {
   const void* residual = nullptr;
@@ -229,8 +231,9 @@ struct Kv4AttnCall {
 // tcgen05 kernel), 28 / 4 heads: 8 requests of 4096 tokens, 112 rows 61 / 56, 168 rows 83 / 62,
 // 224 rows 106 / 63, 448 rows 193 / 94; of 512 tokens, 168 rows 33 / 37, 224 rows 37 / 39, 448
 // rows 62 / 45; one request of 4096 tokens, 224 rows 27 / 45, 448 rows 38 / 46, 896 rows 60 / 48.
-// The kernels cross between 112 rows, where the SMs are full, and 500, where they are not; the
-// cached lengths that tell the two apart are on the device.
+// The kernels cross between 112 rows, where the SMs are full (32 pairs of request and kv head),
+// and 500, where they are not (4 pairs): one threshold for both, so that a lone request with a
+// chunk of 32 to 64 tokens takes up to 1.7 times the other kernel's time.
 constexpr int kKv4PrefillMinRows = 192, kKv4PrefillRows = 256;
 size_t kv4_attention_workspace(int head_dim, int64_t max_rows, int num_sms);
 cudaError_t launch_kv4_attention(const Kv4AttnCall& c, int num_sms, int* dev_status,

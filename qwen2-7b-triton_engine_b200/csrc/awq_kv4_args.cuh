@@ -14,9 +14,10 @@ namespace kv4 {
 constexpr int kPrefixEntries = 1024;     // prefix sums held in shared memory
 constexpr int kDescInts = 8;             // per CTA: the item that starts there and goes on
 // The softmax reference M lies this many powers of two below the largest p s seen when it was
-// set, and moves when one passes 2^8 of that: fp16 weights reach 2^15, half of fp16's limit,
-// and lose bits from 2^-21 and vanish from 2^-32 of the largest on only.
-constexpr float kBelowTop = 7.0f, kMoveAt = 8.0f;
+// set (or below a bound on it, in a step whose value scales lie close together), and moves when
+// one passes 2^15 of M: fp16 weights reach 2^15, half of fp16's limit, and lose bits from 2^-21
+// and vanish from 2^-32 of the largest on only.
+constexpr float kBelowTop = 7.0f, kMoveAt = 8.0f;   // a new reference 2^kMoveAt above M replaces it
 
 struct AttnArgs {
   const uint8_t* cache;

@@ -23,14 +23,16 @@
 // cross CTAs are joined by kv4_prefill_merge in CTA order.
 //
 // Bound: the softmax warps' latency.  Measured on B200, four requests of 1 to 1024 query tokens
-// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 344 us, 0.52 PFLOP/s; a step of 256
+// and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 346 us, 0.52 PFLOP/s; a step of 256
 // rows x 128 tokens takes 3.4 us, of which the MMAs need 1.1, the exponentials 1.1 and the
 // operand traffic in shared memory 1.4; no pipe is busier than 44 % (shared memory).  A tile waits a third of
 // the time for its S, which shares tensor memory with its P: 512 columns hold two tiles of S
 // and O, and no third S.  Measured and not kept (same case, 380 us then): scales and minima as
 // fp16 pairs in shared memory 463 us, all eight softmax warps on one tile after the other 417,
 // S in two buffers of 64 tokens 399, half of the exponentials as polynomials 479, x kept in
-// registers between the two passes 392 (184 registers) to 422.
+// registers between the two passes 392 (184 registers) to 422.  The compiler holds the kernel at
+// the launch's 128 registers a thread and spills 200 to 560 bytes a thread of its forms (128
+// channels in groups of 128: 560); where, and what that costs, is not measured.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <math_constants.h>

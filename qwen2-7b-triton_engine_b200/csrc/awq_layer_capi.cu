@@ -1,7 +1,7 @@
 // awq_layer_capi.cu -- extern "C" entry points of the operators between a layer's products:
 // rotary positions, the paged 4-bit key/value cache and attention over it (declared in
-// include/awq_b200.h).  Validation only; the kernels are in awq_rope.cu, awq_kv4_cache.cu
-// and awq_kv4_attn.cu.
+// include/awq_b200.h).  Validation only; the kernels are in awq_rope.cu, awq_kv4_cache.cu,
+// awq_kv4_attn.cu and awq_kv4_prefill.cu.
 #include <cuda_runtime.h>
 
 #include <cmath>
