@@ -150,7 +150,9 @@ def workspace_for(device: torch.device, nbytes: int, stream=None) -> torch.Tenso
 
     The kernels leave its arrival counters at zero after every call, so it is
     zeroed once per allocation only.  One workspace per stream keeps concurrent
-    streams from sharing counters.
+    streams from sharing counters.  A graph that captures calls on it needs the tensor kept
+    alive (a larger request replaces it) and must not replay beside other users of it; this
+    package's own calls take a workspace of the graph's instead.
     """
     if stream is None:
         stream = torch.cuda.current_stream(device)
@@ -162,6 +164,19 @@ def workspace_for(device: torch.device, nbytes: int, stream=None) -> torch.Tenso
             ws = torch.zeros(size, dtype=torch.uint8, device=device)
             _workspaces[key] = ws
         return ws
+
+
+def _call_workspace(lib, dev: torch.device, need: int, stream) -> torch.Tensor:
+    """The workspace of one call on ``stream`` (the current one): the stream's, or while it
+    captures a graph one in that graph's own memory, whose counters the graph zeroes, so that
+    graphs may replay beside one another and beside other calls."""
+    if _ext is not None:
+        return _ext.workspace(dev.index, stream.cuda_stream, need)
+    if not torch.cuda.is_current_stream_capturing():
+        return workspace_for(dev, need, stream)
+    ws = torch.empty(max(need, _lib.WS_COUNTER_BYTES), dtype=torch.uint8, device=dev)
+    _lib.check(lib.awq_workspace_init(ws.data_ptr(), _lib.WS_COUNTER_BYTES, stream.cuda_stream))
+    return ws
 
 
 # Per-call host work that only depends on the weights' metadata or the shape is cached:
@@ -268,7 +283,7 @@ def gemm(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor, scales:
     with _DeviceGuard(dev):
         stream = torch.cuda.current_stream(dev)
         need = _workspace_need(lib, dev, M, N, K, gs)
-        ws = workspace_for(dev, need, stream) if need else None
+        ws = _call_workspace(lib, dev, need, stream) if need else None
         if bias is None:
             _lib.check(lib.awq_gemm_f16_ex(
                 x2d.data_ptr(), x2d.stride(0), qweight.data_ptr(), qzeros.data_ptr(),
@@ -292,8 +307,8 @@ def gemm_epilogue(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor
     bias fp16 [N], activation None / "none", "relu", "silu", "gelu" or "gelu_tanh", residual
     fp16 [M, N] (rows may be strided); fp32 up to the one rounding.  ``out`` may be
     ``residual`` (the residual stream updated in place); otherwise it must overlap no input.
-    Outside graph capture the split-K workspace is the one of the current stream; a captured
-    call gets its own, so that graphs may replay at the same time."""
+    Outside graph capture the split-K workspace is the one of the current stream; captured
+    calls get one of their graph's, so that graphs may replay at the same time."""
     if _ext is not None and all(t is None or isinstance(t, torch.Tensor)
                                 for t in (x2d, qweight, qzeros, scales, bias, residual, out)):
         return _ext.gemm_epilogue(x2d, qweight, qzeros, scales, int(group_size), bias, activation,
@@ -352,14 +367,7 @@ def gemm_epilogue(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor
     with _DeviceGuard(dev):
         stream = torch.cuda.current_stream(dev)
         need = _workspace_need(lib, dev, M, N, K, gs)
-        ws = None
-        if need and torch.cuda.is_current_stream_capturing():
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            # only the arrival counters at its head must start at zero
-            _lib.check(lib.awq_workspace_init(ws.data_ptr(), min(need, _lib.WS_COUNTER_BYTES),
-                                              stream.cuda_stream))
-        elif need:
-            ws = workspace_for(dev, need, stream)
+        ws = _call_workspace(lib, dev, need, stream) if need else None
         _lib.check(lib.awq_gemm_f16_epilogue(
             x2d.data_ptr(), max(x2d.stride(0), K), qweight.data_ptr(), qzeros.data_ptr(),
             scales.data_ptr(), bias.data_ptr() if bias is not None else None, act,
@@ -404,7 +412,7 @@ def gemm_silu_mul(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tensor
     with _DeviceGuard(dev):
         stream = torch.cuda.current_stream(dev)
         need = _workspace_need(lib, dev, M, N, K, gs, silu_mul=True)
-        ws = workspace_for(dev, need, stream)
+        ws = _call_workspace(lib, dev, need, stream)
         _lib.check(lib.awq_gemm_f16_silu_mul(
             x2d.data_ptr(), x2d.stride(0), qweight.data_ptr(), qzeros.data_ptr(),
             scales.data_ptr(), out.data_ptr(), out.stride(0), M, N, K, gs, ws.data_ptr(),
@@ -559,7 +567,7 @@ def gemm_allreduce(x2d: torch.Tensor, qweight: torch.Tensor, qzeros: torch.Tenso
     lib = _lib.load()
     with _DeviceGuard(dev):
         need = lib.awq_gemm_workspace_bytes(M, N, K, int(group_size))
-        ws = workspace_for(dev, need) if need else None
+        ws = _call_workspace(lib, dev, need, torch.cuda.current_stream(dev)) if need else None
         _lib.check(lib.awq_gemm_f16_allreduce(
             comm._ptr, x2d.data_ptr(), x2d.stride(0), qweight.data_ptr(), qzeros.data_ptr(),
             scales.data_ptr(), out.data_ptr(), out.stride(0), M, N, K, int(group_size),

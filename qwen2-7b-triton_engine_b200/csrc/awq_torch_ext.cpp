@@ -81,9 +81,18 @@ std::pair<int64_t, int64_t> check_weights(const at::Tensor& qw, const at::Tensor
 }
 
 // Zero-initialised split-K workspace per (device, stream), grown on demand.  The kernels
-// leave its counters at zero after every call, so it is zeroed once per allocation.
+// leave its counters at zero after every call, so it is zeroed once per allocation.  The calls
+// that a stream records into one graph share a workspace of that graph's own memory, whose
+// counters the graph zeroes: graphs may replay beside one another and beside other calls, and
+// none is left with memory that a later, larger call has given back.
 std::mutex g_mu;
 std::map<std::pair<int, cudaStream_t>, at::Tensor> g_ws;
+struct CaptureWorkspace {
+  unsigned long long id = 0;      // of the capture
+  at::Tensor ws;
+};
+std::map<std::pair<int, cudaStream_t>, CaptureWorkspace> g_capture_ws;
+constexpr size_t kCounterBytes = 64 * 1024;   // head of a workspace that must start at zero
 std::map<std::tuple<int, int64_t, int64_t, int64_t, int64_t, bool>, size_t> g_need;
 
 size_t workspace_need(int dev, int64_t M, int64_t N, int64_t K, int64_t gs, bool silu) {
@@ -102,12 +111,29 @@ size_t workspace_need(int dev, int64_t M, int64_t N, int64_t K, int64_t gs, bool
 }
 
 at::Tensor workspace_for(const at::Device& dev, cudaStream_t st, size_t need) {
-  std::lock_guard<std::mutex> lk(g_mu);
-  at::Tensor& ws = g_ws[{dev.index(), st}];
-  if (!ws.defined() || (size_t)ws.numel() < need) {
-    const int64_t size = need > (size_t)(1 << 20) ? (int64_t)need : (int64_t)(1 << 20);
-    ws = at::zeros({size}, at::TensorOptions().dtype(at::kByte).device(dev));
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(st, &cap, &id) != cudaSuccess) {
+    (void)cudaGetLastError();      // the launch that follows reports what is wrong
+    cap = cudaStreamCaptureStatusNone;
   }
+  const int64_t size = need > (size_t)(1 << 20) ? (int64_t)need : (int64_t)(1 << 20);
+  const auto options = at::TensorOptions().dtype(at::kByte).device(dev);
+  const std::pair<int, cudaStream_t> key(dev.index(), st);
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (cap == cudaStreamCaptureStatusActive) {
+    CaptureWorkspace& c = g_capture_ws[key];
+    if (!c.ws.defined() || c.id != id || (size_t)c.ws.numel() < need) {
+      at::Tensor ws = at::empty({size}, options);
+      if (const int rc = awq_workspace_init(ws.data_ptr(), kCounterBytes, st)) raise_awq(rc);
+      c.ws = ws;
+      c.id = id;
+    }
+    return c.ws;
+  }
+  if (!g_capture_ws.empty()) g_capture_ws.erase(key);
+  at::Tensor& ws = g_ws[key];
+  if (!ws.defined() || (size_t)ws.numel() < need) ws = at::zeros({size}, options);
   return ws;
 }
 
@@ -305,18 +331,7 @@ at::Tensor gemm_epilogue(at::Tensor x, at::Tensor qw, at::Tensor qz, at::Tensor 
   cudaStream_t st = at::cuda::getCurrentCUDAStream(dev.index()).stream();
   const size_t nb = workspace_need(dev.index(), M, N, K, gs, false);
   at::Tensor ws;
-  if (nb) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    TORCH_CHECK(cudaStreamIsCapturing(st, &cap) == cudaSuccess, "cudaStreamIsCapturing failed");
-    if (cap == cudaStreamCaptureStatusNone) {
-      ws = workspace_for(dev, st, nb);
-    } else {
-      // a captured call has a workspace of its own: graphs may replay at the same time; only
-      // the arrival counters at its head must start at zero
-      ws = at::empty({(int64_t)nb}, x.options().dtype(at::kByte));
-      check(awq_workspace_init(ws.data_ptr(), nb < 65536 ? nb : 65536, st));
-    }
-  }
+  if (nb) ws = workspace_for(dev, st, nb);
   check(awq_gemm_f16_epilogue(x.data_ptr(), std::max(x.stride(0), K), qw.data_ptr<int32_t>(),
                               qz.data_ptr<int32_t>(), s.data_ptr(), bias.defined() ? bias.data_ptr() : nullptr,
                               act, res.defined() ? res.data_ptr() : nullptr,
@@ -536,6 +551,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                const at::Tensor& s, int64_t gs) {
           return forward_impl(x, qw, qz, s, gs, c10::nullopt, true);
         });
+  m.def("workspace", [](int64_t device, int64_t stream, int64_t need) {   // of a call on that stream
+    return workspace_for(at::Device(at::kCUDA, (c10::DeviceIndex)device),
+                         reinterpret_cast<cudaStream_t>(stream), (size_t)need);
+  });
   m.def("gemm_epilogue", &gemm_epilogue);
   m.def("rope_axes", &rope_axes);
   m.def("kv4_pages_step", &kv4_pages_step);
