@@ -25,7 +25,7 @@
 // Bound: the softmax warps' latency.  Measured on B200, four requests of 1 to 1024 query tokens
 // and 777 to 8192 cached ones, 28 / 4 heads of 128 channels: 346 us, 0.52 PFLOP/s; a step of 256
 // rows x 128 tokens takes 3.4 us, of which the MMAs need 1.1, the exponentials 1.1 and the
-// operand traffic in shared memory 1.4; no pipe is busier than 44 % (shared memory).  A tile waits a third of
+// operand traffic in shared memory 1.4; no pipe is busier than 43 % (shared memory).  A tile waits a third of
 // the time for its S, which shares tensor memory with its P: 512 columns hold two tiles of S
 // and O, and no third S.  Measured and not kept (same case, 380 us then): scales and minima as
 // fp16 pairs in shared memory 463 us, all eight softmax warps on one tile after the other 417,
